@@ -41,6 +41,7 @@ extern "C" {
 #define TANS_B200_DATA_BAD_STATE 2   /* initial state outside [L, 2L)       */
 #define TANS_B200_DATA_BAD_TABLE 4   /* spread/freqs/table entry malformed  */
 #define TANS_B200_DATA_TIMEOUT 8     /* a bounded in-kernel wait ran out    */
+#define TANS_B200_DATA_BAD_INDEX 16  /* slot, page, position or length out of range */
 
 /* Table size L = M (tans_codec.py:24-25).  4096 is the reference's and the
  * parity build; the library is also built with -DTANS_B200_TABLE_SIZE=2048
@@ -366,6 +367,108 @@ int tans_b200_decode_noalloc(const uint8_t *compressed, int64_t compressed_bytes
                              int64_t n_syms, uint8_t *out, int64_t n_streams,
                              int64_t n_fp8_per_stream, int32_t *status,
                              void *stream);
+
+/* ------------------------------------------------ decoder-layer operators
+ *
+ * What a decoder layer with e4m3 weights needs between and around its matrix
+ * products (no counterpart in the reference).  Element types of activations:
+ */
+#define TANS_B200_BF16 0
+#define TANS_B200_F16 1
+#define TANS_B200_F32 2
+
+/* Residual addition and RMS norm of token rows:
+ *   s = x + residual (f32; s = x if residual is null),  h = s rounded,
+ *   y = s * rsqrt(mean(s^2) + eps) * weight
+ * and either y in x's type (y set, q and scale null) or (y null)
+ *   scale[r] = max|y| / 448 (1 for a row of zeros), q = e4m3(y / scale).
+ * x, residual, h: [rows][cols] with strides between rows in elements (the
+ * last dimension dense); y, q: dense; weight: [cols] of x's type or f32.  h is
+ * written only with a residual and may be x or residual itself.  A NaN makes
+ * its row NaN.  cols: 1..57344.  dtype: any of the three. */
+int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
+                           int64_t r_stride, const void *weight, int weight_dtype, float eps,
+                           void *h, int64_t h_stride, void *y, uint8_t *q, float *scale,
+                           int64_t rows, int64_t cols, int dtype, void *stream);
+
+/* The quantisation alone: scale[r] = max|x| / 448, q = e4m3(x / scale). */
+int tans_b200_quantize_tokens(const void *x, int64_t x_stride, uint8_t *q, float *scale,
+                              int64_t rows, int64_t cols, int dtype, void *stream);
+
+/* e4m3 matrix product with its epilogue:
+ *   y[t][r] = act(x_scale[t] * w_scale[r] * sum_c x[t][c] * w[r][c] + bias[r])
+ *             * mul[t][r] + residual[t][r]
+ * x [m][cols] and w [rows][cols] e4m3, both dense and 16-byte aligned, cols a
+ * multiple of 16; x_scale [m], w_scale [rows] f32; bias [rows], mul and
+ * residual [m][rows] (dense) of y's type, each may be null; y [m][rows] dense,
+ * bf16 or f16 (dtype); y may be mul or residual itself.  f32 accumulation, one
+ * rounding.  act: */
+#define TANS_B200_ACT_NONE 0
+#define TANS_B200_ACT_RELU 1
+#define TANS_B200_ACT_SILU 2
+#define TANS_B200_ACT_GELU_TANH 3
+int tans_b200_linear(const uint8_t *x, const float *x_scale, const uint8_t *w,
+                     const float *w_scale, const void *bias, int act, const void *mul,
+                     const void *residual, void *y, int64_t m, int64_t rows, int64_t cols,
+                     int dtype, int32_t *status, void *stream);
+
+/* A paged cache of keys and values in 4 bits: per 16 elements, 8 bytes of
+ * e2m1 codes (the even element in the low half of a byte) and one e4m3 scale.
+ *   codes  [pages][heads][page_size][dim/2],  scales [pages][heads][page_size][dim/16]
+ * all dense and 16-byte aligned; page_size a power of two up to 65536; dim 64,
+ * 128 or 256.  An element is code * scale * gain[head]; k_gain and v_gain f32
+ * [heads] may be null (1). */
+typedef struct tans_b200_kv4 {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    const float *k_gain, *v_gain;
+    int64_t pages, heads, page_size, dim;
+} tans_b200_kv4;
+
+/* Put tokens into the cache, and rotate q on the way.  k, v [tokens][heads][dim]
+ * and q [tokens][q_heads][dim] (may be null) are bf16 or f16 with strides
+ * between tokens (multiples of 8 elements), the heads dense.  The first 2*half
+ * elements of every key and query head are turned by the angles of row
+ * positions[t] of cos and sin, f32 [max_position][half]: element pairs
+ * (i, i + half), or (2i, 2i + 1) if interleaved; half 0: no rotation.  Token t
+ * goes to slot slots[t] = page * page_size + place; a negative slot leaves it
+ * out of the cache.  No two tokens of a call may share a slot.  q_out: dense,
+ * not q.  A slot or position out of range sets TANS_B200_DATA_BAD_INDEX; such
+ * a token is left out, or not rotated. */
+int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, int64_t k_stride,
+                         const void *v, int64_t v_stride, const int64_t *slots, const void *q,
+                         int64_t q_stride, int64_t q_heads, void *q_out,
+                         const int64_t *positions, const float *cos, const float *sin,
+                         int64_t max_position, int64_t half, int interleaved, int64_t tokens,
+                         int dtype, int32_t *status, void *stream);
+
+/* The values that the cache holds in the given slots, k and v
+ * [tokens][heads][dim] dense, any of the three types; zeros for a negative
+ * slot, and for one out of range (TANS_B200_DATA_BAD_INDEX). */
+int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slots, void *k, void *v,
+                       int64_t tokens, int dtype, int32_t *status, void *stream);
+
+/* Attention of new tokens over the cache (their own keys and values appended
+ * before).  q, out [tokens][q_heads][dim] bf16 or f16, q with a stride between
+ * tokens; query heads h * group .. h * group + group - 1 share KV head h.
+ * Sequence b: its new tokens are rows starts[b] .. starts[b+1] - 1 of q (starts
+ * null: row b), at most most_new; it holds lens[b] tokens, the new ones last, in
+ * pages table[b * table_stride + i], i < max_pages.  The i-th of n new tokens
+ * sees keys up to lens[b] - n + i, with window > 0 only the last `window` of
+ * them.  scale multiplies the scores.  lse (f32 [tokens][q_heads], may be
+ * null): log of the sum of exponentials.  A token that sees no key gets zeros
+ * and lse -inf.  Malformed starts, lens or pages set TANS_B200_DATA_BAD_INDEX
+ * and read nothing out of bounds.  workspace: caller-owned device memory,
+ * 16-byte aligned, of tans_b200_kv4_attention_workspace_bytes() bytes (may be
+ * 0); calls that overlap must not share it. */
+int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cache, int64_t q_heads,
+                                            int64_t max_pages, int64_t seqs, int64_t tokens,
+                                            int64_t most_new, int64_t window, int64_t *bytes);
+int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q, int64_t q_stride,
+                            int64_t q_heads, const int32_t *table, int64_t table_stride,
+                            int64_t max_pages, const int32_t *lens, const int32_t *starts,
+                            int64_t seqs, int64_t tokens, int64_t most_new, float scale,
+                            int64_t window, void *out, float *lse, void *workspace,
+                            int64_t workspace_bytes, int dtype, int32_t *status, void *stream);
 
 /* ------------------------------------------------------- device encoder */
 

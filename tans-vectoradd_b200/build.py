@@ -4,7 +4,8 @@
 
 Sources: csrc/kernels.cu (decode/add/GEMV kernels + their entry points),
 csrc/encode.cu (device slab encoder), csrc/pipeline.cu (host-memory
-pipelined fused add) and csrc/host.cpp (CPU encoder, host table builders,
+pipelined fused add), csrc/norm.cu, csrc/linear.cu and csrc/kv4.cu
+(decoder-layer operators) and csrc/host.cpp (CPU encoder, host table builders,
 FP8 splitter, errors).
 Output: rans_vectoradd/libtans_b200.so next to the Python package that loads
 it, so the built file travels with the source tree, and the same sources
@@ -30,9 +31,12 @@ OUT_L11 = os.path.join(HERE, "rans_vectoradd", "libtans_b200_l11.so")
 VARIANTS = [(OUT, []), (OUT_L11, ["-DTANS_B200_TABLE_SIZE=2048"])]
 CU_SOURCES = [os.path.join(CSRC, "kernels.cu"), os.path.join(CSRC, "encode.cu"),
               os.path.join(CSRC, "pipeline.cu")]
+# decoder-layer operators: they use no decode table, so one object serves every variant
+LAYER_SOURCES = [os.path.join(CSRC, n) for n in ("norm.cu", "linear.cu", "kv4.cu")]
 HOST_SOURCE = os.path.join(CSRC, "host.cpp")
-SOURCES = CU_SOURCES + [HOST_SOURCE, os.path.join(INCLUDE, "tans_b200.h"),
-                        os.path.join(CSRC, "internal.h")]
+SOURCES = CU_SOURCES + LAYER_SOURCES + [
+    HOST_SOURCE, os.path.join(INCLUDE, "tans_b200.h"), os.path.join(CSRC, "internal.h"),
+    os.path.join(CSRC, "sm100.cuh")]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -64,22 +68,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
     # the system g++ carries OpenMP; some images point CXX at a compiler without it
     cxx = shutil.which("g++") or "g++"
     with tempfile.TemporaryDirectory() as tmp:
-        cmds, links = [], []
+        nvcc_c = lambda src, obj, defs: [  # noqa: E731
+            nvcc, "-c", src, "-o", obj, *ARCH, *defs, "-O3", "-lineinfo", "-std=c++17",
+            "-Xcompiler", "-fPIC", "-ccbin", cxx, "-Xptxas", "-v" if verbose else "-O3"]
+        layer_objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in LAYER_SOURCES]
+        cmds, links = [nvcc_c(s, o, []) for s, o in zip(LAYER_SOURCES, layer_objs)], []
         for vi, (out, defs) in enumerate(todo):
             d = os.path.join(tmp, str(vi))
             os.makedirs(d)
             cu_objs = [os.path.join(d, os.path.basename(s) + ".o") for s in CU_SOURCES]
             h_obj = os.path.join(d, "host.o")
-            cmds += [
-                [nvcc, "-c", src, "-o", obj, *ARCH, *defs, "-O3", "-lineinfo", "-std=c++17",
-                 "-Xcompiler", "-fPIC", "-ccbin", cxx, "-Xptxas", "-v" if verbose else "-O3"]
-                for src, obj in zip(CU_SOURCES, cu_objs)
-            ] + [
+            cmds += [nvcc_c(src, obj, defs) for src, obj in zip(CU_SOURCES, cu_objs)] + [
                 [cxx, "-c", HOST_SOURCE, "-o", h_obj, *defs, "-O3", "-fPIC", "-fopenmp",
                  "-std=c++17", "-Wall", "-Wextra"],
             ]
             tmp_out = os.path.join(d, os.path.basename(out))
-            links.append(([nvcc, "-shared", *ARCH, "-ccbin", cxx, *cu_objs, h_obj, "-o", tmp_out,
+            links.append(([nvcc, "-shared", *ARCH, "-ccbin", cxx, *cu_objs, *layer_objs, h_obj, "-o",
+                           tmp_out,
                            "-Xcompiler", "-fopenmp", "-lgomp", "-cudart", "shared"], tmp_out, out))
         procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
                  for c in cmds]

@@ -1,0 +1,257 @@
+// norm.cu — residual addition, RMS norm and e4m3 quantisation of token rows.
+//
+//   s = x + r                        (f32; s = x without a residual)
+//   h = rn(s)                        the residual stream, x's type
+//   y = s * rsqrt(mean(s^2) + eps) * w
+//   scale = max|y| / 448 (1 for a row of zeros, never below the smallest normal f32),
+//   q = e4m3(y / scale)
+//
+// All of it in f32, each output rounded once; the mean square is that of the
+// unrounded sum.  max|y| needs no second pass: the factor rsqrt(..) is one
+// positive number a row, so max|y| = rsqrt(..) * max|s * w|, and one block
+// reduction gives both the sum of squares and that maximum.
+//
+// One CTA a row, the row in registers between the reduction and the outputs:
+// every input is read once and every output written once, so the kernel is
+// bound by memory for many rows and by launch and reduction latency for few.
+
+#include "sm100.cuh"
+
+namespace tans_b200 {
+namespace {
+
+struct NormArgs {
+    const void *x, *residual, *weight;  // residual, weight: may be null
+    int64_t x_stride, r_stride, h_stride;  // elements between rows
+    void *h, *y;     // h: null without a residual; y: null when quantising
+    uint8_t *q;
+    float *scale;
+    int32_t cols;
+    float eps;
+    bool weight_f32;
+    bool norm;
+};
+
+// Sum of a and maximum (NaN kept) of b over the block; every thread gets both.
+__device__ __forceinline__ void block_reduce(float &a, float &b, float2 *buf) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return;
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    const float2 v = (threadIdx.x & 31) < warps ? buf[threadIdx.x & 31] : make_float2(0.f, 0.f);
+    a = v.x;
+    b = v.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+}
+
+// The row's factor and quantisation scale from its sum of squares and max|s * w|.
+__device__ __forceinline__ void row_factors(const NormArgs &p, float sumsq, float amax, float &inv,
+                                            float &scale) {
+    inv = p.norm ? rsqrtf(sumsq / (float)p.cols + p.eps) : 1.f;
+    const float top = amax * inv;
+    scale = top == 0.f ? 1.f : max_nan(top / 448.f, 1.17549435e-38f);
+}
+
+// Rows of whole 8-element vectors, 16-byte aligned everywhere: thread t holds
+// vectors t, t + blockDim, ...
+template <typename T, int VPT>
+__global__ void __launch_bounds__(1024) norm_vec_kernel(const NormArgs p) {
+    __shared__ float2 buf[32];
+    pdl_enter();
+    const int64_t row = blockIdx.x;
+    const int vecs = p.cols / 8;
+    const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+    const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
+    float s[VPT][8];
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < vecs) load8(x + 8 * v, s[i]);
+    }
+    if (r) {
+        T *h = static_cast<T *>(p.h) + row * p.h_stride;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+            const int v = threadIdx.x + i * blockDim.x;
+            if (v < vecs) {
+                float a[8];
+                load8(r + 8 * v, a);
+#pragma unroll
+                for (int k = 0; k < 8; k++) s[i][k] += a[k];
+                store8(h + 8 * v, s[i]);
+            }
+        }
+    }
+    float sumsq = 0.f, amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; i++) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < vecs) {
+            float w[8];
+            if (!p.norm) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) w[k] = 1.f;
+            } else if (p.weight_f32) {
+                load8(static_cast<const float *>(p.weight) + 8 * v, w);
+            } else {
+                load8(static_cast<const T *>(p.weight) + 8 * v, w);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                sumsq += s[i][k] * s[i][k];
+                s[i][k] *= w[k];
+                amax = max_nan(amax, fabsf(s[i][k]));
+            }
+        }
+    }
+    block_reduce(sumsq, amax, buf);
+    float inv, scale;
+    row_factors(p, sumsq, amax, inv, scale);
+    if (p.q) {
+        if (threadIdx.x == 0) p.scale[row] = scale;
+        uint8_t *q = p.q + row * p.cols;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+            const int v = threadIdx.x + i * blockDim.x;
+            if (v < vecs) {
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[k] = s[i][k] * inv / scale;
+                uint2 u;
+                u.x = e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16;
+                u.y = e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16;
+                *reinterpret_cast<uint2 *>(q + 8 * v) = u;
+            }
+        }
+    } else {
+        T *y = static_cast<T *>(p.y) + row * p.cols;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) {
+            const int v = threadIdx.x + i * blockDim.x;
+            if (v < vecs) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) s[i][k] *= inv;
+                store8(y + 8 * v, s[i]);
+            }
+        }
+    }
+}
+
+// Any width, stride and alignment: element by element, s * w kept in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
+    extern __shared__ float srow[];
+    __shared__ float2 buf[32];
+    pdl_enter();
+    const int64_t row = blockIdx.x;
+    const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
+    const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
+    T *h = r ? static_cast<T *>(p.h) + row * p.h_stride : nullptr;
+    float sumsq = 0.f, amax = 0.f;
+    for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+        float s = to_f32(x[c]);
+        if (r) {
+            s += to_f32(r[c]);
+            h[c] = from_f32<T>(s);
+        }
+        sumsq += s * s;
+        if (p.norm)
+            s *= p.weight_f32 ? static_cast<const float *>(p.weight)[c] : to_f32(static_cast<const T *>(p.weight)[c]);
+        amax = max_nan(amax, fabsf(s));
+        srow[c] = s;
+    }
+    block_reduce(sumsq, amax, buf);
+    float inv, scale;
+    row_factors(p, sumsq, amax, inv, scale);
+    if (p.q && threadIdx.x == 0) p.scale[row] = scale;
+    for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+        const float y = srow[c] * inv;
+        if (p.q)
+            p.q[row * p.cols + c] = (uint8_t)e4m3x2(y / scale, 0.f);
+        else
+            static_cast<T *>(p.y)[row * p.cols + c] = from_f32<T>(y);
+    }
+}
+
+constexpr int kMaxCols = 56 * 1024;  // f32 values of one row that fit a CTA's shared memory
+
+template <typename T>
+int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
+    const auto vec_ok = [&](const void *ptr, int64_t stride) {
+        return !ptr || (is_aligned(ptr, 16) && stride % (16 / (int64_t)sizeof(T)) == 0);
+    };
+    const bool vec = p.cols % 8 == 0 && p.cols <= 1024 * 32 && vec_ok(p.x, p.x_stride) &&
+                     vec_ok(p.residual, p.r_stride) && vec_ok(p.h, p.h_stride) && vec_ok(p.y, p.cols) &&
+                     is_aligned(p.weight, 16) && is_aligned(p.q, 8);
+    const dim3 grid((unsigned)rows);
+    if (!vec) {
+        const int threads = p.cols >= 1024 ? 512 : (p.cols >= 256 ? 128 : 32);
+        const int smem = p.cols * 4;
+        if (smem > 48 * 1024) {
+            const cudaError_t e =
+                cudaFuncSetAttribute(norm_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) return launch_failed("norm_any_kernel", e);
+        }
+        return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
+    }
+    const int vecs = p.cols / 8;
+    // four vectors a thread keep a row's loads in flight at once with many rows resident
+    const int threads = ceil_div(ceil_div(vecs, 4), 32) * 32;
+    if (vecs <= threads) return launch_ex(norm_vec_kernel<T, 1>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
+    if (vecs <= 2 * threads) return launch_ex(norm_vec_kernel<T, 2>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
+    return launch_ex(norm_vec_kernel<T, 4>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
+}
+
+int check_rows(const char *what, int64_t rows, int64_t cols) {
+    if (rows < 0 || rows > INT32_MAX || cols < 1 || cols > kMaxCols)
+        return fail(TANS_B200_ERR_INVALID, "%s: rows must be 0..2^31-1 and cols 1..%d", what, kMaxCols);
+    return TANS_B200_OK;
+}
+
+}  // namespace
+}  // namespace tans_b200
+
+using namespace tans_b200;
+
+extern "C" int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const void *residual, int64_t r_stride,
+                                      const void *weight, int weight_dtype, float eps, void *h, int64_t h_stride,
+                                      void *y, uint8_t *q, float *scale, int64_t rows, int64_t cols, int dtype,
+                                      void *stream) {
+    clear_error();
+    int rc = check_rows("add_rms_norm", rows, cols);
+    if (rc) return rc;
+    if (rows == 0) return TANS_B200_OK;
+    if (!x || !weight || (residual && !h) || (y ? (q || scale) : (!q || !scale)))
+        return fail(TANS_B200_ERR_INVALID,
+                    "add_rms_norm: x, weight, h with a residual, and either y or q and scale are needed");
+    if (weight_dtype != dtype && weight_dtype != TANS_B200_F32)
+        return fail(TANS_B200_ERR_INVALID, "add_rms_norm: the weight must have x's type or be f32");
+    if (!(eps >= 0.f)) return fail(TANS_B200_ERR_INVALID, "add_rms_norm: eps must not be negative");
+    NormArgs p{x, residual, weight, x_stride, r_stride, h_stride, residual ? h : nullptr, y, q, scale,
+               (int32_t)cols, eps, weight_dtype == TANS_B200_F32, true};
+    return dispatch_float(dtype, "add_rms_norm", [&](auto t) {
+        return launch_norm<decltype(t)>(p, rows, (cudaStream_t)stream);
+    });
+}
+
+extern "C" int tans_b200_quantize_tokens(const void *x, int64_t x_stride, uint8_t *q, float *scale, int64_t rows,
+                                         int64_t cols, int dtype, void *stream) {
+    clear_error();
+    int rc = check_rows("quantize_tokens", rows, cols);
+    if (rc) return rc;
+    if (rows == 0) return TANS_B200_OK;
+    if (!x || !q || !scale) return fail(TANS_B200_ERR_INVALID, "quantize_tokens: null pointer");
+    NormArgs p{x, nullptr, nullptr, x_stride, 0, 0, nullptr, nullptr, q, scale, (int32_t)cols, 0.f, false, false};
+    return dispatch_float(dtype, "quantize_tokens", [&](auto t) {
+        return launch_norm<decltype(t)>(p, rows, (cudaStream_t)stream);
+    });
+}

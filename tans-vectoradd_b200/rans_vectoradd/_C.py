@@ -51,7 +51,8 @@ def _status(device: torch.device) -> torch.Tensor:
 
 def data_status(device: torch.device | int | None = None, reset: bool = True) -> int:
     """Synchronise and return the OR of data-error bits (1 offsets, 2 states,
-    4 table) raised by decode/fused calls on `device` since the last reset."""
+    4 table, 8 a bounded wait ran out, 16 an index of the cache operators out
+    of range) raised by calls on `device` since the last reset."""
     dev = torch.device("cuda", torch.cuda.current_device() if device is None else
                        (device if isinstance(device, int) else device.index or 0))
     buf = _status(dev)
@@ -65,7 +66,8 @@ def _post_check(device: torch.device) -> None:
     if os.environ.get("TANS_B200_CHECK", "") not in ("", "0"):
         v = data_status(device)
         if v:
-            raise RuntimeError(f"tANS data error status {v} (1 offsets, 2 states, 4 table)")
+            raise RuntimeError(f"tANS data error status {v} (1 offsets, 2 states, 4 table, 8 timeout, "
+                               "16 cache index)")
 
 
 def _req(cond: bool, msg: str) -> None:

@@ -10,6 +10,8 @@ from __future__ import annotations
 import ctypes
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtans_b200.so")
 LIB_PATH_L11 = os.path.join(_HERE, "libtans_b200_l11.so")
@@ -18,10 +20,18 @@ OK = 0
 DATA_BAD_OFFSETS = 1
 DATA_BAD_STATE = 2
 DATA_BAD_TABLE = 4
+DATA_TIMEOUT = 8
+DATA_BAD_INDEX = 16
 ENC_INPUT_FP8 = 0
 ENC_INPUT_SYMBOLS = 1
 ENC_TOO_LARGE = 1
 ENC_BAD_SYMBOL = 2
+
+
+class KV4(ctypes.Structure):
+    """tans_b200_kv4"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_codes", "k_scales", "v_codes", "v_scales", "k_gain", "v_gain")] + [
+        (n, ctypes.c_int64) for n in ("pages", "heads", "page_size", "dim")]
 
 
 def _load(path: str = LIB_PATH, table_size: int = 4096) -> ctypes.CDLL:
@@ -30,7 +40,7 @@ def _load(path: str = LIB_PATH, table_size: int = 4096) -> ctypes.CDLL:
             f"{path} is missing: build it with `python tans-vectoradd_b200/build.py` "
             "(rans_vectoradd has no CPU fallback)")
     lib = ctypes.CDLL(path)
-    p, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+    p, i64, i32, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
     sig = {
         "tans_b200_last_error": (ctypes.c_char_p, []),
         "tans_b200_version": (ctypes.c_char_p, []),
@@ -69,6 +79,14 @@ def _load(path: str = LIB_PATH, table_size: int = 4096) -> ctypes.CDLL:
         "tans_b200_encode_device_emit": (i32, [i32, i64, i64, i64, p, p, p, p]),
         "tans_b200_fp8_vecadd_fused_split": (i32, [p, i64, p, p, p, p, p, i64, p, p, p, p, p, p,
                                                    i64, i64, i64, p, p]),
+        "tans_b200_add_rms_norm": (i32, [p, i64, p, i64, p, i32, f32, p, i64, p, p, p, i64, i64, i32, p]),
+        "tans_b200_quantize_tokens": (i32, [p, i64, p, p, i64, i64, i32, p]),
+        "tans_b200_linear": (i32, [p, p, p, p, p, i32, p, p, p, i64, i64, i64, i32, p, p]),
+        "tans_b200_kv4_append": (i32, [p, p, i64, p, i64, p, p, i64, i64, p, p, p, p, i64, i64, i32, i64, i32, p, p]),
+        "tans_b200_kv4_read": (i32, [p, p, p, p, i64, i32, p, p]),
+        "tans_b200_kv4_attention_workspace_bytes": (i32, [p, i64, i64, i64, i64, i64, i64, ctypes.POINTER(i64)]),
+        "tans_b200_kv4_attention": (i32, [p, p, i64, i64, p, i64, i64, p, p, i64, i64, i64, f32, i64, p, p, p, i64,
+                                          i32, p, p]),
         "tans_b200_decode_split": (i32, [p, i64, p, p, p, p, p, p, i64, i64, i64, p, p]),
     }
     for name, (res, args) in sig.items():
@@ -107,6 +125,24 @@ def check(rc: int, lib: ctypes.CDLL | None = None) -> None:
     if rc != OK:
         msg = (lib or LIB).tans_b200_last_error().decode(errors="replace")
         raise RuntimeError(msg or f"libtans_b200 error {rc}")
+
+
+class _Here:
+    """Context for a call on the device that is already current."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def on_device(dev: torch.device):
+    """A device guard for `dev`; free of cost where `dev` is already current."""
+    return _HERE_CTX if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def version() -> str:

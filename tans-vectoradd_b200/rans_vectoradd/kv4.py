@@ -1,0 +1,206 @@
+"""Keys and values in a paged 4-bit cache (no counterpart in the reference).
+
+The cache of a decoder whose weights are this package's e4m3: 16 elements of a
+head are 8 bytes of e2m1 codes and one e4m3 scale, 4.5 bits an element, and an
+element is code * scale * gain[head].  `append` rotates and stores new tokens
+(and rotates their queries in the same launch), `read` gives stored tokens
+back, `attention` runs new tokens over the cache.  All of it on sm_100a kernels
+(csrc/kv4.cu), on torch's current stream.
+
+    cache = kv4.KV4Cache.allocate(pages, kv_heads, page_size=64, head_dim=128, device="cuda")
+    q = kv4.append(cache, k, v, slots, positions=pos, cos=cos, sin=sin, q=q)
+    out = kv4.attention(cache, q, block_table, lens)
+
+Slots, positions, pages and lengths are device data: what is out of range is
+never followed and shows in `rans_vectoradd._C.data_status()` (bit 16).
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from ._C import _post_check, _req, _status, _stream
+from ._lib import LIB, KV4, check, on_device
+
+_HALF = {torch.bfloat16: 0, torch.float16: 1}
+_FLOAT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@dataclass
+class KV4Cache:
+    """k/v codes u8 [pages, heads, page_size, dim/2] and e4m3 scales u8
+    [pages, heads, page_size, dim/16]; optional f32 gains [heads]."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    k_gain: torch.Tensor | None = None
+    v_gain: torch.Tensor | None = None
+
+    def __post_init__(self):
+        shape = self.k_codes.shape
+        _req(len(shape) == 4 and shape[3] * 2 in (64, 128, 256),
+             "codes must be [pages, heads, page_size, dim/2] with dim 64, 128 or 256")
+        pages, heads, size, half = shape
+        _req(size > 0 and size & (size - 1) == 0, "page_size must be a power of two")
+        scales = (pages, heads, size, half // 8)
+        dev = self.k_codes.device
+        for t, want in ((self.k_codes, shape), (self.v_codes, shape), (self.k_scales, scales),
+                        (self.v_scales, scales)):
+            _req(t.dtype == torch.uint8 and t.is_cuda and t.is_contiguous() and t.shape == want
+                 and t.device == dev,
+                 "cache arrays must be contiguous CUDA uint8, codes [.., dim/2] and scales [.., dim/16], "
+                 "on one device")
+        for t in (self.k_gain, self.v_gain):
+            _req(t is None or (t.dtype == torch.float32 and t.shape == (heads,) and t.is_contiguous()
+                               and t.device == dev), "gains must be contiguous f32 [heads]")
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self._c = KV4(ptr(self.k_codes), ptr(self.k_scales), ptr(self.v_codes), ptr(self.v_scales),
+                      ptr(self.k_gain), ptr(self.v_gain), pages, heads, size, 2 * half)
+        self._ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def allocate(cls, pages: int, heads: int, page_size: int = 64, head_dim: int = 128,
+                 device="cuda", k_gain=None, v_gain=None) -> "KV4Cache":
+        """A cache of zeros."""
+        z = lambda per: torch.zeros(pages, heads, page_size, head_dim // per,  # noqa: E731
+                                    dtype=torch.uint8, device=device)
+        return cls(z(2), z(16), z(2), z(16), k_gain, v_gain)
+
+    @property
+    def device(self) -> torch.device:
+        return self.k_codes.device
+
+    @property
+    def heads(self) -> int:
+        return self._c.heads
+
+    @property
+    def page_size(self) -> int:
+        return self._c.page_size
+
+    @property
+    def head_dim(self) -> int:
+        return self._c.dim
+
+    def token_bytes(self) -> int:
+        """Bytes that one token takes, keys and values of all heads."""
+        return self.heads * self.head_dim * 9 // 8
+
+
+def _heads(name: str, t: torch.Tensor, cache: KV4Cache, dtype: torch.dtype) -> int:
+    """Checks [tokens, heads, dim] with dense heads; the stride between tokens."""
+    D = cache.head_dim
+    _req(t.dim() == 3 and t.shape[2] == D and t.dtype == dtype and t.device == cache.device,
+         f"{name} must be [tokens, heads, {D}] {dtype} on the cache's device")
+    st = t.stride()
+    _req((st[2] == 1 and (st[1] == D or t.shape[1] == 1)) or t.numel() == 0,
+         f"{name}'s heads must be dense (strides {D} and 1)")
+    return st[0] if t.shape[0] > 1 else t.shape[1] * D
+
+
+def _index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: torch.device) -> int:
+    _req(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == dev,
+         f"{name} must be a contiguous {dtype} tensor of {n} on the cache's device")
+    return t.data_ptr()
+
+
+def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *,
+           positions: torch.Tensor | None = None, cos: torch.Tensor | None = None,
+           sin: torch.Tensor | None = None, q: torch.Tensor | None = None,
+           interleaved: bool = False) -> torch.Tensor | None:
+    """Store tokens k, v [tokens, heads, dim] (bf16 or f16) in slots [tokens]
+    int64 (page * page_size + place; negative: not stored; no two alike), the
+    keys rotated by positions [tokens] int64, rows of cos and sin f32
+    [max_position, half] (pairs (i, i + half), or (2i, 2i+1) if interleaved;
+    2 * half <= dim).  Returns q [tokens, q_heads, dim] rotated alike, if given."""
+    dt, dev = k.dtype, cache.device
+    _req(dt in _HALF, "k must be bfloat16 or float16")
+    ks, vs = _heads("k", k, cache, dt), _heads("v", v, cache, dt)
+    T = k.shape[0]
+    _req(k.shape[1] == cache.heads and v.shape == k.shape, "k and v must have the cache's heads")
+    half = top = qs = qh = 0
+    pos_p = cos_p = sin_p = None
+    if positions is not None:
+        _req(cos is not None and sin is not None, "positions need cos and sin")
+        _req(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
+             and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == dev,
+             "cos and sin must be contiguous f32 [max_position, half] on the cache's device")
+        top, half = cos.shape
+        pos_p, cos_p, sin_p = _index("positions", positions, T, torch.int64, dev), cos.data_ptr(), sin.data_ptr()
+    else:
+        _req(cos is None and sin is None, "cos and sin need positions")
+    out = None
+    if q is not None:
+        qs, qh = _heads("q", q, cache, dt), q.shape[1]
+        _req(q.shape[0] == T, "q must have k's tokens")
+    with on_device(dev):
+        if q is not None:
+            out = torch.empty(q.shape, dtype=dt, device=dev)
+        check(LIB.tans_b200_kv4_append(
+            cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, _index("slots", slots, T, torch.int64, dev),
+            None if q is None else q.data_ptr(), qs, qh, None if out is None else out.data_ptr(), pos_p, cos_p,
+            sin_p, top, half, int(interleaved), T, _HALF[dt], _status(dev).data_ptr(), _stream(dev)))
+    _post_check(dev)
+    return out
+
+
+def read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16
+         ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [tokens, heads, dim] that the cache holds in slots
+    [tokens] int64 (zeros for a negative slot)."""
+    _req(dtype in _FLOAT, "dtype must be bfloat16, float16 or float32")
+    dev, T = cache.device, slots.shape[0]
+    with on_device(dev):
+        k = torch.empty((T, cache.heads, cache.head_dim), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        check(LIB.tans_b200_kv4_read(cache._ref, _index("slots", slots, T, torch.int64, dev), k.data_ptr(),
+                                     v.data_ptr(), T, _FLOAT[dtype], _status(dev).data_ptr(), _stream(dev)))
+    _post_check(dev)
+    return k, v
+
+
+def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
+              starts: torch.Tensor | None = None, most_new: int = 1, scale: float | None = None,
+              window: int = 0, return_lse: bool = False, workspace: torch.Tensor | None = None):
+    """out [tokens, q_heads, dim] of new tokens q over the cache.
+
+    table [seqs, max_pages] int32: the pages of each sequence; lens [seqs]
+    int32: the tokens it holds, its new ones (already appended) last.  starts
+    [seqs + 1] int32: the rows of q that are each sequence's new tokens, at
+    most most_new of them; without it every sequence has one.  Causal: the i-th
+    of n new tokens sees keys up to lens - n + i, only the last `window` of them
+    if window > 0.  scale defaults to dim ** -0.5.  A token that sees nothing
+    gets zeros.  With return_lse also the f32 [tokens, q_heads] logarithm of the
+    sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
+    least `attention_workspace_bytes`, else allocated."""
+    dt, dev = q.dtype, cache.device
+    _req(dt in _HALF, "q must be bfloat16 or float16")
+    qs = _heads("q", q, cache, dt)
+    T, H, D = q.shape
+    B = lens.shape[0] if lens.dim() == 1 else -1
+    _req(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] == B and table.device == dev
+         and (table.stride(1) == 1 or table.shape[1] <= 1), "table must be int32 [seqs, max_pages], rows dense")
+    lens_p = _index("lens", lens, B, torch.int32, dev)
+    starts_p = None if starts is None else _index("starts", starts, B + 1, torch.int32, dev)
+    P = table.shape[1]
+    with on_device(dev):
+        out = torch.empty(q.shape, dtype=dt, device=dev)
+        lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+        need = ctypes.c_int64()
+        check(LIB.tans_b200_kv4_attention_workspace_bytes(cache._ref, H, P, B, T, most_new, window,
+                                                          ctypes.byref(need)))
+        if need.value and workspace is None:
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+        check(LIB.tans_b200_kv4_attention(
+            cache._ref, q.data_ptr(), qs, H, table.data_ptr(), table.stride(0), P, lens_p, starts_p, B, T, most_new,
+            D ** -0.5 if scale is None else scale, window, out.data_ptr(), None if lse is None else lse.data_ptr(),
+            ws, ws_bytes, _HALF[dt], _status(dev).data_ptr(), _stream(dev)))
+    _post_check(dev)
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["KV4Cache", "append", "read", "attention"]
