@@ -215,21 +215,28 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //   lse = log(sum(exp(S)));  no visible key: O = 0, lse = -inf.
 //
 // The rows of one KV head are its new tokens times the query heads that share
-// it (row = token * group + head in group); a CTA takes 16 of them, the M of
-// one m16n8k16 MMA, and its warps take 16-key blocks of the visible range in
-// turn.  Codes become MMA operands in registers, with no trip through shared
-// memory:
+// it (row = token * group + head in group); 16 of them are the M of an
+// m16n8k16 MMA and make a tile.  The keys of a (sequence, head, tile) are cut
+// into units of 64, 16 for each of a CTA's four warps, which keep a running
+// maximum and sum each and join at the end.
+//
+// Codes go from shared memory (a ring of asynchronous copies per warp) to MMA
+// operands in registers:
 //  * S = Q K^T: the contraction runs over D in any order, so lane (g, t) takes
-//    key g of each 8-key half and the t-th quarter of its D codes, D/8
-//    contiguous bytes; the k-th step uses codes 4k .. 4k+3 of that quarter, and
-//    the Q fragments are loaded in the same order.
-//  * O = P V: lane (g, t) takes the g-th eighth of D of keys 2t, 2t+1, 2t+8,
-//    2t+9, the keys of its P fragment; merging the nibbles of two keys gives
-//    bytes whose conversion is the f16 pair (key, key + 1) of one element.
-// code * scale is exact in f16 and bf16, Q enters in its own type, P in f16
-// relative to a running maximum; sums, maxima and O stay in f32.
+//    one key of each 8-key half and the t-th quarter of its D codes, D/8
+//    contiguous bytes; step j uses codes 4j .. 4j+3 of that quarter, and
+//    the Q fragments are laid out in the same order.
+//  * O = P V: lane (g, t) takes the g-th eighth of D of the four keys of its P
+//    fragment; merging the nibbles of two keys gives bytes whose conversion is
+//    the f16 pair (key, other key) of one element.
+// code * scale is exact in f16; P enters in f16 relative to a maximum that may
+// lag by up to 2^8; sums, maxima and O stay in f32.  bf16 queries become f16
+// after a power of two per row that brings their largest element to 2^14: an
+// element loses bits only below 2^-28 of that.
 
 constexpr int kAttnWarps = 4;
+constexpr int kUnit = 16 * kAttnWarps;  // keys
+constexpr int kStages = 4;              // 16-key blocks in a warp's ring
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
@@ -242,21 +249,58 @@ struct AttendArgs {
     const int32_t *starts; // [seqs + 1] first new token of each sequence, null: one each
     void *out;             // [tokens][q_heads][D]
     float *lse;            // [tokens][q_heads], may be null
-    int32_t tokens, group, max_pages, most_new, window;
+    float *parts;          // workspace of a split launch, else null
+    int32_t tokens, seqs, group, max_pages, most_new, window;
     float scale;           // softmax scale
     int32_t *status;
 };
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (std::is_same_v<T, __half>)
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// A sequence's part in the work.  lo and hi cover the keys of all its rows.
+struct Sequence {
+    int first, news, len, lo, hi;
+    int tiles, units;  // units of one tile; at least one, which writes the zeros of rows that see nothing
+};
+
+__device__ __forceinline__ Sequence sequence(const AttendArgs &p, int seq) {
+    Sequence s{seq, 1, 0, 0, 0, 0, 0};
+    bool bad = false;
+    if (p.starts) {
+        s.first = p.starts[seq];
+        s.news = p.starts[seq + 1] - s.first;
+        if (s.first < 0 || s.news < 0 || s.news > p.most_new || s.first > p.tokens - s.news) {
+            bad = true;
+            s.news = 0;
+        }
+    }
+    s.len = p.lens[seq];
+    const int64_t room = (int64_t)p.max_pages << p.cache.page_log2;
+    if (s.len < 0 || s.len > room) {
+        bad = true;
+        s.len = s.len < 0 ? 0 : (int)room;
+    }
+    if (bad && p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+    s.hi = s.len - 1;
+    const int last = s.len - s.news;  // the last key of the first new token
+    s.lo = p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0;
+    s.tiles = ceil_div(s.news * p.group, 16);
+    s.units = max(1, ceil_div(s.hi + 1 - (s.lo & ~(kUnit - 1)), kUnit));
+    return s;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t *src, bool real) {
+    const int n = real ? BYTES : 0;  // what is not read is filled with zeros
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
     else
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
+                     : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
@@ -269,146 +313,220 @@ __device__ __forceinline__ uint32_t h2_of(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
-// f16x2 whose values are exact in bf16 -> bf16x2
-__device__ __forceinline__ uint32_t h2_to_bf2(uint32_t h) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
-
-// e4m3 byte -> f16x2 with the value in both halves (exact)
-__device__ __forceinline__ uint32_t e4m3_h2(uint32_t b) {
+// two e4m3 bytes -> f16x2 (exact)
+__device__ __forceinline__ uint32_t e4m3x2_h2(uint32_t two) {
     uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)(b | b << 8)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)two));
     return h2;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void load_words(const uint8_t *p, uint32_t (&w)[BYTES / 4]) {
-    if constexpr (BYTES >= 16) {
-#pragma unroll
-        for (int i = 0; i < BYTES / 16; i++) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p + 16 * i);
-            w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-        }
-    } else if constexpr (BYTES == 8) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p);
-        w[0] = u.x, w[1] = u.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t *>(p);
-    }
+// four bytes of two e2m1 codes each -> four f16x2 (exact), low code in the low half
+__device__ __forceinline__ void e2m1x8_h2(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(w));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArgs p) {
-    constexpr int kSteps = D / 16;          // MMA steps of S
-    constexpr int kTiles = D / 8;           // MMA column tiles of O
-    constexpr int kQ = D / 4, kE = D / 8;   // elements of a quarter and of an eighth of a head
-    extern __shared__ float merge[];        // [warps][16][D] O, then [warps][16] maxima and sums
-    pdl_enter();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int seq = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * 16;
-    int first, news;
-    if (p.starts) {
-        first = p.starts[seq];
-        news = p.starts[seq + 1] - first;
-        if (first < 0 || news < 0 || news > p.most_new || first > p.tokens - news) {
-            if (p.status && threadIdx.x == 0) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            return;
-        }
-    } else {
-        first = seq;
-        news = 1;
-    }
-    const int rows = news * p.group;
-    if (row0 >= rows) return;
-    int len = p.lens[seq];
-    const int64_t room = (int64_t)p.max_pages << p.cache.page_log2;
-    if (len < 0 || len > room) {
-        if (p.status && threadIdx.x == 0) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-        len = len < 0 ? 0 : (int)room;
-    }
-    // keys lo[i] .. hi[i] are those of this lane's two rows; lo_all .. hi_all cover the tile
-    const auto last_key = [&](int row) { return len - news + row / p.group; };
-    const auto first_key = [&](int last) { return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0; };
-    const int row_end = min(row0 + 16, rows) - 1;
-    const int lo_all = first_key(last_key(row0)), hi_all = last_key(row_end);
-    const int lo_in = first_key(last_key(row_end)), hi_in = last_key(row0);  // seen by every row
-    int lo[2], hi[2];
-    int64_t at_row[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = min(row0 + g + 8 * i, row_end);
-        hi[i] = last_key(row);
-        lo[i] = first_key(hi[i]);
-        at_row[i] = (int64_t)(first + row / p.group) * p.q_stride + ((int64_t)head * p.group + row % p.group) * D;
-    }
+// 2^x, relative error under 2^-22, results below the normal range flushed to 0
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
-    // Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
-    uint32_t qf[kSteps][4];
-#pragma unroll
-    for (int j = 0; j < kSteps; j++)
+template <int D>
+struct AttnLayout {
+    static constexpr int kCodes = 16 * D / 2, kScales = 16 * D / 16;       // bytes of a 16-key block
+    static constexpr int kBlock = 2 * (kCodes + kScales);                  // K codes, V codes, K scales, V scales
+    static constexpr int kRing = kAttnWarps * kStages * kBlock;
+    static constexpr int kMerge = kAttnWarps * 16 * (D + 2) * 4;           // the warps' O, maxima and sums
+    static constexpr int kQ = D / 16 * 512;                                // Q fragments
+    static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ;
+    static constexpr int kPart = 16 * (D + 2);                             // floats of a partial result
+};
+
+// Rows of a tile for one (sequence, head), keys k0 .. k1 (multiples of kUnit
+// from the sequence's first unit): the four warps' results lie in `merge`
+// afterwards as [warp][16][D] O, [warp][16] maxima, [warp][16] sums.
+template <typename T, int D>
+__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence &q, int seq, int head, int row0, int k0,
+                                             int k1, uint8_t *smem) {
+    using L = AttnLayout<D>;
+    constexpr int kSteps = D / 16;         // MMA steps of S
+    constexpr int kTiles = D / 8;          // MMA column tiles of O
+    constexpr int kE = D / 8;              // elements of an eighth of a head
+    constexpr int kVS = (D + 127) / 128;   // scales of an eighth
+    constexpr int kKS = D / 64;            // scales of a quarter
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int rows = q.news * p.group, row_end = min(row0 + 16, rows) - 1;
+    const auto last_key = [&](int row) { return q.len - q.news + row / p.group; };
+    const auto first_key = [&](int last) { return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0; };
+    // keys lo[i] .. hi[i] are those of this lane's two rows; lo_all .. hi_all cover
+    // the tile, lo_in .. hi_in are seen by every row of it
+    const int lo_all = first_key(last_key(row0)), hi_all = last_key(row_end);
+    const int lo_in = first_key(last_key(row_end)), hi_in = last_key(row0);
+    int lo[2], hi[2];
+    uint8_t *ring = smem + warp * (kStages * L::kBlock);
+    uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
+    float to_log2[2];
+    {
+        const float c = p.scale * kLog2e * (p.cache.k_gain ? p.cache.k_gain[head] : 1.f);
+        // Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
+        uint2 u[2][kSteps];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const T *>(p.q) + at_row[i] + t * kQ + 4 * j);
-            qf[j][i] = u.x;
-            qf[j][2 + i] = u.y;
+            const int row = min(row0 + g + 8 * i, row_end);
+            hi[i] = last_key(row);
+            lo[i] = first_key(hi[i]);
+            const T *src = static_cast<const T *>(p.q) + (int64_t)(q.first + row / p.group) * p.q_stride +
+                           ((int64_t)head * p.group + row % p.group) * D + t * (D / 4);
+#pragma unroll
+            for (int j = 0; j < kSteps; j++) u[i][j] = *reinterpret_cast<const uint2 *>(src + 4 * j);
+            to_log2[i] = c;
+            if constexpr (!std::is_same_v<T, __half>) {
+                float top = 0.f;
+#pragma unroll
+                for (int j = 0; j < kSteps; j++) {
+                    const T *e = reinterpret_cast<const T *>(&u[i][j]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) top = fmaxf(top, fabsf(to_f32(e[k])));
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // top * 2^k in [2^14, 2^15)
+                k = top == 0.f || top > 3.4e38f ? 0 : min(k, 100);
+                const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+                to_log2[i] = c * __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+                for (int j = 0; j < kSteps; j++) {
+                    const T *e = reinterpret_cast<const T *>(&u[i][j]);
+                    u[i][j] = make_uint2(h2_of(to_f32(e[0]) * up, to_f32(e[1]) * up),
+                                         h2_of(to_f32(e[2]) * up, to_f32(e[3]) * up));
+                }
+            }
         }
-    const float to_log2 = p.scale * kLog2e * (p.cache.k_gain ? p.cache.k_gain[head] : 1.f);
+        if (warp == 0) {
+#pragma unroll
+            for (int j = 0; j < kSteps; j++) qs[j * 32 + lane] = make_uint4(u[0][j].x, u[1][j].x, u[0][j].y, u[1][j].y);
+        }
+    }
+    __syncthreads();
+
+    const int32_t *table = p.table + (int64_t)seq * p.table_stride;
+    const int in_page = (1 << p.cache.page_log2) - 1;
+    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
+    // the page of key base + (lane & 15), loaded a block ahead of its use
+    const auto page_of = [&](int base) -> int {
+        const int key = base + (lane & 15);
+        return base < k1 && key >= lo_all && key <= hi_all ? table[key >> p.cache.page_log2] : 0;
+    };
+    // start the copies of the block at `base` (its keys' pages in `pages`) into `stage`
+    const auto fetch = [&](int base, int pages, int stage) {
+        if (base < k1) {
+            if ((pages < 0 || pages >= p.cache.pages) && p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+            const bool ok = pages >= 0 && pages < p.cache.pages;
+            const int pg = ok ? pages : 0;
+            const uint32_t dst = ring_sa + (uint32_t)stage * L::kBlock;
+            constexpr int kRow = D / 32;  // 16-byte chunks of a token's codes
+#pragma unroll
+            for (int i = 0; i < 16 * kRow / 32; i++) {
+                const int r = (lane + 32 * i) / kRow, c = lane % kRow, key = base + r;
+                const int64_t at = token_at(p.cache, __shfl_sync(0xffffffffu, pg, r), head, key & in_page);
+                const bool real = key >= lo_all && key <= hi_all;
+                const int64_t off = real ? at * (D / 2) + 16 * c : 0;
+                copy_async<16>(dst + r * (D / 2) + 16 * c, p.cache.k_codes + off, real);
+                // V chunks change places so that four keys' reads meet different banks
+                const int cv = D == 128 ? c ^ (r >> 1 & 2) : c;
+                copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * cv, p.cache.v_codes + off, real);
+            }
+            const int r = lane & 15, key = base + r;
+            const bool real = key >= lo_all && key <= hi_all;
+            const int64_t off = real ? token_at(p.cache, pg, head, key & in_page) * (D / 16) : 0;
+            const uint8_t *src = lane < 16 ? p.cache.k_scales : p.cache.v_scales;
+            copy_async<D / 16>(dst + 2 * L::kCodes + (lane >> 4) * L::kScales + r * (D / 16), src + off, real);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 
     float o[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-    const int32_t *table = p.table + (int64_t)seq * p.table_stride;
-    const int in_page = (1 << p.cache.page_log2) - 1;
-    const auto place = [&](int key) -> int64_t {  // where a key's head lies, in token units
-        int64_t page = table[key >> p.cache.page_log2];
-        if (page < 0 || page >= p.cache.pages) {
-            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            page = 0;
-        }
-        return token_at(p.cache, page, head, key & in_page);
-    };
 
-    for (int base = (lo_all & ~15) + 16 * warp; base <= hi_all; base += 16 * kAttnWarps) {
+    int base = k0 + 16 * warp, ahead = base, stage = 0;
+    int pages = page_of(ahead);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) {
+        const int now = pages;
+        pages = page_of(ahead + kUnit);
+        fetch(ahead, now, i);
+        ahead += kUnit;
+    }
+    for (; base < k1; base += kUnit) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        {
+            const int now = pages;
+            pages = page_of(ahead + kUnit);
+            fetch(ahead, now, stage == 0 ? kStages - 1 : stage - 1);
+            ahead += kUnit;
+        }
+        const uint8_t *blk = ring + stage * L::kBlock;
+        if (++stage == kStages) stage = 0;
+        // Column n of an 8-key half is key n ^ (n >> 1 & 1): the V reads of
+        // lanes t = 0..3 then fall on rows of both parities.
         // ---- scores of 16 keys
         float s[2][4] = {};
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int key = base + 8 * h + g;
-            uint32_t w[D / 32] = {};
-            uint32_t sc[(D + 63) / 64] = {};
-            if (key >= lo_all && key <= hi_all) {
-                const int64_t at = place(key);
-                load_words<D / 8>(p.cache.k_codes + at * (D / 2) + t * (D / 8), w);
-                const uint8_t *sp = p.cache.k_scales + at * (D / 16);
+            const int r = 8 * h + (g ^ (g >> 1 & 1));
+            uint32_t w[D / 32], f[kKS];
+            if constexpr (D == 64) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(blk + r * (D / 2) + t * (D / 8));
+                w[0] = v.x, w[1] = v.y;
+            } else {
 #pragma unroll
-                for (int i = 0; i < (D + 63) / 64; i++) sc[i] = sp[t * kQ / 16 + i];
+                for (int i = 0; i < D / 128; i++) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(blk + r * (D / 2) + t * (D / 8) + 16 * i);
+                    w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                }
+            }
+            const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
+            if constexpr (kKS == 1) {
+                f[0] = e4m3x2_h2(*sp * 0x101u);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kKS; i += 2) {
+                    const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
+                    f[i] = __byte_perm(two, two, 0x1010);
+                    f[i + 1] = __byte_perm(two, two, 0x3232);
+                }
             }
 #pragma unroll
-            for (int j = 0; j < kSteps; j++) {
-                const uint32_t two = w[j / 2] >> (16 * (j & 1));
-                const uint32_t f = e4m3_h2(sc[4 * j / 16]);
-                uint32_t b0 = mul_h2(e2m1x2_f16(two & 0xFFu), f), b1 = mul_h2(e2m1x2_f16((two >> 8) & 0xFFu), f);
-                if constexpr (!std::is_same_v<T, __half>) {
-                    b0 = h2_to_bf2(b0);
-                    b1 = h2_to_bf2(b1);
-                }
-                mma16816<T>(s[h], qf[j], b0, b1);
+            for (int j = 0; j < kSteps; j += 2) {
+                uint32_t b[4];
+                e2m1x8_h2(w[j / 2], b);
+#pragma unroll
+                for (int i = 0; i < 4; i++) b[i] = mul_h2(b[i], f[j / 4]);
+                mma_f16(s[h], qs[j * 32 + lane], b[0], b[1]);
+                mma_f16(s[h], qs[(j + 1) * 32 + lane], b[2], b[3]);
             }
         }
         // ---- the running maximum and the weights
         const bool edge = base < lo_in || base + 15 > hi_in;
-        float p_[2][4];
         bool grew = false;
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const int i = c >> 1, key = base + 8 * h + 2 * t + (c & 1);
-                float v = s[h][c] * to_log2;
-                if (edge && (key < lo[i] || key > hi[i])) v = -INFINITY;
+                const int i = c >> 1;
+                float v = s[h][c] * to_log2[i];
+                if (edge) {
+                    const int key = base + 8 * h + ((2 * t + (c & 1)) ^ (t & 1));
+                    if (key < lo[i] || key > hi[i]) v = -INFINITY;
+                }
                 s[h][c] = v;
                 grew |= v > top[i] + 8.f;
             }
@@ -434,24 +552,29 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 const int i = c >> 1;
-                p_[h][c] = exp2f(s[h][c] - (top[i] == -INFINITY ? 0.f : top[i]));
-                sum[i] += p_[h][c];
+                s[h][c] = exp2_fast(s[h][c] - (top[i] == -INFINITY ? 0.f : top[i]));
+                sum[i] += s[h][c];
             }
-        const uint32_t pf[4] = {h2_of(p_[0][0], p_[0][1]), h2_of(p_[0][2], p_[0][3]), h2_of(p_[1][0], p_[1][1]),
-                                h2_of(p_[1][2], p_[1][3])};
-        // ---- values of keys 2t, 2t + 1, 2t + 8, 2t + 9
-        uint32_t w[4][(D / 16 + 3) / 4] = {};
-        uint32_t sc[4][(D + 127) / 128] = {};
+        const uint4 pf = make_uint4(h2_of(s[0][0], s[0][1]), h2_of(s[0][2], s[0][3]), h2_of(s[1][0], s[1][1]),
+                                    h2_of(s[1][2], s[1][3]));
+        // ---- values of the lane's four keys
+        uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const int key = base + 2 * t + (k & 1) + 8 * (k >> 1);
-            if (key >= lo_all && key <= hi_all) {
-                const int64_t at = place(key);
-                load_words<D / 16>(p.cache.v_codes + at * (D / 2) + g * (D / 16), w[k]);
-                const uint8_t *sp = p.cache.v_scales + at * (D / 16);
-#pragma unroll
-                for (int i = 0; i < (D + 127) / 128; i++) sc[k][i] = sp[g * kE / 16 + i];
+            const int r = 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+            const uint8_t *vp = blk + L::kCodes + r * (D / 2);
+            if constexpr (D == 64) {
+                w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
+            } else if constexpr (D == 128) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(vp + ((8 * g) ^ ((r >> 1 & 2) << 4)));
+                w[k][0] = v.x, w[k][1] = v.y;
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
+                w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
             }
+#pragma unroll
+            for (int i = 0; i < kVS; i++)
+                sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
         }
         // A NaN scale on a key that only some rows see must not reach the
         // others as 0 * NaN: its values count as 0 here and are added below.
@@ -460,11 +583,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int i = 0; i < (D + 127) / 128; i++) nan_key |= (sc[k][i] & 0x7Fu) == 0x7Fu;
+                for (int i = 0; i < kVS; i++) nan_key |= (sc[k][i] & 0x7Fu) == 0x7Fu;
             nan_key = __any_sync(0xffffffffu, nan_key);
         }
 #pragma unroll
-        for (int i = 0; i < (D + 127) / 128; i++) {
+        for (int i = 0; i < kVS; i++) {
             uint32_t f[2];
 #pragma unroll
             for (int b = 0; b < 2; b++) {
@@ -473,20 +596,24 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
                     if ((lo8 & 0x7Fu) == 0x7Fu) lo8 = 0;
                     if ((hi8 & 0x7Fu) == 0x7Fu) hi8 = 0;
                 }
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f[b]) : "h"((uint16_t)(lo8 | hi8 << 8)));
+                f[b] = e4m3x2_h2(lo8 | hi8 << 8);
             }
             constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
 #pragma unroll
-            for (int j = 0; j < kPer; j++) {
-                const int word = (i * 16 + j) / 8, sh = 4 * (j & 6);
-                uint32_t b[2];
+            for (int j = 0; j < kPer; j += 8) {
+                const int word = (i * 16 + j) / 8;
+                uint32_t even[2][4], odd[2][4];
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint32_t u = w[2 * x][word] >> sh, v = w[2 * x + 1][word] >> sh;
-                    const uint32_t byte = (j & 1) ? ((u >> 4) & 0xFu) | (v & 0xF0u) : (u & 0xFu) | ((v & 0xFu) << 4);
-                    b[x] = mul_h2(e2m1x2_f16(byte), f[x]);
+                for (int b = 0; b < 2; b++) {
+                    const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
+                    e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
+                    e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
                 }
-                mma16816<__half>(o[i * 16 + j], pf, b[0], b[1]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    mma_f16(o[i * 16 + j + 2 * e], pf, mul_h2(even[0][e], f[0]), mul_h2(even[1][e], f[1]));
+                    mma_f16(o[i * 16 + j + 2 * e + 1], pf, mul_h2(odd[0][e], f[0]), mul_h2(odd[1][e], f[1]));
+                }
             }
         }
         if (nan_key) {
@@ -495,19 +622,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const int key = base + 8 * h + 2 * t;
-                    seen[2 * h + i] = h2_of(key >= lo[i] && key <= hi[i] ? 1.f : 0.f,
-                                            key + 1 >= lo[i] && key + 1 <= hi[i] ? 1.f : 0.f);
+                    const int a = base + 8 * h + ((2 * t) ^ (t & 1)), b = base + 8 * h + ((2 * t + 1) ^ (t & 1));
+                    seen[2 * h + i] = h2_of(a >= lo[i] && a <= hi[i] ? 1.f : 0.f, b >= lo[i] && b <= hi[i] ? 1.f : 0.f);
                 }
 #pragma unroll
-            for (int i = 0; i < (D + 127) / 128; i++) {
+            for (int i = 0; i < kVS; i++) {
                 uint32_t b[2];
 #pragma unroll
                 for (int x = 0; x < 2; x++)
                     b[x] = h2_of((sc[2 * x][i] & 0x7Fu) == 0x7Fu ? 1.f : 0.f,
                                  (sc[2 * x + 1][i] & 0x7Fu) == 0x7Fu ? 1.f : 0.f);
                 float n[4] = {};
-                mma16816<__half>(n, seen, b[0], b[1]);
+                mma_f16(n, make_uint4(seen[0], seen[1], seen[2], seen[3]), b[0], b[1]);
                 constexpr int kPer = kE < 16 ? kE : 16;
 #pragma unroll
                 for (int j = 0; j < kPer; j++)
@@ -516,9 +642,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
                         if (n[c] > 0.f) o[i * 16 + j][c] = NAN;
             }
         }
+        __syncwarp();  // the block is read before its place in the ring is filled again
     }
 
-    // ---- join the warps
+    // ---- the warps' results, side by side
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float *merge = reinterpret_cast<float *>(smem);
     float *tops = merge + kAttnWarps * 16 * D, *sums = tops + kAttnWarps * 16;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
@@ -529,48 +659,255 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArg
             sums[warp * 16 + g + 8 * i] = sum[i];
         }
     }
-    // tile j, column n of the MMA is element (n * kE + j): two columns a lane
+    // tile j, column n of the MMA is element n * kE + j: two columns a lane
 #pragma unroll
     for (int j = 0; j < kTiles; j++)
 #pragma unroll
         for (int c = 0; c < 4; c++)
             merge[(warp * 16 + g + 8 * (c >> 1)) * D + (2 * t + (c & 1)) * kE + j] = o[j][c];
     __syncthreads();
-    const float gain = p.cache.v_gain ? p.cache.v_gain[head] : 1.f;
-    for (int r = warp; r <= row_end - row0; r += kAttnWarps) {
-        float m = -INFINITY, l = 0.f, f[kAttnWarps];
+}
+
+// The factor that brings a part with maximum `top` and sum `sum` to the common
+// maximum m (0 where it is -inf); a part that saw nothing has factor 0, one
+// whose scores are all NaN keeps its NaN.
+__device__ __forceinline__ float part_factor(float top, float sum, float m) {
+    return top == -INFINITY && sum == 0.f ? 0.f : exp2f(top - (m == -INFINITY ? 0.f : m));
+}
+
+// One row of the output from its sum l and O v, both relative to the maximum m; a lane has every 32nd element.
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const AttendArgs &p, int head, int heads, int64_t token, int in_group, float m,
+                                          float l, const float (&v)[D / 32]) {
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (token * heads + head) * p.group + in_group;
+    const float inv = l == 0.f ? 0.f : (p.cache.v_gain ? p.cache.v_gain[head] : 1.f) / l;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+        static_cast<T *>(p.out)[at * D + lane + 32 * i] = from_f32<T>(l == 0.f ? 0.f : v[i] * inv);
+    if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) / kLog2e + logf(l);
+}
+
+// Joins the four warps' results of a piece: into the output if the piece is
+// the tile's whole range, else into a part of the workspace.
+template <typename T, int D>
+__device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &q, int head, int row0, const uint8_t *smem,
+                                           float *part) {
+    const float *merge = reinterpret_cast<const float *>(smem);
+    const float *tops = merge + kAttnWarps * 16 * D, *sums = tops + kAttnWarps * 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows = min(16, q.news * p.group - row0);
+    for (int r = warp; r < rows; r += kAttnWarps) {
+        float m = -INFINITY, l = 0.f, f[kAttnWarps], v[D / 32];
 #pragma unroll
         for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, tops[w * 16 + r]);
 #pragma unroll
         for (int w = 0; w < kAttnWarps; w++) {
-            f[w] = tops[w * 16 + r] == -INFINITY && !(sums[w * 16 + r] != sums[w * 16 + r])
-                       ? 0.f
-                       : exp2f(tops[w * 16 + r] - (m == -INFINITY ? 0.f : m));
+            f[w] = part_factor(tops[w * 16 + r], sums[w * 16 + r], m);
             l += f[w] * sums[w * 16 + r];
         }
-        const int row = row0 + r;
-        const int64_t at = (int64_t)(first + row / p.group) * gridDim.y * p.group + (int64_t)head * p.group + row % p.group;
-        const float inv = l == 0.f ? 0.f : gain / l;
-        for (int e = lane; e < D; e += 32) {
-            float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            v[i] = 0.f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; w++)
-                if (f[w] != 0.f) v += f[w] * merge[(w * 16 + r) * D + e];
-            static_cast<T *>(p.out)[at * D + e] = from_f32<T>(l == 0.f ? 0.f : v * inv);
+                if (f[w] != 0.f) v[i] += f[w] * merge[(w * 16 + r) * D + lane + 32 * i];
         }
-        if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (m == -INFINITY ? 0.f : m) / kLog2e + logf(l);
+        if (part) {
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) part[r * D + lane + 32 * i] = v[i];
+            if (lane == 0) {
+                part[16 * D + r] = m;
+                part[16 * D + 16 + r] = l;
+            }
+        } else {
+            const int row = row0 + r;
+            write_row<T, D>(p, head, p.cache.heads, q.first + row / p.group, row % p.group, m, l, v);
+        }
     }
 }
 
+// One CTA a (tile, head, sequence), over all its keys.
 template <typename T, int D>
-int launch_attend(const AttendArgs &p, int seqs, int max_rows, cudaStream_t st) {
-    const int smem = (kAttnWarps * 16 * D + 2 * kAttnWarps * 16) * 4;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return launch_failed("attend_kernel", e);
+__global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    pdl_enter();
+    const int seq = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * 16;
+    const Sequence q = sequence(p, seq);
+    if (row0 >= q.news * p.group) return;
+    const int k0 = q.lo & ~(kUnit - 1);
+    attend_piece<T, D>(p, q, seq, head, row0, k0, k0 + q.units * kUnit, smem);
+    join_warps<T, D>(p, q, head, row0, smem, nullptr);
+}
+
+// Split form: the units of all tiles in a row (sequence, head, tile, unit),
+// cut into equal stretches, one a CTA, whatever the sequences' lengths.  A
+// CTA's first tile may have begun in an earlier one (part 0 of its
+// workspace), its last may go on in the next (part 1); those are joined by
+// attend_join_kernel, whose CTA c takes the tile that begins in stretch c
+// and does not end there, as `head` describes it.
+struct SplitHead {
+    int32_t pieces;  // 0: none
+    int32_t seq, head, row0, rows, first;
+    int32_t pad[2];
+};
+
+template <int D>
+__host__ __device__ constexpr int64_t split_floats() {
+    return sizeof(SplitHead) / 4 + 2 * AttnLayout<D>::kPart;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kAttnWarps * 32) attend_split_kernel(const AttendArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int64_t warp_sum[kAttnWarps], found_at;
+    __shared__ int found_seq;
+    constexpr int kThreads = kAttnWarps * 32;
+    pdl_enter();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float *mine = p.parts + blockIdx.x * split_floats<D>();
+    SplitHead *info = reinterpret_cast<SplitHead *>(mine);
+    if (tid == 0) info->pieces = 0;
+    const auto units_of = [&](int seq) -> int64_t {
+        if (seq >= p.seqs) return 0;
+        const Sequence s = sequence(p, seq);
+        return (int64_t)s.tiles * s.units * p.cache.heads;
+    };
+    int64_t total = 0;
+    for (int b = tid; b < p.seqs; b += kThreads) total += units_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) warp_sum[warp] = total;
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < kAttnWarps; w++) total += warp_sum[w];
+    const int64_t per = ceil_div<int64_t>(total, gridDim.x);
+    int64_t u = per * blockIdx.x;
+    const int64_t u_end = u + per < total ? u + per : total;
+    if (u >= u_end) return;
+    // the sequence in which unit u lies, and that sequence's first unit
+    int64_t before = 0;
+    for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
+        const int64_t n = units_of(b0 + tid);
+        int64_t inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = inc;
+        __syncthreads();
+        int64_t at = before + inc - n;
+        for (int w = 0; w < kAttnWarps; w++) {
+            if (w < warp) at += warp_sum[w];
+            before += warp_sum[w];
+        }
+        if (u >= at && u < at + n) {
+            found_seq = b0 + tid;
+            found_at = at;
+        }
+        __syncthreads();
+        if (u < before) break;
     }
-    return launch_ex(attend_kernel<T, D>, dim3(ceil_div(max_rows, 16), p.cache.heads, seqs), dim3(kAttnWarps * 32), smem,
-                     1, st, "attend_kernel", p);
+    int seq = found_seq;
+    int64_t seq_at = found_at;
+    while (u < u_end) {
+        const Sequence q = sequence(p, seq);
+        const int64_t n = (int64_t)q.tiles * q.units * p.cache.heads;
+        while (u < u_end && u < seq_at + n) {
+            const int64_t rel = u - seq_at;
+            const int pair = (int)(rel / q.units), unit = (int)(rel % q.units);
+            const int head = pair / q.tiles, row0 = pair % q.tiles * 16;
+            const int take = (int)(u_end - u < q.units - unit ? u_end - u : q.units - unit);
+            const int k0 = (q.lo & ~(kUnit - 1)) + unit * kUnit;
+            attend_piece<T, D>(p, q, seq, head, row0, k0, k0 + take * kUnit, smem);
+            float *part = take == q.units ? nullptr
+                                          : mine + sizeof(SplitHead) / 4 + (unit > 0 ? 0 : AttnLayout<D>::kPart);
+            join_warps<T, D>(p, q, head, row0, smem, part);
+            if (take < q.units && unit == 0 && tid == 0)
+                *info = SplitHead{1 + (int)ceil_div<int64_t>(q.units - take, per), seq, head, row0,
+                                  min(16, q.news * p.group - row0), q.first, {0, 0}};
+            u += take;
+            __syncthreads();
+        }
+        seq_at += n;
+        seq++;
+    }
+}
+
+// One warp a row of a tile in several parts: part 1 of CTA c, then part 0 of
+// the CTAs after it.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs p) {
+    pdl_enter();
+    const float *at = p.parts + blockIdx.x * split_floats<D>();
+    const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
+    const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (h.pieces == 0 || r >= h.rows) return;
+    const auto part = [&](int i) {
+        return at + i * split_floats<D>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D>::kPart);
+    };
+    float m = -INFINITY;
+    for (int i = lane; i < h.pieces; i += 32) m = fmaxf(m, part(i)[16 * D + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, v[D / 32] = {};
+    for (int i0 = 0; i0 < h.pieces; i0 += 32) {
+        float f = 0.f, s = 0.f;
+        if (i0 + lane < h.pieces) {
+            s = part(i0 + lane)[16 * D + 16 + r];
+            f = part_factor(part(i0 + lane)[16 * D + r], s, m);
+        }
+        const int n = min(32, h.pieces - i0);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            l += fi * __shfl_sync(0xffffffffu, s, i);
+            const float *o = part(i0 + i) + r * D;
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) {
+                const float x = o[lane + 32 * e];
+                if (fi != 0.f) v[e] += fi * x;
+            }
+        }
+    }
+    const int row = h.row0 + r;
+    write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
+}
+
+// CTAs of the split form: 0 for the whole form.  Few (sequence, head, tile)s
+// with long ranges are split over the card; enough of them, or short ranges,
+// are not.
+int split_ctas(const Cache &c, int64_t max_pages, int64_t seqs, int64_t tiles, int64_t window, int64_t most_new, int sms) {
+    int64_t keys = max_pages << c.page_log2;
+    if (window > 0 && window + most_new < keys) keys = window + most_new;
+    const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
+    if (units <= 8) return 0;
+    const int64_t all = seqs * c.heads * tiles * units;
+    const int64_t most = 4 * (int64_t)sms;
+    return (int)(all < most ? all : most);
+}
+
+template <typename K>
+int prepare_attend(K kernel, int smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    return e == cudaSuccess ? TANS_B200_OK : launch_failed("attend_kernel", e);
+}
+
+template <typename T, int D>
+int launch_attend(const AttendArgs &p, int tiles, int ctas, cudaStream_t st) {
+    constexpr int smem = AttnLayout<D>::kBytes;
+    if (!ctas) {
+        const int rc = prepare_attend(attend_kernel<T, D>, smem);
+        return rc ? rc
+                  : launch_ex(attend_kernel<T, D>, dim3(tiles, p.cache.heads, p.seqs), dim3(kAttnWarps * 32), smem, 1, st,
+                              "attend_kernel", p);
+    }
+    int rc = prepare_attend(attend_split_kernel<T, D>, smem);
+    if (!rc)
+        rc = launch_ex(attend_split_kernel<T, D>, dim3(ctas), dim3(kAttnWarps * 32), smem, 1, st, "attend_split_kernel", p);
+    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, 4), dim3(128), 0, 1, st, "attend_join_kernel", p);
 }
 
 int flat_grid(int64_t total) {
@@ -664,12 +1001,45 @@ extern "C" int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slo
     });
 }
 
+namespace {
+
+// Checks what the workspace depends on; CTAs of the split form in *ctas.
+int plan_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t tokens,
+                   int64_t most_new, int64_t window, int *ctas) {
+    int rc = check_cache("kv4_attention", cache, c);
+    if (rc) return rc;
+    if (seqs < 0 || seqs > 65535 || tokens < 0 || tokens > INT32_MAX || q_heads < 1 || q_heads % c->heads ||
+        q_heads > 65535 || most_new < 1 || max_pages < 0 || window < 0)
+        return fail(TANS_B200_ERR_INVALID,
+                    "kv4_attention: q_heads must be a multiple of the cache's heads, seqs at most 65535, most_new at "
+                    "least 1, max_pages and window not negative");
+    if (max_pages > INT32_MAX || (max_pages << c->page_log2) > INT32_MAX - 4096 ||
+        most_new > INT32_MAX || most_new * (q_heads / c->heads) > (1 << 28))
+        return fail(TANS_B200_ERR_INVALID, "kv4_attention: a sequence holds at most 2^31-4097 tokens");
+    int dev, sms;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return launch_failed("kv4_attention", e);
+    *ctas = split_ctas(*c, max_pages, seqs, ceil_div<int64_t>(most_new * (q_heads / c->heads), 16), window, most_new, sms);
+    return TANS_B200_OK;
+}
+
+int64_t workspace_floats(int64_t dim) {
+    return dim == 64 ? split_floats<64>() : (dim == 128 ? split_floats<128>() : split_floats<256>());
+}
+
+}  // namespace
+
 extern "C" int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cache, int64_t q_heads, int64_t max_pages,
                                                        int64_t seqs, int64_t tokens, int64_t most_new,
                                                        int64_t window, int64_t *bytes) {
     clear_error();
     if (!bytes) return fail(TANS_B200_ERR_INVALID, "kv4_attention: null pointer");
-    *bytes = 0;
+    Cache c;
+    int ctas = 0;
+    const int rc = plan_attention(cache, &c, q_heads, max_pages, seqs, tokens, most_new, window, &ctas);
+    if (rc) return rc;
+    *bytes = ctas * workspace_floats(cache->dim) * 4;
     return TANS_B200_OK;
 }
 
@@ -680,22 +1050,18 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
                                        void *workspace, int64_t workspace_bytes, int dtype, int32_t *status,
                                        void *stream) {
     clear_error();
+    if (tokens == 0 || seqs == 0) return TANS_B200_OK;
     AttendArgs p{};
-    int rc = check_cache("kv4_attention", cache, &p.cache);
+    int ctas = 0;
+    int rc = plan_attention(cache, &p.cache, q_heads, max_pages, seqs, tokens, most_new, window, &ctas);
     if (rc) return rc;
-    if (seqs < 0 || seqs > 65535 || tokens < 0 || tokens > INT32_MAX || q_heads < 1 ||
-        q_heads % p.cache.heads || q_heads > 65535 || most_new < 1 || max_pages < 0 || window < 0)
-        return fail(TANS_B200_ERR_INVALID,
-                    "kv4_attention: q_heads must be a multiple of the cache's heads, seqs at most 65535, most_new at "
-                    "least 1, max_pages and window not negative");
     if (!starts && tokens != seqs)
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: one new token a sequence without starts");
-    if (tokens == 0 || seqs == 0) return TANS_B200_OK;
     if (!q || !out || !lens || (!table && max_pages) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_attention: q, out (16-byte aligned, q's stride a multiple of 8), lens and table are needed");
-    if ((max_pages << p.cache.page_log2) > INT32_MAX - 64 || most_new * (q_heads / p.cache.heads) > (1 << 28))
-        return fail(TANS_B200_ERR_INVALID, "kv4_attention: a sequence holds at most 2^31-65 tokens");
+    if (workspace_bytes < ctas * workspace_floats(cache->dim) * 4 || (ctas && (!workspace || !is_aligned(workspace, 16))))
+        return fail(TANS_B200_ERR_INVALID, "kv4_attention: the workspace is too small or not 16-byte aligned");
     p.q = q;
     p.q_stride = q_stride;
     p.table = table;
@@ -704,21 +1070,23 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     p.starts = starts;
     p.out = out;
     p.lse = lse;
+    p.parts = static_cast<float *>(workspace);
     p.tokens = (int32_t)tokens;
+    p.seqs = (int32_t)seqs;
     p.group = (int32_t)(q_heads / p.cache.heads);
     p.max_pages = (int32_t)max_pages;
     p.most_new = (int32_t)most_new;
-    p.window = window > INT32_MAX ? 0 : (int32_t)window;
+    p.window = window > INT32_MAX - 1 ? 0 : (int32_t)window;
     p.scale = scale;
     p.status = status;
-    const int max_rows = (int)(most_new * p.group);
+    const int tiles = (int)ceil_div<int64_t>(most_new * p.group, 16);
     return dispatch_half(dtype, "kv4_attention", [&](auto t) {
         using T = decltype(t);
         cudaStream_t st = (cudaStream_t)stream;
         switch (cache->dim) {
-            case 64: return launch_attend<T, 64>(p, (int)seqs, max_rows, st);
-            case 128: return launch_attend<T, 128>(p, (int)seqs, max_rows, st);
-            default: return launch_attend<T, 256>(p, (int)seqs, max_rows, st);
+            case 64: return launch_attend<T, 64>(p, tiles, ctas, st);
+            case 128: return launch_attend<T, 128>(p, tiles, ctas, st);
+            default: return launch_attend<T, 256>(p, tiles, ctas, st);
         }
     });
 }
