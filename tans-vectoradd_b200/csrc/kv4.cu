@@ -23,7 +23,7 @@ struct Cache {
     uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
     const float *k_gain, *v_gain;  // [heads], null: 1
     int64_t pages;
-    int32_t heads, page_log2;
+    int32_t heads, page_log2, dim;
 };
 
 // Index of (page, head, token in page) in units of one token's head.
@@ -341,10 +341,18 @@ struct AttnLayout {
     static constexpr int kCodes = 16 * D / 2, kScales = 16 * D / 16;       // bytes of a 16-key block
     static constexpr int kBlock = 2 * (kCodes + kScales);                  // K codes, V codes, K scales, V scales
     static constexpr int kRing = kAttnWarps * kStages * kBlock;
-    static constexpr int kMerge = kAttnWarps * 16 * (D + 2) * 4;           // the warps' O, maxima and sums
+    static constexpr int kRow = D + 8;                                     // floats of a row of O: no bank conflicts
+    static constexpr int kMerge = kAttnWarps * 16 * (kRow + 2) * 4;        // the warps' O, maxima and sums
     static constexpr int kQ = D / 16 * 512;                                // Q fragments
     static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ;
+    static constexpr int kCtas = D == 256 ? 2 : 4;                         // resident on an SM
     static constexpr int kPart = 16 * (D + 2);                             // floats of a partial result
+    // 16-byte chunk c of row r of a block's codes lies in chunk k_chunk(r, c) of
+    // that row (V: v_chunk), so that the lanes of a read meet different banks
+    static __device__ int k_chunk(int r, int c) { return D == 256 ? c ^ (r & 1) : c; }
+    static __device__ int v_chunk(int r, int c) { return D == 256 ? c ^ (r & 6) : (D == 128 ? c ^ (r >> 1 & 2) : c); }
+    // place of element e in a merged row: the order of the MMA's columns
+    static __device__ int place(int e) { return e % (D / 8) * 8 + e / (D / 8); }
 };
 
 // Rows of a tile for one (sequence, head), keys k0 .. k1 (multiples of kUnit
@@ -359,7 +367,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     constexpr int kE = D / 8;              // elements of an eighth of a head
     constexpr int kVS = (D + 127) / 128;   // scales of an eighth
     constexpr int kKS = D / 64;            // scales of a quarter
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rows = q.news * p.group, row_end = min(row0 + 16, rows) - 1;
     const auto last_key = [&](int row) { return q.len - q.news + row / p.group; };
     const auto first_key = [&](int last) { return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0; };
@@ -370,7 +378,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     int lo[2], hi[2];
     uint8_t *ring = smem + warp * (kStages * L::kBlock);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
-    float to_log2[2];
+    float to_log2[2];  // positive: its sign goes into Q, and 0 becomes a number that no score can raise above 2^-20
     {
         const float c = p.scale * kLog2e * (p.cache.k_gain ? p.cache.k_gain[head] : 1.f);
         // Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
@@ -384,7 +392,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
                            ((int64_t)head * p.group + row % p.group) * D + t * (D / 4);
 #pragma unroll
             for (int j = 0; j < kSteps; j++) u[i][j] = *reinterpret_cast<const uint2 *>(src + 4 * j);
-            to_log2[i] = c;
+            to_log2[i] = fabsf(c);
+            const uint32_t flip = c < 0.f ? 0x80008000u : 0u;
             if constexpr (!std::is_same_v<T, __half>) {
                 float top = 0.f;
 #pragma unroll
@@ -398,7 +407,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
                 int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // top * 2^k in [2^14, 2^15)
                 k = top == 0.f || top > 3.4e38f ? 0 : min(k, 100);
                 const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-                to_log2[i] = c * __uint_as_float((uint32_t)(127 - k) << 23);
+                to_log2[i] *= __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
                 for (int j = 0; j < kSteps; j++) {
                     const T *e = reinterpret_cast<const T *>(&u[i][j]);
@@ -406,6 +415,9 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
                                          h2_of(to_f32(e[2]) * up, to_f32(e[3]) * up));
                 }
             }
+            to_log2[i] = max_nan(to_log2[i], 1e-37f);
+#pragma unroll
+            for (int j = 0; j < kSteps; j++) u[i][j].x ^= flip, u[i][j].y ^= flip;
         }
         if (warp == 0) {
 #pragma unroll
@@ -415,37 +427,52 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     __syncthreads();
 
     const int32_t *table = p.table + (int64_t)seq * p.table_stride;
-    const int in_page = (1 << p.cache.page_log2) - 1;
+    const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
+    const bool whole_pages = page_log2 >= 4;  // a block lies in one page
     const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
+    const int c16 = lane % (D / 32);  // this lane's 16-byte chunk of a token's codes
+    const uint8_t *scales = lane < 16 ? p.cache.k_scales : p.cache.v_scales;
     // the page of key base + (lane & 15), loaded a block ahead of its use
     const auto page_of = [&](int base) -> int {
-        const int key = base + (lane & 15);
-        return base < k1 && key >= lo_all && key <= hi_all ? table[key >> p.cache.page_log2] : 0;
+        return base < k1 && hi_all >= lo_all
+                   ? table[max(lo_all, min(base + (whole_pages ? 0 : lane & 15), hi_all)) >> page_log2]
+                   : 0;
     };
-    // start the copies of the block at `base` (its keys' pages in `pages`) into `stage`
-    const auto fetch = [&](int base, int pages, int stage) {
+    // start the copies of the block at `base` (its keys' pages in `page`) into `stage`
+    const auto fetch = [&](int base, int page, int stage) {
         if (base < k1) {
-            if ((pages < 0 || pages >= p.cache.pages) && p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            const bool ok = pages >= 0 && pages < p.cache.pages;
-            const int pg = ok ? pages : 0;
-            const uint32_t dst = ring_sa + (uint32_t)stage * L::kBlock;
-            constexpr int kRow = D / 32;  // 16-byte chunks of a token's codes
-#pragma unroll
-            for (int i = 0; i < 16 * kRow / 32; i++) {
-                const int r = (lane + 32 * i) / kRow, c = lane % kRow, key = base + r;
-                const int64_t at = token_at(p.cache, __shfl_sync(0xffffffffu, pg, r), head, key & in_page);
-                const bool real = key >= lo_all && key <= hi_all;
-                const int64_t off = real ? at * (D / 2) + 16 * c : 0;
-                copy_async<16>(dst + r * (D / 2) + 16 * c, p.cache.k_codes + off, real);
-                // V chunks change places so that four keys' reads meet different banks
-                const int cv = D == 128 ? c ^ (r >> 1 & 2) : c;
-                copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * cv, p.cache.v_codes + off, real);
+            if ((uint64_t)(int64_t)page >= (uint64_t)p.cache.pages) {
+                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+                page = 0;
             }
-            const int r = lane & 15, key = base + r;
-            const bool real = key >= lo_all && key <= hi_all;
-            const int64_t off = real ? token_at(p.cache, pg, head, key & in_page) * (D / 16) : 0;
-            const uint8_t *src = lane < 16 ? p.cache.k_scales : p.cache.v_scales;
-            copy_async<D / 16>(dst + 2 * L::kCodes + (lane >> 4) * L::kScales + r * (D / 16), src + off, real);
+            const uint32_t dst = ring_sa + (uint32_t)stage * L::kBlock;
+            const uint32_t dst_s = dst + 2 * L::kCodes + lane * (D / 16);
+            if (whole_pages && base >= lo_all && base + 15 <= hi_all) {
+                const int64_t at = token_at(p.cache, page, head, base & in_page);
+                const uint8_t *k = p.cache.k_codes + at * (D / 2) + 16 * lane;
+                const uint8_t *v = p.cache.v_codes + at * (D / 2) + 16 * lane;
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) {
+                    const int r = (lane + 32 * i) / (D / 32);
+                    copy_async<16>(dst + r * (D / 2) + 16 * L::k_chunk(r, c16), k + 512 * i, true);
+                    copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), v + 512 * i, true);
+                }
+                copy_async<D / 16>(dst_s, scales + (at + (lane & 15)) * (D / 16), true);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) {
+                    const int r = (lane + 32 * i) / (D / 32), key = base + r;
+                    const int64_t at = token_at(p.cache, __shfl_sync(0xffffffffu, page, r), head, key & in_page);
+                    const bool real = key >= lo_all && key <= hi_all;
+                    const int64_t off = real ? at * (D / 2) + 16 * c16 : 0;
+                    copy_async<16>(dst + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
+                    copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), p.cache.v_codes + off, real);
+                }
+                const int key = base + (lane & 15);
+                const bool real = key >= lo_all && key <= hi_all;
+                const int64_t off = real ? token_at(p.cache, page, head, key & in_page) * (D / 16) : 0;
+                copy_async<D / 16>(dst_s, scales + off, real);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -453,25 +480,24 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     float o[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    // the running maximum, what is subtracted (it, or 0 while it is -inf), the sums
+    float top[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
 
-    int base = k0 + 16 * warp, ahead = base, stage = 0;
-    int pages = page_of(ahead);
+    int base = k0 + 16 * warp, stage = 0;
+    int page = page_of(base);
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) {
-        const int now = pages;
-        pages = page_of(ahead + kUnit);
-        fetch(ahead, now, i);
-        ahead += kUnit;
+        const int now = page;
+        page = page_of(base + (i + 1) * kUnit);
+        fetch(base + i * kUnit, now, i);
     }
     for (; base < k1; base += kUnit) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
         {
-            const int now = pages;
-            pages = page_of(ahead + kUnit);
-            fetch(ahead, now, stage == 0 ? kStages - 1 : stage - 1);
-            ahead += kUnit;
+            const int now = page;
+            page = page_of(base + kStages * kUnit);
+            fetch(base + (kStages - 1) * kUnit, now, stage == 0 ? kStages - 1 : stage - 1);
         }
         const uint8_t *blk = ring + stage * L::kBlock;
         if (++stage == kStages) stage = 0;
@@ -479,66 +505,72 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         // lanes t = 0..3 then fall on rows of both parities.
         // ---- scores of 16 keys
         float s[2][4] = {};
+        {
+            uint32_t w[2][D / 32], f[2][kKS];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = 8 * h + (g ^ (g >> 1 & 1));
-            uint32_t w[D / 32], f[kKS];
-            if constexpr (D == 64) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(blk + r * (D / 2) + t * (D / 8));
-                w[0] = v.x, w[1] = v.y;
-            } else {
+            for (int h = 0; h < 2; h++) {
+                const int r = 8 * h + (g ^ (g >> 1 & 1));
+                const uint8_t *kp = blk + r * (D / 2);
+                if constexpr (D == 64) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(kp + 8 * t);
+                    w[h][0] = v.x, w[h][1] = v.y;
+                } else {
 #pragma unroll
-                for (int i = 0; i < D / 128; i++) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(blk + r * (D / 2) + t * (D / 8) + 16 * i);
-                    w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                    for (int i = 0; i < D / 128; i++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(kp + 16 * L::k_chunk(r, t * (D / 128) + i));
+                        w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
+                    }
                 }
-            }
-            const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
-            if constexpr (kKS == 1) {
-                f[0] = e4m3x2_h2(*sp * 0x101u);
-            } else {
+                const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
+                if constexpr (kKS == 1) {
+                    f[h][0] = e4m3x2_h2(*sp * 0x101u);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kKS; i += 2) {
-                    const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
-                    f[i] = __byte_perm(two, two, 0x1010);
-                    f[i + 1] = __byte_perm(two, two, 0x3232);
+                    for (int i = 0; i < kKS; i += 2) {
+                        const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
+                        f[h][i] = __byte_perm(two, two, 0x1010);
+                        f[h][i + 1] = __byte_perm(two, two, 0x3232);
+                    }
                 }
             }
 #pragma unroll
             for (int j = 0; j < kSteps; j += 2) {
-                uint32_t b[4];
-                e2m1x8_h2(w[j / 2], b);
+                const uint4 qa = qs[j * 32 + lane], qb = qs[(j + 1) * 32 + lane];
 #pragma unroll
-                for (int i = 0; i < 4; i++) b[i] = mul_h2(b[i], f[j / 4]);
-                mma_f16(s[h], qs[j * 32 + lane], b[0], b[1]);
-                mma_f16(s[h], qs[(j + 1) * 32 + lane], b[2], b[3]);
+                for (int h = 0; h < 2; h++) {
+                    uint32_t b[4];
+                    e2m1x8_h2(w[h][j / 2], b);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) b[i] = mul_h2(b[i], f[h][j / 4]);
+                    mma_f16(s[h], qa, b[0], b[1]);
+                    mma_f16(s[h], qb, b[2], b[3]);
+                }
             }
         }
         // ---- the running maximum and the weights
         const bool edge = base < lo_in || base + 15 > hi_in;
-        bool grew = false;
+        if (edge) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int i = c >> 1;
-                float v = s[h][c] * to_log2[i];
-                if (edge) {
+                for (int c = 0; c < 4; c++) {
                     const int key = base + 8 * h + ((2 * t + (c & 1)) ^ (t & 1));
-                    if (key < lo[i] || key > hi[i]) v = -INFINITY;
+                    if (key < lo[c >> 1] || key > hi[c >> 1]) s[h][c] = -INFINITY;
                 }
-                s[h][c] = v;
-                grew |= v > top[i] + 8.f;
-            }
-        if (__any_sync(0xffffffffu, grew)) {
+        }
+        float m[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            m[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1])) * to_log2[i];
+        if (__any_sync(0xffffffffu, m[0] > top[0] + 8.f || m[1] > top[1] + 8.f)) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float m = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-                m = fmaxf(m, top[i]);
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const float f = m == -INFINITY ? 1.f : exp2f(top[i] - m);
-                top[i] = m;
+                float n = fmaxf(m[i], top[i]);
+                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 1));
+                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2));
+                less[i] = n == -INFINITY ? 0.f : n;
+                const float f = exp2f(top[i] - less[i]);  // nothing to scale yet while top is -inf
+                top[i] = n;
                 sum[i] *= f;
 #pragma unroll
                 for (int j = 0; j < kTiles; j++) {
@@ -551,9 +583,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                const int i = c >> 1;
-                s[h][c] = exp2_fast(s[h][c] - (top[i] == -INFINITY ? 0.f : top[i]));
-                sum[i] += s[h][c];
+                s[h][c] = exp2_fast(__fmaf_rn(s[h][c], to_log2[c >> 1], -less[c >> 1]));
+                sum[c >> 1] += s[h][c];
             }
         const uint4 pf = make_uint4(h2_of(s[0][0], s[0][1]), h2_of(s[0][2], s[0][3]), h2_of(s[1][0], s[1][1]),
                                     h2_of(s[1][2], s[1][3]));
@@ -566,10 +597,10 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
             if constexpr (D == 64) {
                 w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
             } else if constexpr (D == 128) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(vp + ((8 * g) ^ ((r >> 1 & 2) << 4)));
+                const uint2 v = *reinterpret_cast<const uint2 *>(vp + 16 * L::v_chunk(r, g >> 1) + 8 * (g & 1));
                 w[k][0] = v.x, w[k][1] = v.y;
             } else {
-                const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
+                const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * L::v_chunk(r, g));
                 w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
             }
 #pragma unroll
@@ -578,26 +609,20 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         }
         // A NaN scale on a key that only some rows see must not reach the
         // others as 0 * NaN: its values count as 0 here and are added below.
-        bool nan_key = false;
+        uint32_t nan_keys = 0;
         if (edge) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int i = 0; i < kVS; i++) nan_key |= (sc[k][i] & 0x7Fu) == 0x7Fu;
-            nan_key = __any_sync(0xffffffffu, nan_key);
+                for (int i = 0; i < kVS; i++)
+                    if ((sc[k][i] & 0x7Fu) == 0x7Fu) {
+                        nan_keys |= 1u << (k * kVS + i);
+                        sc[k][i] = 0;
+                    }
         }
 #pragma unroll
         for (int i = 0; i < kVS; i++) {
-            uint32_t f[2];
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                uint32_t lo8 = sc[2 * b][i], hi8 = sc[2 * b + 1][i];
-                if (nan_key) {
-                    if ((lo8 & 0x7Fu) == 0x7Fu) lo8 = 0;
-                    if ((hi8 & 0x7Fu) == 0x7Fu) hi8 = 0;
-                }
-                f[b] = e4m3x2_h2(lo8 | hi8 << 8);
-            }
+            const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
             constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
 #pragma unroll
             for (int j = 0; j < kPer; j += 8) {
@@ -616,7 +641,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
                 }
             }
         }
-        if (nan_key) {
+        if (edge && __any_sync(0xffffffffu, nan_keys)) {
             uint32_t seen[4];
 #pragma unroll
             for (int h = 0; h < 2; h++)
@@ -630,8 +655,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
                 uint32_t b[2];
 #pragma unroll
                 for (int x = 0; x < 2; x++)
-                    b[x] = h2_of((sc[2 * x][i] & 0x7Fu) == 0x7Fu ? 1.f : 0.f,
-                                 (sc[2 * x + 1][i] & 0x7Fu) == 0x7Fu ? 1.f : 0.f);
+                    b[x] = h2_of(nan_keys >> (2 * x * kVS + i) & 1 ? 1.f : 0.f,
+                                 nan_keys >> ((2 * x + 1) * kVS + i) & 1 ? 1.f : 0.f);
                 float n[4] = {};
                 mma_f16(n, make_uint4(seen[0], seen[1], seen[2], seen[3]), b[0], b[1]);
                 constexpr int kPer = kE < 16 ? kE : 16;
@@ -649,7 +674,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float *merge = reinterpret_cast<float *>(smem);
-    float *tops = merge + kAttnWarps * 16 * D, *sums = tops + kAttnWarps * 16;
+    float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
@@ -658,13 +683,11 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
             tops[warp * 16 + g + 8 * i] = top[i];
             sums[warp * 16 + g + 8 * i] = sum[i];
         }
+#pragma unroll
+        for (int j = 0; j < kTiles; j++)  // tile j, columns 2t and 2t + 1
+            *reinterpret_cast<float2 *>(merge + (warp * 16 + g + 8 * i) * L::kRow + 8 * j + 2 * t) =
+                make_float2(o[j][2 * i], o[j][2 * i + 1]);
     }
-    // tile j, column n of the MMA is element n * kE + j: two columns a lane
-#pragma unroll
-    for (int j = 0; j < kTiles; j++)
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-            merge[(warp * 16 + g + 8 * (c >> 1)) * D + (2 * t + (c & 1)) * kE + j] = o[j][c];
     __syncthreads();
 }
 
@@ -694,7 +717,8 @@ template <typename T, int D>
 __device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &q, int head, int row0, const uint8_t *smem,
                                            float *part) {
     const float *merge = reinterpret_cast<const float *>(smem);
-    const float *tops = merge + kAttnWarps * 16 * D, *sums = tops + kAttnWarps * 16;
+    using L = AttnLayout<D>;
+    const float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = min(16, q.news * p.group - row0);
     for (int r = warp; r < rows; r += kAttnWarps) {
@@ -711,7 +735,7 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &
             v[i] = 0.f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; w++)
-                if (f[w] != 0.f) v[i] += f[w] * merge[(w * 16 + r) * D + lane + 32 * i];
+                if (f[w] != 0.f) v[i] += f[w] * merge[(w * 16 + r) * L::kRow + L::place(lane + 32 * i)];
         }
         if (part) {
 #pragma unroll
@@ -729,7 +753,7 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &
 
 // One CTA a (tile, head, sequence), over all its keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) attend_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
     const int seq = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * 16;
@@ -758,7 +782,7 @@ __host__ __device__ constexpr int64_t split_floats() {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) attend_split_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_split_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int64_t warp_sum[kAttnWarps], found_at;
     __shared__ int found_seq;
@@ -836,41 +860,46 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attend_split_kernel(const Att
     }
 }
 
-// One warp a row of a tile in several parts: part 1 of CTA c, then part 0 of
-// the CTAs after it.
+// One CTA a row of a tile in several parts: part 1 of CTA c, then part 0 of
+// the CTAs after it, every eighth for each warp.
+constexpr int kJoinWarps = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
+    __shared__ float tops[kJoinWarps], sums[kJoinWarps], o[kJoinWarps][D];
     pdl_enter();
     const float *at = p.parts + blockIdx.x * split_floats<D>();
     const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
-    const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (h.pieces == 0 || r >= h.rows) return;
     const auto part = [&](int i) {
         return at + i * split_floats<D>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D>::kPart);
     };
-    float m = -INFINITY;
-    for (int i = lane; i < h.pieces; i += 32) m = fmaxf(m, part(i)[16 * D + r]);
+    float m = -INFINITY, l = 0.f, v[D / 32] = {};
+    for (int i = threadIdx.x; i < h.pieces; i += kJoinWarps * 32) m = fmaxf(m, part(i)[16 * D + r]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, v[D / 32] = {};
-    for (int i0 = 0; i0 < h.pieces; i0 += 32) {
-        float f = 0.f, s = 0.f;
-        if (i0 + lane < h.pieces) {
-            s = part(i0 + lane)[16 * D + 16 + r];
-            f = part_factor(part(i0 + lane)[16 * D + r], s, m);
-        }
-        const int n = min(32, h.pieces - i0);
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+    for (int w = 0; w < kJoinWarps; w++) m = fmaxf(m, tops[w]);
 #pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const float fi = __shfl_sync(0xffffffffu, f, i);
-            l += fi * __shfl_sync(0xffffffffu, s, i);
-            const float *o = part(i0 + i) + r * D;
+    for (int i = warp; i < h.pieces; i += kJoinWarps) {
+        const float *x = part(i);
+        const float s = x[16 * D + 16 + r], f = part_factor(x[16 * D + r], s, m);
+        l += f * s;
 #pragma unroll
-            for (int e = 0; e < D / 32; e++) {
-                const float x = o[lane + 32 * e];
-                if (fi != 0.f) v[e] += fi * x;
-            }
-        }
+        for (int e = 0; e < D / 32; e++) v[e] += f == 0.f ? 0.f : f * x[r * D + lane + 32 * e];
+    }
+    if (lane == 0) sums[warp] = l;
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) o[warp][lane + 32 * e] = v[e];
+    __syncthreads();
+    if (warp) return;
+    l = 0.f;
+    for (int w = 0; w < kJoinWarps; w++) l += sums[w];
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) {
+        v[e] = 0.f;
+        for (int w = 0; w < kJoinWarps; w++) v[e] += o[w][lane + 32 * e];
     }
     const int row = h.row0 + r;
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
@@ -885,7 +914,7 @@ int split_ctas(const Cache &c, int64_t max_pages, int64_t seqs, int64_t tiles, i
     const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
     if (units <= 8) return 0;
     const int64_t all = seqs * c.heads * tiles * units;
-    const int64_t most = 4 * (int64_t)sms;
+    const int64_t most = (c.dim == 256 ? AttnLayout<256>::kCtas : AttnLayout<128>::kCtas) * (int64_t)sms;
     return (int)(all < most ? all : most);
 }
 
@@ -896,18 +925,19 @@ int prepare_attend(K kernel, int smem) {
 }
 
 template <typename T, int D>
-int launch_attend(const AttendArgs &p, int tiles, int ctas, cudaStream_t st) {
+int launch_attend(const AttendArgs &p, int max_rows, int ctas, cudaStream_t st) {
     constexpr int smem = AttnLayout<D>::kBytes;
     if (!ctas) {
         const int rc = prepare_attend(attend_kernel<T, D>, smem);
         return rc ? rc
-                  : launch_ex(attend_kernel<T, D>, dim3(tiles, p.cache.heads, p.seqs), dim3(kAttnWarps * 32), smem, 1, st,
+                  : launch_ex(attend_kernel<T, D>, dim3(ceil_div(max_rows, 16), p.cache.heads, p.seqs), dim3(kAttnWarps * 32), smem, 1, st,
                               "attend_kernel", p);
     }
     int rc = prepare_attend(attend_split_kernel<T, D>, smem);
     if (!rc)
         rc = launch_ex(attend_split_kernel<T, D>, dim3(ctas), dim3(kAttnWarps * 32), smem, 1, st, "attend_split_kernel", p);
-    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, 4), dim3(128), 0, 1, st, "attend_join_kernel", p);
+    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, max_rows < 16 ? max_rows : 16),
+                               dim3(kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
 }
 
 int flat_grid(int64_t total) {
@@ -928,7 +958,7 @@ int check_cache(const char *what, const tans_b200_kv4 *c, Cache *out) {
         !is_aligned(c->v_scales, 16))
         return fail(TANS_B200_ERR_INVALID, "%s: cache arrays must be 16-byte aligned", what);
     *out = Cache{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->k_gain, c->v_gain, c->pages,
-                 (int32_t)c->heads, __builtin_ctz((unsigned)c->page_size)};
+                 (int32_t)c->heads, __builtin_ctz((unsigned)c->page_size), (int32_t)c->dim};
     return TANS_B200_OK;
 }
 
@@ -1079,14 +1109,14 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     p.window = window > INT32_MAX - 1 ? 0 : (int32_t)window;
     p.scale = scale;
     p.status = status;
-    const int tiles = (int)ceil_div<int64_t>(most_new * p.group, 16);
+    const int rows = (int)(most_new * p.group);
     return dispatch_half(dtype, "kv4_attention", [&](auto t) {
         using T = decltype(t);
         cudaStream_t st = (cudaStream_t)stream;
         switch (cache->dim) {
-            case 64: return launch_attend<T, 64>(p, tiles, ctas, st);
-            case 128: return launch_attend<T, 128>(p, tiles, ctas, st);
-            default: return launch_attend<T, 256>(p, tiles, ctas, st);
+            case 64: return launch_attend<T, 64>(p, rows, ctas, st);
+            case 128: return launch_attend<T, 128>(p, rows, ctas, st);
+            default: return launch_attend<T, 256>(p, rows, ctas, st);
         }
     });
 }
