@@ -351,16 +351,45 @@ struct AttnLayout {
     // that row (V: v_chunk), so that the lanes of a read meet different banks
     static __device__ int k_chunk(int r, int c) { return D == 256 ? c ^ (r & 1) : c; }
     static __device__ int v_chunk(int r, int c) { return D == 256 ? c ^ (r & 6) : (D == 128 ? c ^ (r >> 1 & 2) : c); }
+    static constexpr bool kSameChunks = D != 256;  // v_chunk of rows 512 bytes apart is the same
     // place of element e in a merged row: the order of the MMA's columns
     static __device__ int place(int e) { return e % (D / 8) * 8 + e / (D / 8); }
 };
 
-// Rows of a tile for one (sequence, head), keys k0 .. k1 (multiples of kUnit
-// from the sequence's first unit): the four warps' results lie in `merge`
-// afterwards as [warp][16][D] O, [warp][16] maxima, [warp][16] sums.
+// One piece of a tile's work, in shared memory.
+struct Piece {
+    Sequence q;
+    int seq, head, row0;
+    int k0, k1;  // keys, multiples of kUnit
+    // keys that some row of the tile sees, and those that every row sees
+    int lo_all, hi_all, lo_in, hi_in;
+    int hi[16];  // the last key that each row sees
+};
+
+__device__ __forceinline__ int first_seen(const AttendArgs &p, int last) {
+    return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0;
+}
+
+// Fills in what follows from q, row0, k0 and k1; called by one whole warp, lane r < 16 for row r.
+__device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
+    const int lane = threadIdx.x & 31;
+    const int end = min(x.row0 + 16, x.q.news * p.group) - 1;
+    const auto last_key = [&](int row) { return x.q.len - x.q.news + row / p.group; };
+    if (lane < 16) x.hi[lane] = last_key(min(x.row0 + lane, end));
+    if (lane == 0) {
+        x.hi_in = last_key(x.row0);
+        x.hi_all = last_key(end);
+        x.lo_all = first_seen(p, x.hi_in);
+        x.lo_in = first_seen(p, x.hi_all);
+        x.k0 = max(x.k0, x.lo_all & ~(kUnit - 1));
+        x.k1 = min(x.k1, (x.hi_all & ~(kUnit - 1)) + kUnit);
+    }
+}
+
+// Runs a piece (set by the caller, before a block barrier): afterwards the four
+// warps' results lie in `smem` as [warp][16][kRow] O, [warp][16] maxima and sums.
 template <typename T, int D>
-__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence &q, int seq, int head, int row0, int k0,
-                                             int k1, uint8_t *smem) {
+__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem) {
     using L = AttnLayout<D>;
     constexpr int kSteps = D / 16;         // MMA steps of S
     constexpr int kTiles = D / 8;          // MMA column tiles of O
@@ -368,27 +397,89 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
     constexpr int kVS = (D + 127) / 128;   // scales of an eighth
     constexpr int kKS = D / 64;            // scales of a quarter
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rows = q.news * p.group, row_end = min(row0 + 16, rows) - 1;
-    const auto last_key = [&](int row) { return q.len - q.news + row / p.group; };
-    const auto first_key = [&](int last) { return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0; };
-    // keys lo[i] .. hi[i] are those of this lane's two rows; lo_all .. hi_all cover
-    // the tile, lo_in .. hi_in are seen by every row of it
-    const int lo_all = first_key(last_key(row0)), hi_all = last_key(row_end);
-    const int lo_in = first_key(last_key(row_end)), hi_in = last_key(row0);
-    int lo[2], hi[2];
-    uint8_t *ring = smem + warp * (kStages * L::kBlock);
+    const int head = x.head, k1 = x.k1, lo_all = x.lo_all, hi_all = x.hi_all;
+    const uint8_t *ring = smem + warp * (kStages * L::kBlock);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
-    float to_log2[2];  // positive: its sign goes into Q, and 0 becomes a number that no score can raise above 2^-20
+
+    // ---- copies of 16-key blocks into the warp's ring
+    const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
+    const int32_t *table = p.table + (int64_t)x.seq * p.table_stride;
+    const int c16 = lane % (D / 32);                                // this lane's 16-byte chunk of a token's codes
+    const int r16 = lane & 15;                                      // the token whose scales it copies
+    const int64_t head_at = (int64_t)head << page_log2;
+    const uint8_t *k_src = p.cache.k_codes + head_at * (D / 2) + 16 * lane;
+    const uint8_t *v_src = p.cache.v_codes + head_at * (D / 2) + 16 * lane;
+    const uint8_t *s_src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + (head_at + r16) * (D / 16);
+    const uint32_t page_tokens = (uint32_t)p.cache.heads << page_log2;
+    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
+    const uint32_t k_dst = ring_sa + lane / (D / 32) * (D / 2) + 16 * L::k_chunk(lane / (D / 32), c16);
+    const uint32_t v_dst = ring_sa + L::kCodes + lane / (D / 32) * (D / 2) + 16 * L::v_chunk(lane / (D / 32), c16);
+    // blocks within one page whose keys all exist: first .. first + span
+    const bool whole_pages = page_log2 >= 4;
+    const int easy = lo_all, easy_span = whole_pages ? hi_all - 15 - lo_all : -1;
+    // the page of key base + r16, or with whole pages of the block, loaded ahead of its use
+    const auto page_of = [&](int base) -> int {
+        return base < k1 ? table[max(lo_all, min(whole_pages ? base : base + r16, hi_all)) >> page_log2] : 0;
+    };
+    // start the copies of the block at `base`, its keys' pages in `page`, `at` bytes into the ring
+    const auto fetch = [&](int base, int page, uint32_t at) {
+        if (base < k1) {
+            if ((uint32_t)page >= (uint32_t)p.cache.pages) {
+                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+                page = 0;
+            }
+            const uint32_t s_dst = ring_sa + 2 * L::kCodes + lane * (D / 16) + at;
+            if (base >= easy && base - easy <= easy_span) {
+                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(base & in_page);
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) {
+                    copy_async<16>(k_dst + at + 512 * i, k_src + tok * (D / 2) + 512 * i, true);
+                    copy_async<16>(L::kSameChunks ? v_dst + at + 512 * i
+                                                  : ring_sa + at + L::kCodes + (lane + 32 * i) / (D / 32) * (D / 2) +
+                                                        16 * L::v_chunk((lane + 32 * i) / (D / 32), c16),
+                                   v_src + tok * (D / 2) + 512 * i, true);
+                }
+                copy_async<D / 16>(s_dst, s_src + tok * (D / 16), true);
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < D / 64; i++) {
+                    const int r = (lane + 32 * i) / (D / 32), key = base + r;
+                    const bool real = key >= lo_all && key <= hi_all;
+                    const uint32_t pg = (uint32_t)__shfl_sync(0xffffffffu, page, r);
+                    const uint64_t tok = head_at + (uint64_t)pg * page_tokens + (uint32_t)(key & in_page);
+                    const uint64_t off = real ? tok * (D / 2) + 16 * c16 : 0;
+                    copy_async<16>(ring_sa + at + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
+                    copy_async<16>(ring_sa + at + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16),
+                                   p.cache.v_codes + off, real);
+                }
+                const int key = base + r16;
+                const bool real = key >= lo_all && key <= hi_all;
+                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(key & in_page);
+                // s_src stands r16 tokens into the head's first page
+                copy_async<D / 16>(s_dst, s_src + (real ? (int64_t)(tok - r16) * (D / 16) : 0), real);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int base = x.k0 + 16 * warp;
+    int page = page_of(base);
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; i++) {
+        const int now = page;
+        page = page_of(base + (i + 1) * kUnit);
+        fetch(base + i * kUnit, now, i * L::kBlock);
+    }
+
+    // ---- Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
+    float to_log2[2];  // positive: its sign goes into Q, and 0 becomes a number that lifts no score above 2^-20
     {
         const float c = p.scale * kLog2e * (p.cache.k_gain ? p.cache.k_gain[head] : 1.f);
-        // Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
+        const int end = min(x.row0 + 16, x.q.news * p.group) - 1;
         uint2 u[2][kSteps];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int row = min(row0 + g + 8 * i, row_end);
-            hi[i] = last_key(row);
-            lo[i] = first_key(hi[i]);
-            const T *src = static_cast<const T *>(p.q) + (int64_t)(q.first + row / p.group) * p.q_stride +
+            const int row = min(x.row0 + g + 8 * i, end);
+            const T *src = static_cast<const T *>(p.q) + (int64_t)(x.q.first + row / p.group) * p.q_stride +
                            ((int64_t)head * p.group + row % p.group) * D + t * (D / 4);
 #pragma unroll
             for (int j = 0; j < kSteps; j++) u[i][j] = *reinterpret_cast<const uint2 *>(src + 4 * j);
@@ -425,82 +516,25 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         }
     }
     __syncthreads();
-
-    const int32_t *table = p.table + (int64_t)seq * p.table_stride;
-    const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
-    const bool whole_pages = page_log2 >= 4;  // a block lies in one page
-    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
-    const int c16 = lane % (D / 32);  // this lane's 16-byte chunk of a token's codes
-    const uint8_t *scales = lane < 16 ? p.cache.k_scales : p.cache.v_scales;
-    // the page of key base + (lane & 15), loaded a block ahead of its use
-    const auto page_of = [&](int base) -> int {
-        return base < k1 && hi_all >= lo_all
-                   ? table[max(lo_all, min(base + (whole_pages ? 0 : lane & 15), hi_all)) >> page_log2]
-                   : 0;
-    };
-    // start the copies of the block at `base` (its keys' pages in `page`) into `stage`
-    const auto fetch = [&](int base, int page, int stage) {
-        if (base < k1) {
-            if ((uint64_t)(int64_t)page >= (uint64_t)p.cache.pages) {
-                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-                page = 0;
-            }
-            const uint32_t dst = ring_sa + (uint32_t)stage * L::kBlock;
-            const uint32_t dst_s = dst + 2 * L::kCodes + lane * (D / 16);
-            if (whole_pages && base >= lo_all && base + 15 <= hi_all) {
-                const int64_t at = token_at(p.cache, page, head, base & in_page);
-                const uint8_t *k = p.cache.k_codes + at * (D / 2) + 16 * lane;
-                const uint8_t *v = p.cache.v_codes + at * (D / 2) + 16 * lane;
-#pragma unroll
-                for (int i = 0; i < D / 64; i++) {
-                    const int r = (lane + 32 * i) / (D / 32);
-                    copy_async<16>(dst + r * (D / 2) + 16 * L::k_chunk(r, c16), k + 512 * i, true);
-                    copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), v + 512 * i, true);
-                }
-                copy_async<D / 16>(dst_s, scales + (at + (lane & 15)) * (D / 16), true);
-            } else {
-#pragma unroll
-                for (int i = 0; i < D / 64; i++) {
-                    const int r = (lane + 32 * i) / (D / 32), key = base + r;
-                    const int64_t at = token_at(p.cache, __shfl_sync(0xffffffffu, page, r), head, key & in_page);
-                    const bool real = key >= lo_all && key <= hi_all;
-                    const int64_t off = real ? at * (D / 2) + 16 * c16 : 0;
-                    copy_async<16>(dst + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
-                    copy_async<16>(dst + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), p.cache.v_codes + off, real);
-                }
-                const int key = base + (lane & 15);
-                const bool real = key >= lo_all && key <= hi_all;
-                const int64_t off = real ? token_at(p.cache, page, head, key & in_page) * (D / 16) : 0;
-                copy_async<D / 16>(dst_s, scales + off, real);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
+    const int inner = x.lo_in, inner_span = x.hi_in - 15 - x.lo_in;  // blocks that every row sees whole
 
     float o[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    // the running maximum, what is subtracted (it, or 0 while it is -inf), the sums
-    float top[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-
-    int base = k0 + 16 * warp, stage = 0;
-    int page = page_of(base);
-#pragma unroll
-    for (int i = 0; i < kStages - 1; i++) {
-        const int now = page;
-        page = page_of(base + (i + 1) * kUnit);
-        fetch(base + i * kUnit, now, i);
-    }
+    // scores up to this need no new maximum; what is subtracted; the sums
+    float limit[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+    uint32_t at = 0;  // the block's place in the ring, in bytes
+#pragma unroll 1
     for (; base < k1; base += kUnit) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
         {
             const int now = page;
             page = page_of(base + kStages * kUnit);
-            fetch(base + (kStages - 1) * kUnit, now, stage == 0 ? kStages - 1 : stage - 1);
+            fetch(base + (kStages - 1) * kUnit, now, at == 0 ? (kStages - 1) * L::kBlock : at - L::kBlock);
         }
-        const uint8_t *blk = ring + stage * L::kBlock;
-        if (++stage == kStages) stage = 0;
+        const uint8_t *blk = ring + at;
+        at = at == (kStages - 1) * L::kBlock ? 0 : at + L::kBlock;
         // Column n of an 8-key half is key n ^ (n >> 1 & 1): the V reads of
         // lanes t = 0..3 then fall on rows of both parities.
         // ---- scores of 16 keys
@@ -548,29 +582,32 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
             }
         }
         // ---- the running maximum and the weights
-        const bool edge = base < lo_in || base + 15 > hi_in;
+        const bool edge = base < inner || base - inner > inner_span;
         if (edge) {
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int i = 0; i < 2; i++) {
+                const int hi = x.hi[g + 8 * i], lo = first_seen(p, hi);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int key = base + 8 * h + ((2 * t + (c & 1)) ^ (t & 1));
-                    if (key < lo[c >> 1] || key > hi[c >> 1]) s[h][c] = -INFINITY;
+                    const int key = base + 8 * (c >> 1) + ((2 * t + (c & 1)) ^ (t & 1));
+                    if (key < lo || key > hi) s[c >> 1][2 * i + (c & 1)] = -INFINITY;
                 }
+            }
         }
         float m[2];
 #pragma unroll
         for (int i = 0; i < 2; i++)
             m[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1])) * to_log2[i];
-        if (__any_sync(0xffffffffu, m[0] > top[0] + 8.f || m[1] > top[1] + 8.f)) {
+        if (__any_sync(0xffffffffu, m[0] > limit[0] || m[1] > limit[1])) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float n = fmaxf(m[i], top[i]);
+                const float top = limit[i] == -INFINITY ? -INFINITY : less[i];
+                float n = fmaxf(m[i], top);
                 n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 1));
                 n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2));
+                limit[i] = n + 8.f;
                 less[i] = n == -INFINITY ? 0.f : n;
-                const float f = exp2f(top[i] - less[i]);  // nothing to scale yet while top is -inf
-                top[i] = n;
+                const float f = exp2f(top - less[i]);  // nothing to scale yet while top is -inf
                 sum[i] *= f;
 #pragma unroll
                 for (int j = 0; j < kTiles; j++) {
@@ -644,12 +681,14 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         if (edge && __any_sync(0xffffffffu, nan_keys)) {
             uint32_t seen[4];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int i = 0; i < 2; i++) {
+                const int hi = x.hi[g + 8 * i], lo = first_seen(p, hi);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+                for (int h = 0; h < 2; h++) {
                     const int a = base + 8 * h + ((2 * t) ^ (t & 1)), b = base + 8 * h + ((2 * t + 1) ^ (t & 1));
-                    seen[2 * h + i] = h2_of(a >= lo[i] && a <= hi[i] ? 1.f : 0.f, b >= lo[i] && b <= hi[i] ? 1.f : 0.f);
+                    seen[2 * h + i] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
                 }
+            }
 #pragma unroll
             for (int i = 0; i < kVS; i++) {
                 uint32_t b[2];
@@ -680,7 +719,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Sequence
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
         if (t == 0) {
-            tops[warp * 16 + g + 8 * i] = top[i];
+            tops[warp * 16 + g + 8 * i] = limit[i] == -INFINITY ? -INFINITY : less[i];
             sums[warp * 16 + g + 8 * i] = sum[i];
         }
 #pragma unroll
@@ -714,13 +753,12 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, int head, int hea
 // Joins the four warps' results of a piece: into the output if the piece is
 // the tile's whole range, else into a part of the workspace.
 template <typename T, int D>
-__device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &q, int head, int row0, const uint8_t *smem,
-                                           float *part) {
+__device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, const uint8_t *smem, float *part) {
     const float *merge = reinterpret_cast<const float *>(smem);
     using L = AttnLayout<D>;
     const float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = min(16, q.news * p.group - row0);
+    const int rows = min(16, x.q.news * p.group - x.row0);
     for (int r = warp; r < rows; r += kAttnWarps) {
         float m = -INFINITY, l = 0.f, f[kAttnWarps], v[D / 32];
 #pragma unroll
@@ -745,8 +783,8 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Sequence &
                 part[16 * D + 16 + r] = l;
             }
         } else {
-            const int row = row0 + r;
-            write_row<T, D>(p, head, p.cache.heads, q.first + row / p.group, row % p.group, m, l, v);
+            const int row = x.row0 + r;
+            write_row<T, D>(p, x.head, p.cache.heads, x.q.first + row / p.group, row % p.group, m, l, v);
         }
     }
 }
@@ -756,12 +794,22 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
-    const int seq = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * 16;
-    const Sequence q = sequence(p, seq);
-    if (row0 >= q.news * p.group) return;
-    const int k0 = q.lo & ~(kUnit - 1);
-    attend_piece<T, D>(p, q, seq, head, row0, k0, k0 + q.units * kUnit, smem);
-    join_warps<T, D>(p, q, head, row0, smem, nullptr);
+    __shared__ Piece x;
+    const Sequence q = sequence(p, blockIdx.z);
+    if ((int)blockIdx.x * 16 >= q.news * p.group) return;
+    if (threadIdx.x < 32) {
+        if (threadIdx.x == 0) {
+            x.q = q;
+            x.seq = blockIdx.z, x.head = blockIdx.y, x.row0 = blockIdx.x * 16;
+            x.k0 = q.lo & ~(kUnit - 1);
+            x.k1 = x.k0 + q.units * kUnit;
+        }
+        __syncwarp();
+        set_rows(p, x);
+    }
+    __syncthreads();
+    attend_piece<T, D>(p, x, smem);
+    join_warps<T, D>(p, x, smem, nullptr);
 }
 
 // Split form: the units of all tiles in a row (sequence, head, tile, unit),
@@ -784,8 +832,10 @@ __host__ __device__ constexpr int64_t split_floats() {
 template <typename T, int D>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_split_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int64_t warp_sum[kAttnWarps], found_at;
-    __shared__ int found_seq;
+    __shared__ int64_t warp_sum[kAttnWarps], found_at, at;
+    __shared__ int found_seq, left, take;
+    __shared__ bool begins;
+    __shared__ Piece x;
     constexpr int kThreads = kAttnWarps * 32;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -806,7 +856,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
     total = 0;
     for (int w = 0; w < kAttnWarps; w++) total += warp_sum[w];
     const int64_t per = ceil_div<int64_t>(total, gridDim.x);
-    int64_t u = per * blockIdx.x;
+    const int64_t u = per * blockIdx.x;
     const int64_t u_end = u + per < total ? u + per : total;
     if (u >= u_end) return;
     // the sequence in which unit u lies, and that sequence's first unit
@@ -822,84 +872,120 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
         __syncthreads();
         if (lane == 31) warp_sum[warp] = inc;
         __syncthreads();
-        int64_t at = before + inc - n;
+        int64_t from = before + inc - n;
         for (int w = 0; w < kAttnWarps; w++) {
-            if (w < warp) at += warp_sum[w];
+            if (w < warp) from += warp_sum[w];
             before += warp_sum[w];
         }
-        if (u >= at && u < at + n) {
+        if (u >= from && u < from + n) {
             found_seq = b0 + tid;
-            found_at = at;
+            found_at = from;
         }
         __syncthreads();
         if (u < before) break;
     }
-    int seq = found_seq;
-    int64_t seq_at = found_at;
-    while (u < u_end) {
-        const Sequence q = sequence(p, seq);
-        const int64_t n = (int64_t)q.tiles * q.units * p.cache.heads;
-        while (u < u_end && u < seq_at + n) {
-            const int64_t rel = u - seq_at;
-            const int pair = (int)(rel / q.units), unit = (int)(rel % q.units);
-            const int head = pair / q.tiles, row0 = pair % q.tiles * 16;
-            const int take = (int)(u_end - u < q.units - unit ? u_end - u : q.units - unit);
-            const int k0 = (q.lo & ~(kUnit - 1)) + unit * kUnit;
-            attend_piece<T, D>(p, q, seq, head, row0, k0, k0 + take * kUnit, smem);
-            float *part = take == q.units ? nullptr
-                                          : mine + sizeof(SplitHead) / 4 + (unit > 0 ? 0 : AttnLayout<D>::kPart);
-            join_warps<T, D>(p, q, head, row0, smem, part);
-            if (take < q.units && unit == 0 && tid == 0)
-                *info = SplitHead{1 + (int)ceil_div<int64_t>(q.units - take, per), seq, head, row0,
-                                  min(16, q.news * p.group - row0), q.first, {0, 0}};
-            u += take;
-            __syncthreads();
+    if (tid == 0) {
+        x.seq = found_seq;
+        x.q = sequence(p, x.seq);
+        at = u - found_at;  // units from the sequence's first
+        left = (int)(u_end - u);
+    }
+    __syncthreads();
+    while (left > 0) {
+        if (tid < 32) {
+            if (tid == 0) {
+                while (at >= (int64_t)x.q.tiles * x.q.units * p.cache.heads) {
+                    at -= (int64_t)x.q.tiles * x.q.units * p.cache.heads;
+                    x.q = sequence(p, ++x.seq);
+                }
+                const int pair = (int)(at / x.q.units), unit = (int)(at % x.q.units);
+                take = min(left, x.q.units - unit);
+                begins = unit == 0;
+                x.head = pair / x.q.tiles;
+                x.row0 = pair % x.q.tiles * 16;
+                x.k0 = (x.q.lo & ~(kUnit - 1)) + unit * kUnit;
+                x.k1 = x.k0 + take * kUnit;
+                if (begins && take < x.q.units)
+                    *info = SplitHead{1 + (int)ceil_div<int64_t>(x.q.units - take, per), x.seq, x.head, x.row0,
+                                      min(16, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
+            }
+            __syncwarp();
+            set_rows(p, x);
         }
-        seq_at += n;
-        seq++;
+        __syncthreads();
+        attend_piece<T, D>(p, x, smem);
+        join_warps<T, D>(p, x, smem,
+                         begins && take == x.q.units ? nullptr
+                                                     : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D>::kPart : 0));
+        __syncthreads();
+        if (tid == 0) {
+            at += take;
+            left -= take;
+        }
+        __syncthreads();
     }
 }
 
-// One CTA a row of a tile in several parts: part 1 of CTA c, then part 0 of
-// the CTAs after it, every eighth for each warp.
-constexpr int kJoinWarps = 8;
+// Joins the parts of a tile: part 1 of CTA c, then part 0 of the CTAs after
+// it.  A CTA takes four rows, four warps each that take turns at the parts;
+// the parts' factors come first, so that the loads of O wait for nothing.
+constexpr int kJoinRows = 4, kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
-    __shared__ float tops[kJoinWarps], sums[kJoinWarps], o[kJoinWarps][D];
+__global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
+    constexpr int kMost = 512;  // parts whose factors are kept at a time
+    __shared__ float factor[kJoinRows][kMost], o_of[kJoinRows][kJoinWarps][D];
     pdl_enter();
     const float *at = p.parts + blockIdx.x * split_floats<D>();
     const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
-    const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (h.pieces == 0 || r >= h.rows) return;
+    const int slot = threadIdx.x >> 7, turn = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31;
+    const int r = blockIdx.y * kJoinRows + slot;
+    if (h.pieces == 0 || (int)blockIdx.y * kJoinRows >= h.rows) return;
     const auto part = [&](int i) {
         return at + i * split_floats<D>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D>::kPart);
     };
+    const bool real = r < h.rows;
     float m = -INFINITY, l = 0.f, v[D / 32] = {};
-    for (int i = threadIdx.x; i < h.pieces; i += kJoinWarps * 32) m = fmaxf(m, part(i)[16 * D + r]);
+    for (int i = lane; real && i < h.pieces; i += 32) m = fmaxf(m, part(i)[16 * D + r]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-    if (lane == 0) tops[warp] = m;
-    __syncthreads();
-    for (int w = 0; w < kJoinWarps; w++) m = fmaxf(m, tops[w]);
-#pragma unroll 4
-    for (int i = warp; i < h.pieces; i += kJoinWarps) {
-        const float *x = part(i);
-        const float s = x[16 * D + 16 + r], f = part_factor(x[16 * D + r], s, m);
-        l += f * s;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i0 = 0; i0 < h.pieces; i0 += kMost) {
+        const int n = min(kMost, h.pieces - i0);
+        __syncthreads();
+        for (int i = turn * 32 + lane; real && i < n; i += kJoinWarps * 32) {
+            const float s = part(i0 + i)[16 * D + 16 + r], f = part_factor(part(i0 + i)[16 * D + r], s, m);
+            factor[slot][i] = f;
+            l += f * s;
+        }
+        __syncthreads();
+        if (real) {
+#pragma unroll 8
+            for (int i = turn; i < n; i += kJoinWarps) {
+                const float *o = part(i0 + i) + r * D + lane;
+                const float f = factor[slot][i];
 #pragma unroll
-        for (int e = 0; e < D / 32; e++) v[e] += f == 0.f ? 0.f : f * x[r * D + lane + 32 * e];
+                for (int e = 0; e < D / 32; e++) {
+                    const float x = o[32 * e];
+                    v[e] += f == 0.f ? 0.f : f * x;
+                }
+            }
+        }
     }
-    if (lane == 0) sums[warp] = l;
 #pragma unroll
-    for (int e = 0; e < D / 32; e++) o[warp][lane + 32 * e] = v[e];
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) o_of[slot][turn][lane + 32 * e] = v[e];
     __syncthreads();
-    if (warp) return;
+    if (lane == 0) factor[slot][turn] = l;
+    __syncthreads();
+    if (turn || !real) return;
     l = 0.f;
-    for (int w = 0; w < kJoinWarps; w++) l += sums[w];
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) l += factor[slot][w];
 #pragma unroll
     for (int e = 0; e < D / 32; e++) {
         v[e] = 0.f;
-        for (int w = 0; w < kJoinWarps; w++) v[e] += o[w][lane + 32 * e];
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; w++) v[e] += o_of[slot][w][lane + 32 * e];
     }
     const int row = h.row0 + r;
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
@@ -936,8 +1022,8 @@ int launch_attend(const AttendArgs &p, int max_rows, int ctas, cudaStream_t st) 
     int rc = prepare_attend(attend_split_kernel<T, D>, smem);
     if (!rc)
         rc = launch_ex(attend_split_kernel<T, D>, dim3(ctas), dim3(kAttnWarps * 32), smem, 1, st, "attend_split_kernel", p);
-    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, max_rows < 16 ? max_rows : 16),
-                               dim3(kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
+    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, ceil_div(max_rows < 16 ? max_rows : 16, kJoinRows)),
+                               dim3(kJoinRows * kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
 }
 
 int flat_grid(int64_t total) {
