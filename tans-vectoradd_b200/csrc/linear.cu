@@ -8,6 +8,14 @@
 // bias in registers.  Both operands are K-major as they lie in memory: tiles
 // of 128 e4m3 columns (one 128-byte swizzle span) come by tensor-map copies,
 // which fill ragged edges with zeros, into a ring of shared-memory stages.
+//
+// Two forms.  linear_split_kernel: a CTA owns 128 rows x up to 128 tokens,
+// and a cluster of up to 8 CTAs shares their columns and adds its partial sums
+// over distributed shared memory: few tokens read the weight once, bound by
+// memory, with enough CTAs to keep it busy.  linear_pair_kernel: CTA pairs
+// (cta_group::2) own 256 rows x 256 tokens, stay resident over the tiles and
+// write one tile out of tensor memory while they multiply the next: many
+// tokens, bound by the tensor cores.
 
 #include "sm100.cuh"
 
@@ -19,16 +27,18 @@ namespace {
 constexpr int kMaxStages = 8;
 constexpr uint32_t kWaitLimit = 1u << 16;  // polls per wait
 constexpr uint32_t kPollNs = 10000;        // suspend-time hint per poll: bound ~0.66 s
-constexpr int kThreads = 192;              // copy warp, MMA warp, four epilogue warps
+constexpr uint32_t kTileA = 128 * 128;     // bytes of 128 rows x 128 columns
 
 struct LinearArgs {
-    CUtensorMap wmap, xmap;  // boxes of 128 columns x 128 rows / bn tokens, 128-byte swizzle
+    CUtensorMap wmap, xmap;  // boxes of 128 columns x 128 rows / tokens, 128-byte swizzle
     const float *x_scale, *w_scale;
     const void *bias, *mul, *residual;
     void *y;
     int64_t m, rows;
     int32_t chunks;  // of 128 columns
-    int32_t bn, stages, act;
+    int32_t bn;      // tokens of a tile
+    int32_t stages, act;
+    int32_t row_tiles, token_tiles, splits;
     int32_t *status;
 };
 
@@ -39,16 +49,26 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
 // Wait for the phase of `bar` with the given parity; false when the wait runs
-// out or (checked every 16 polls) *failed became non-zero.
+// out or (checked every 16 polls) *failed became non-zero.  kCluster: arrivals
+// of the cluster's other CTA are acquired too.
+template <bool kCluster = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile int32_t *failed) {
     for (uint32_t i = 0; i < kWaitLimit; i++) {
         uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
-            "selp.b32 %0, 1, 0, P1;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity), "n"(kPollNs)
-            : "memory");
+        if constexpr (kCluster)
+            asm volatile(
+                "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+                "selp.b32 %0, 1, 0, P1;\n\t}"
+                : "=r"(done)
+                : "r"(bar), "r"(parity), "n"(kPollNs)
+                : "memory");
+        else
+            asm volatile(
+                "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+                "selp.b32 %0, 1, 0, P1;\n\t}"
+                : "=r"(done)
+                : "r"(bar), "r"(parity), "n"(kPollNs)
+                : "memory");
         if (done) return true;
         if ((i & 15u) == 15u && failed && *failed) return false;
     }
@@ -76,8 +96,53 @@ __device__ __forceinline__ float activate(float v, int act) {
     return __fdividef(v, 1.f + __expf(-u));
 }
 
+// One output: the epilogue of an accumulator `a` of row r (scale ws, bias) and token t.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ LinearArgs p) {
+__device__ __forceinline__ void write_out(const LinearArgs &p, float a, float ws, float bias, float xs, int64_t t, int64_t r) {
+    a = activate(a * ws * xs + bias, p.act);
+    const int64_t at = t * p.rows + r;
+    if (p.mul) a *= to_f32(static_cast<const T *>(p.mul)[at]);
+    if (p.residual) a += to_f32(static_cast<const T *>(p.residual)[at]);
+    static_cast<T *>(p.y)[at] = from_f32<T>(a);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) {
+    uint32_t d;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(saddr), "r"(rank));
+    return d;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t tmem_columns(uint32_t n) {  // an allocation: a power of two, at least 32
+    return n <= 32 ? 32u : (n <= 64 ? 64u : (n <= 128 ? 128u : (n <= 256 ? 256u : 512u)));
+}
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
+    static_assert(N == 16, "16 columns");
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// ------------------------------------------------------------ split form
+//
+// Copy warp, MMA warp, four epilogue warps.  With p.splits > 1 the CTAs of a
+// cluster take equal stretches of the chunks; each puts
+// its f32 sums into its own shared memory ([token][row]) and, after a cluster
+// barrier, adds the stretches' sums of its share of the tokens in rank order.
+constexpr int kSplitThreads = 192;
+
+template <typename T>
+__global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __grid_constant__ LinearArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_s;
@@ -85,10 +150,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     volatile int32_t *failed = &failed_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t a_sa = (shared_addr(smem) + 1023u) & ~1023u;
-    const uint32_t a_bytes = 128u * 128u, b_bytes = (uint32_t)p.bn * 128u;
-    const uint32_t b_sa = a_sa + (uint32_t)p.stages * a_bytes;
+    const uint32_t b_bytes = (uint32_t)p.bn * 128u;
+    const uint32_t b_sa = a_sa + (uint32_t)p.stages * kTileA;
     const uint32_t full0 = shared_addr(full), empty0 = shared_addr(empty), done0 = shared_addr(&done);
-    const uint32_t ncols = p.bn <= 32 ? 32u : (p.bn <= 64 ? 64u : (p.bn <= 128 ? 128u : 256u));
+    const uint32_t ncols = tmem_columns(p.bn);
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(full0 + 8u * s, 1);
@@ -107,22 +172,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;");
     const uint32_t tmem = tmem_s;
-    const int32_t r0 = (int32_t)blockIdx.x * 128, t0 = (int32_t)blockIdx.y * p.bn;
+    const uint32_t rank = p.splits > 1 ? cluster_rank() : 0u;
+    const int32_t r0 = (int32_t)blockIdx.x / p.splits * 128, t0 = (int32_t)blockIdx.y * p.bn;
+    const int32_t c0 = (int32_t)((int64_t)p.chunks * rank / p.splits);
+    const int32_t n = (int32_t)((int64_t)p.chunks * (rank + 1) / p.splits) - c0;  // at least one
     pdl_enter();
 
     if (warp == 0 && lane == 0) {  // ------------------------------ copies
         int s = 0;
         uint32_t ph = 1;  // a fresh stage counts as empty
-        for (int32_t c = 0; c < p.chunks; c++) {
+        for (int32_t c = 0; c < n; c++) {
             if (!mbar_wait(empty0 + 8u * s, ph, failed)) {
                 *failed = 1;
                 break;
             }
             const uint32_t bar = full0 + 8u * s;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(a_bytes + b_bytes)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kTileA + b_bytes)
                          : "memory");
-            copy_box(&p.wmap, a_sa + (uint32_t)s * a_bytes, bar, c * 128, r0);
-            copy_box(&p.xmap, b_sa + (uint32_t)s * b_bytes, bar, c * 128, t0);
+            copy_box(&p.wmap, a_sa + (uint32_t)s * kTileA, bar, (c0 + c) * 128, r0);
+            copy_box(&p.xmap, b_sa + (uint32_t)s * b_bytes, bar, (c0 + c) * 128, t0);
             copied_s = c + 1;
             if (++s == p.stages) s = 0, ph ^= 1u;
         }
@@ -132,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int32_t c = 0; c < p.chunks; c++) {
+        for (int32_t c = 0; c < n; c++) {
             if (!mbar_wait(full0 + 8u * s, ph, failed)) {
                 ok = false;
                 break;
@@ -143,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
                 asm volatile(
                     "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(tmem),
-                    "l"(smem_desc(a_sa + (uint32_t)s * a_bytes + 32u * j)),
+                    "l"(smem_desc(a_sa + (uint32_t)s * kTileA + 32u * j)),
                     "l"(smem_desc(b_sa + (uint32_t)s * b_bytes + 32u * j)), "r"(idesc), "r"((uint32_t)(c > 0 || j > 0)),
                     "r"(0u));
             asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -158,41 +226,256 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     }
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;");
-    if (*failed) {
-        if (threadIdx.x == 0) {  // copies in flight land before the CTA may end
-            if (p.status) atomicOr(p.status, TANS_B200_DATA_TIMEOUT);
-            for (int32_t c = copied_s > p.stages ? copied_s - p.stages : 0; c < copied_s; c++)
-                mbar_wait(full0 + 8u * (c % p.stages), (uint32_t)((c / p.stages) & 1), nullptr);
-        }
-    } else if (warp >= 2) {  // ------------------------------------- epilogue
-        const int quarter = warp & 3;
-        const int64_t r = r0 + 32 * quarter + lane;
+    if (*failed && threadIdx.x == 0) {  // copies in flight land before the CTA may end
+        if (p.status) atomicOr(p.status, TANS_B200_DATA_TIMEOUT);
+        for (int32_t c = copied_s > p.stages ? copied_s - p.stages : 0; c < copied_s; c++)
+            mbar_wait(full0 + 8u * (c % p.stages), (uint32_t)((c / p.stages) & 1), nullptr);
+    }
+    const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
+    if (warp >= 2 && !*failed) {  // this CTA's sums out of tensor memory
+        const int row = 32 * (warp & 3) + lane;
+        const int64_t r = r0 + row;
         const bool real = r < p.rows;
         const float ws = real ? p.w_scale[r] : 0.f;
         const float bias = real && p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f;
-        for (int col = 0; col < p.bn && t0 + col < p.m; col += 8) {
-            uint32_t v[8];
-            asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                         : "r"(tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)col));
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        float *sums = reinterpret_cast<float *>(smem + (a_sa - shared_addr(smem)));
+        for (int col = 0; col < tokens; col += 16) {
+            uint32_t v[16];
+            tmem_load(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)col, v);
+            if (p.splits > 1) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int64_t t = t0 + col + k;
-                if (real && t < p.m) {
-                    float a = activate(__uint_as_float(v[k]) * ws * p.x_scale[t] + bias, p.act);
-                    if (p.mul) a *= to_f32(static_cast<const T *>(p.mul)[t * p.rows + r]);
-                    if (p.residual) a += to_f32(static_cast<const T *>(p.residual)[t * p.rows + r]);
-                    static_cast<T *>(p.y)[t * p.rows + r] = from_f32<T>(a);
-                }
+                for (int k = 0; k < 16; k++) sums[(col + k) * 128 + row] = __uint_as_float(v[k]);
+            } else if (real) {
+#pragma unroll
+                for (int k = 0; k < 16; k++)
+                    if (col + k < tokens)
+                        write_out<T>(p, __uint_as_float(v[k]), ws, bias, p.x_scale[t0 + col + k], t0 + col + k, r);
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
-    __syncthreads();
+    __syncwarp();
+    if (p.splits > 1) {
+        cluster_sync();
+        if (!*failed) {
+            const int32_t lo = tokens * (int32_t)rank / p.splits, hi = tokens * (int32_t)(rank + 1) / p.splits;
+            for (int32_t i = threadIdx.x; i < (hi - lo) * 128; i += kSplitThreads) {
+                const int32_t col = lo + (i >> 7), row = i & 127;
+                const int64_t r = r0 + row;
+                if (r >= p.rows) continue;
+                float a = 0.f;
+                for (int s = 0; s < p.splits; s++) {
+                    float v;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                 : "=f"(v)
+                                 : "r"(cluster_addr(a_sa, s) + (uint32_t)(col * 128 + row) * 4u));
+                    a += v;
+                }
+                write_out<T>(p, a, p.w_scale[r], p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f,
+                             p.x_scale[t0 + col], t0 + col, r);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while another reads its sums
+    } else {
+        __syncthreads();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ncols));
+    }
+}
+
+// ------------------------------------------------------------- pair form
+//
+// A cluster of two CTAs per tile of 256 rows x bn tokens: each copies its 128
+// rows of w and its half of the tokens, all bytes counted on the first CTA's
+// `full` barrier, whose MMA thread multiplies for both (M = 256) and frees the
+// stage in both.  The accumulator has two places in tensor memory; eight warps
+// in each CTA write its 128 rows of one tile while the next is multiplied.
+// Tiles are taken in bands of eight token tiles, the row tiles in turn within
+// a band, so that the tiles in work at a time share their operands in L2.
+constexpr int kPairThreads = 320;
+constexpr int kBand = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __grid_constant__ LinearArgs p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_s;
+    __shared__ int32_t failed_s;
+    volatile int32_t *failed = &failed_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t a_sa = (shared_addr(smem) + 1023u) & ~1023u;
+    const uint32_t b_bytes = (uint32_t)p.bn * 64u;  // this CTA's half of the tokens
+    const uint32_t b_sa = a_sa + (uint32_t)p.stages * kTileA;
+    const uint32_t full0 = shared_addr(full), empty0 = shared_addr(empty);
+    const uint32_t accf0 = shared_addr(acc_full), acce0 = shared_addr(acc_empty);
+    const uint32_t ncols = tmem_columns(2 * p.bn);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(full0 + 8u * s, 1);
+            mbar_init(empty0 + 8u * s, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(accf0 + 8u * i, 1);
+            mbar_init(acce0 + 8u * i, 16);  // eight warps in each CTA
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;");
+        failed_s = 0;
+    }
+    cluster_sync();
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_addr(&tmem_s)),
+                     "r"(ncols));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const uint32_t tmem = tmem_s;
+    const int32_t tiles = p.row_tiles * p.token_tiles, pairs = (int32_t)gridDim.x / 2;
+    const auto tile_at = [&](int32_t tile, int32_t &r0, int32_t &t0) {
+        const int32_t band = tile / (p.row_tiles * kBand), in = tile - band * p.row_tiles * kBand;
+        const int32_t width = min(kBand, p.token_tiles - band * kBand);
+        r0 = in / width * 256;
+        t0 = (band * kBand + in % width) * p.bn;
+    };
+    const auto give_up = [&] {  // seen by both CTAs
+        *failed = 1;
+        asm volatile("st.relaxed.cluster.shared::cluster.b32 [%0], 1;" ::"r"(cluster_addr(shared_addr(&failed_s), rank ^ 1u))
+                     : "memory");
+    };
+    pdl_enter();
+
+    if (warp == 0 && lane == 0) {  // ------------------------------ copies
+        int s = 0;
+        uint32_t ph = 1;
+        int64_t copied = 0;
+        const uint32_t lead = cluster_addr(full0, 0);
+        for (int32_t tile = blockIdx.x / 2; tile < tiles && !*failed; tile += pairs) {
+            int32_t r0, t0;
+            tile_at(tile, r0, t0);
+            r0 += 128 * (int32_t)rank;
+            t0 += p.bn / 2 * (int32_t)rank;
+            for (int32_t c = 0; c < p.chunks; c++) {
+                if (!mbar_wait(empty0 + 8u * s, ph, failed)) {
+                    give_up();
+                    break;
+                }
+                if (rank == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full0 + 8u * s),
+                                 "r"(2u * (kTileA + b_bytes))
+                                 : "memory");
+                const auto box = [&](const CUtensorMap *map, uint32_t dst, int32_t row) {
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                        "l"(reinterpret_cast<uint64_t>(map)), "r"(c * 128), "r"(row), "r"(lead + 8u * s)
+                        : "memory");
+                };
+                box(&p.wmap, a_sa + (uint32_t)s * kTileA, r0);
+                box(&p.xmap, b_sa + (uint32_t)s * b_bytes, t0);
+                copied++;
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+        }
+        if (*failed && rank == 0)  // copies in flight land before the pair may end
+            for (int64_t c = copied > p.stages ? copied - p.stages : 0; c < copied; c++)
+                mbar_wait(full0 + 8u * (uint32_t)(c % p.stages), (uint32_t)(c / p.stages & 1), nullptr);
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // ---------- MMA, for both CTAs
+        const uint32_t idesc = (1u << 4) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+        const auto commit = [&](uint32_t bar) {
+            asm volatile(
+                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                "h"((uint16_t)3)
+                : "memory");
+        };
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        int32_t it = 0;
+        for (int32_t tile = blockIdx.x / 2; tile < tiles && ok; tile += pairs, it++) {
+            const uint32_t d = tmem + (uint32_t)((it & 1) * p.bn);
+            if (!mbar_wait<true>(acce0 + 8u * (it & 1), ((it >> 1) & 1) ^ 1u, failed)) {
+                ok = false;
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            for (int32_t c = 0; c < p.chunks; c++) {
+                if (!mbar_wait<true>(full0 + 8u * s, ph, failed)) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    asm volatile(
+                        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+                        "l"(smem_desc(a_sa + (uint32_t)s * kTileA + 32u * j)),
+                        "l"(smem_desc(b_sa + (uint32_t)s * b_bytes + 32u * j)), "r"(idesc),
+                        "r"((uint32_t)(c > 0 || j > 0)), "r"(0u));
+                commit(empty0 + 8u * s);
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+            if (ok) commit(accf0 + 8u * (it & 1));
+        }
+        if (!ok) give_up();
+        if (it > 0 && !mbar_wait(accf0 + 8u * ((it - 1) & 1), ((it - 1) >> 1) & 1, nullptr)) give_up();
+    } else if (warp >= 2) {  // ------------------------------------ epilogue
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        int32_t it = 0;
+        for (int32_t tile = blockIdx.x / 2; tile < tiles; tile += pairs, it++) {
+            int32_t r0, t0;
+            tile_at(tile, r0, t0);
+            const int64_t r = r0 + 128 * (int32_t)rank + 32 * quarter + lane;
+            const bool real = r < p.rows;
+            const float ws = real ? p.w_scale[r] : 0.f;
+            const float bias = real && p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f;
+            uint32_t ok = lane ? 1u : (uint32_t)mbar_wait(accf0 + 8u * (it & 1), (it >> 1) & 1, failed);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) give_up();
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
+            const int32_t end = min(tokens, (half + 1) * p.bn / 2);
+            for (int32_t col = half * p.bn / 2; col < end; col += 16) {
+                uint32_t v[16];
+                tmem_load(tmem + (uint32_t)((it & 1) * p.bn) + ((uint32_t)(32 * quarter) << 16) + (uint32_t)col, v);
+                const float xs = col + (lane & 15) < end ? p.x_scale[t0 + col + (lane & 15)] : 0.f;
+                float mu[16], re[16];
+                const int64_t at = (int64_t)(t0 + col) * p.rows + r;
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const bool in = real && col + k < end;
+                    mu[k] = p.mul && in ? to_f32(static_cast<const T *>(p.mul)[at + k * p.rows]) : 1.f;
+                    re[k] = p.residual && in ? to_f32(static_cast<const T *>(p.residual)[at + k * p.rows]) : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    const float x = __shfl_sync(0xffffffffu, xs, k);
+                    const float a = activate(__uint_as_float(v[k]) * ws * x + bias, p.act) * mu[k] + re[k];
+                    if (real && col + k < end) static_cast<T *>(p.y)[at + k * p.rows] = from_f32<T>(a);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;");
+            __syncwarp();
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 cluster_addr(acce0 + 8u * (it & 1), 0))
+                             : "memory");
+        }
+    }
+    __syncwarp();
+    if (*failed && threadIdx.x == 0 && p.status) atomicOr(p.status, TANS_B200_DATA_TIMEOUT);
+    asm volatile("tcgen05.fence::before_thread_sync;");
+    cluster_sync();  // neither CTA leaves while the other may reach its memory
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ncols));
     }
 }
 
@@ -230,12 +513,18 @@ int e4m3_map(CUtensorMap *map, const uint8_t *p, int64_t rows, int64_t cols, int
 }
 
 template <typename T>
-int launch_linear(const LinearArgs &p, cudaStream_t st) {
-    const int smem = 1024 + p.stages * (128 + p.bn) * 128;
-    const cudaError_t e = cudaFuncSetAttribute(linear_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+int launch_linear(const LinearArgs &p, bool pair, int sms, cudaStream_t st) {
+    const int smem = 1024 + p.stages * (int)(kTileA + p.bn * (pair ? 64 : 128));
+    const auto kernel = pair ? linear_pair_kernel<T> : linear_split_kernel<T>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return launch_failed("linear_kernel", e);
-    return launch_ex(linear_kernel<T>, dim3((unsigned)ceil_div<int64_t>(p.rows, 128), (unsigned)ceil_div<int64_t>(p.m, p.bn)),
-                     dim3(kThreads), smem, 1, st, "linear_kernel", p);
+    if (pair) {
+        const int tiles = p.row_tiles * p.token_tiles, pairs = sms / 2;
+        return launch_ex(kernel, dim3(2u * (tiles < pairs ? tiles : pairs)), dim3(kPairThreads), smem, 2, st,
+                         "linear_pair_kernel", p);
+    }
+    return launch_ex(kernel, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)p.token_tiles), dim3(kSplitThreads), smem,
+                     p.splits, st, "linear_split_kernel", p);
 }
 
 }  // namespace
@@ -265,10 +554,36 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
     p.chunks = (int32_t)ceil_div<int64_t>(cols, 128);
     p.act = act;
     p.status = status;
-    p.bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : (m <= 128 ? 128 : 256)));
-    p.stages = p.bn <= 128 ? 6 : 4;
+    int dev, sms;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return launch_failed("linear", e);
+    const int64_t pair_tiles = ceil_div<int64_t>(rows, 256) * ceil_div<int64_t>(m, 256);
+    const bool pair = m > 128 && pair_tiles >= sms / 3;
+    int64_t row_tiles, token_tiles;
+    if (pair) {
+        p.bn = 256;
+        p.splits = 1;
+        p.stages = 6;
+        row_tiles = ceil_div<int64_t>(rows, 256);
+        token_tiles = ceil_div<int64_t>(m, 256);
+    } else {
+        p.bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+        row_tiles = ceil_div<int64_t>(rows, 128);
+        token_tiles = ceil_div<int64_t>(m, p.bn);
+        // two CTAs an SM, each with at least four chunks of columns
+        int64_t splits = 2 * sms / (row_tiles * token_tiles);
+        if (splits > p.chunks / 4) splits = p.chunks / 4;
+        p.splits = (int32_t)(splits < 1 ? 1 : (splits > 8 ? 8 : splits));
+        p.stages = (int32_t)((110 * 1024 - 1024) / (kTileA + p.bn * 128));
+        if (p.stages > kMaxStages) p.stages = kMaxStages;
+    }
+    if (row_tiles * p.splits > INT32_MAX / 4 || token_tiles > 65535 || row_tiles * token_tiles > INT32_MAX / 4)
+        return fail(TANS_B200_ERR_INVALID, "linear: m and rows are too large");
+    p.row_tiles = (int32_t)row_tiles;
+    p.token_tiles = (int32_t)token_tiles;
     int rc = e4m3_map(&p.wmap, w, rows, cols, 128);
-    if (!rc) rc = e4m3_map(&p.xmap, x, m, cols, p.bn);
+    if (!rc) rc = e4m3_map(&p.xmap, x, m, cols, pair ? p.bn / 2 : p.bn);
     if (rc) return rc;
-    return dispatch_half(dtype, "linear", [&](auto t) { return launch_linear<decltype(t)>(p, (cudaStream_t)stream); });
+    return dispatch_half(dtype, "linear", [&](auto t) { return launch_linear<decltype(t)>(p, pair, sms, (cudaStream_t)stream); });
 }
