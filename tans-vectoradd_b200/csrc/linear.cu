@@ -87,19 +87,35 @@ __device__ __forceinline__ void copy_box(const CUtensorMap *map, uint32_t dst, u
         : "memory");
 }
 
-// act(v); SiLU is v / (1 + e^-v), and the tanh form of GELU is
+// act of N values; SiLU is v / (1 + e^-v), and the tanh form of GELU is
 // v / (1 + e^(-2 sqrt(2/pi) (v + 0.044715 v^3))) as 1 + tanh(u) = 2 / (1 + e^-2u).
-__device__ __forceinline__ float activate(float v, int act) {
-    if (act == TANS_B200_ACT_NONE) return v;
-    if (act == TANS_B200_ACT_RELU) return v < 0.f ? 0.f : v;
-    const float u = act == TANS_B200_ACT_SILU ? v : 1.5957691216057308f * (v + 0.044715f * v * v * v);
-    return __fdividef(v, 1.f + __expf(-u));
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
+    if (act == TANS_B200_ACT_NONE) return;
+    if (act == TANS_B200_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+        return;
+    }
+    // the exponent in base 2
+    const bool silu = act == TANS_B200_ACT_SILU;
+    constexpr float kSilu = -1.4426950408889634f, kGelu1 = -2.302208198144325f, kGelu3 = -0.1029432395800235f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float e, r;
+        const float u = v[i] * (silu ? kSilu : __fmaf_rn(kGelu3, v[i] * v[i], kGelu1));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(u));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+        v[i] *= r;
+    }
 }
 
 // One output: the epilogue of an accumulator `a` of row r (scale ws, bias) and token t.
 template <typename T>
 __device__ __forceinline__ void write_out(const LinearArgs &p, float a, float ws, float bias, float xs, int64_t t, int64_t r) {
-    a = activate(a * ws * xs + bias, p.act);
+    float v[1] = {a * ws * xs + bias};
+    activate(v, p.act);
+    a = v[0];
     const int64_t at = t * p.rows + r;
     if (p.mul) a *= to_f32(static_cast<const T *>(p.mul)[at]);
     if (p.residual) a += to_f32(static_cast<const T *>(p.residual)[at]);
@@ -295,6 +311,57 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
 // in each CTA write its 128 rows of one tile while the next is multiplied.
 // Tiles are taken in bands of eight token tiles, the row tiles in turn within
 // a band, so that the tiles in work at a time share their operands in L2.
+
+// A warp's 32 rows (one a lane) of n tokens from the accumulator columns at
+// `acc` on; mul, res and y point to the first token.  The operands of the next
+// 16 tokens are loaded while the present ones are worked out.  kFull: n is a
+// multiple of 16 and every lane's row is real.
+template <typename T, bool kFull>
+__device__ __forceinline__ void write_columns(const LinearArgs &p, uint32_t acc, int32_t n, float ws, float bias,
+                                              const float *x_scale, const T *mul, const T *res, T *y, bool real) {
+    const int lane = threadIdx.x & 31;
+    T mu[16], re[16];
+    float xs;
+    const auto load = [&](int32_t col) {
+        xs = col + (lane & 15) < n ? x_scale[col + (lane & 15)] : 0.f;
+        if (mul) {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (kFull || (real && col + k < n)) mu[k] = mul[(int64_t)(col + k) * p.rows];
+        }
+        if (res) {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (kFull || (real && col + k < n)) re[k] = res[(int64_t)(col + k) * p.rows];
+        }
+    };
+    load(0);
+    for (int32_t col = 0; col < n; col += 16) {
+        uint32_t raw[16];
+        tmem_load(acc + (uint32_t)col, raw);
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+            v[k] = __fmaf_rn(__uint_as_float(raw[k]) * ws, __shfl_sync(0xffffffffu, xs, k), bias);
+        T mu_now[16], re_now[16];
+#pragma unroll
+        for (int k = 0; k < 16; k++) mu_now[k] = mu[k], re_now[k] = re[k];
+        if (col + 16 < n) load(col + 16);
+        activate(v, p.act);
+        if (mul) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] *= to_f32(mu_now[k]);
+        }
+        if (res) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] += to_f32(re_now[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; k++)
+            if (kFull || (real && col + k < n)) y[(int64_t)(col + k) * p.rows] = from_f32<T>(v[k]);
+    }
+}
+
 constexpr int kPairThreads = 320;
 constexpr int kBand = 8;
 
@@ -442,24 +509,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             asm volatile("tcgen05.fence::after_thread_sync;");
             const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
             const int32_t end = min(tokens, (half + 1) * p.bn / 2);
-            for (int32_t col = half * p.bn / 2; col < end; col += 16) {
-                uint32_t v[16];
-                tmem_load(tmem + (uint32_t)((it & 1) * p.bn) + ((uint32_t)(32 * quarter) << 16) + (uint32_t)col, v);
-                const float xs = col + (lane & 15) < end ? p.x_scale[t0 + col + (lane & 15)] : 0.f;
-                float mu[16], re[16];
-                const int64_t at = (int64_t)(t0 + col) * p.rows + r;
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const bool in = real && col + k < end;
-                    mu[k] = p.mul && in ? to_f32(static_cast<const T *>(p.mul)[at + k * p.rows]) : 1.f;
-                    re[k] = p.residual && in ? to_f32(static_cast<const T *>(p.residual)[at + k * p.rows]) : 0.f;
-                }
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const float x = __shfl_sync(0xffffffffu, xs, k);
-                    const float a = activate(__uint_as_float(v[k]) * ws * x + bias, p.act) * mu[k] + re[k];
-                    if (real && col + k < end) static_cast<T *>(p.y)[at + k * p.rows] = from_f32<T>(a);
-                }
+            const int32_t begin = half * p.bn / 2;
+            const uint32_t acc = tmem + (uint32_t)((it & 1) * p.bn) + ((uint32_t)(32 * quarter) << 16);
+            if (begin < end) {
+                const int64_t at = (int64_t)(t0 + begin) * p.rows + r;
+                const T *mul = p.mul ? static_cast<const T *>(p.mul) + at : nullptr;
+                const T *res = p.residual ? static_cast<const T *>(p.residual) + at : nullptr;
+                T *y = static_cast<T *>(p.y) + at;
+                if (r - lane + 32 <= p.rows && (end - begin) % 16 == 0)
+                    write_columns<T, true>(p, acc + begin, end - begin, ws, bias, p.x_scale + t0 + begin, mul, res, y, true);
+                else
+                    write_columns<T, false>(p, acc + begin, end - begin, ws, bias, p.x_scale + t0 + begin, mul, res, y, real);
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
             __syncwarp();
