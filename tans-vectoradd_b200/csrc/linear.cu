@@ -39,6 +39,7 @@ struct LinearArgs {
     int32_t bn;      // tokens of a tile
     int32_t stages, act;
     int32_t row_tiles, token_tiles, splits;
+    bool vec;        // rows a multiple of 8 and mul, residual and y 16-byte aligned
     int32_t *status;
 };
 
@@ -110,18 +111,6 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
     }
 }
 
-// One output: the epilogue of an accumulator `a` of row r (scale ws, bias) and token t.
-template <typename T>
-__device__ __forceinline__ void write_out(const LinearArgs &p, float a, float ws, float bias, float xs, int64_t t, int64_t r) {
-    float v[1] = {a * ws * xs + bias};
-    activate(v, p.act);
-    a = v[0];
-    const int64_t at = t * p.rows + r;
-    if (p.mul) a *= to_f32(static_cast<const T *>(p.mul)[at]);
-    if (p.residual) a += to_f32(static_cast<const T *>(p.residual)[at]);
-    static_cast<T *>(p.y)[at] = from_f32<T>(a);
-}
-
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -149,16 +138,54 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The last step of eight rows r .. r + 7 (`real` of them exist) of token t:
+// v = act(..) becomes v * mul + residual, rounded once.
+template <typename T>
+struct Operands {
+    uint4 mul, residual;  // eight values each, loaded ahead where p.vec allows
+};
+template <typename T>
+__device__ __forceinline__ void load_operands(const LinearArgs &p, int64_t at, Operands<T> &o) {
+    if (p.vec && p.mul) o.mul = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.mul) + at);
+    if (p.vec && p.residual) o.residual = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
+}
+template <typename T>
+__device__ __forceinline__ void write_eight(const LinearArgs &p, float (&v)[8], int64_t at, int32_t real, const Operands<T> &o) {
+    if (p.vec) {  // rows are a multiple of 8: all eight exist
+        const T *mu = reinterpret_cast<const T *>(&o.mul), *re = reinterpret_cast<const T *>(&o.residual);
+        if (p.mul) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] *= to_f32(mu[k]);
+        }
+        if (p.residual) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] += to_f32(re[k]);
+        }
+        store8(static_cast<T *>(p.y) + at, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < real) {
+                if (p.mul) v[k] *= to_f32(static_cast<const T *>(p.mul)[at + k]);
+                if (p.residual) v[k] += to_f32(static_cast<const T *>(p.residual)[at + k]);
+                static_cast<T *>(p.y)[at + k] = from_f32<T>(v[k]);
+            }
+    }
+}
+
 // ------------------------------------------------------------ split form
 //
-// Copy warp, MMA warp, four epilogue warps.  With p.splits > 1 the CTAs of a
-// cluster take equal stretches of the chunks; each puts
-// its f32 sums into its own shared memory ([token][row]) and, after a cluster
-// barrier, adds the stretches' sums of its share of the tokens in rank order.
+// Copy warp, MMA warp, and four warps that read tensor memory.  The CTAs of a
+// cluster take equal stretches of the chunks; each puts its f32 sums into its
+// own shared memory ([token][row]) and, after a cluster barrier, adds the
+// stretches' sums of its share of the tokens in rank order.  There a thread
+// has the same eight rows of every token it writes; four-row groups of every
+// other 32 rows change places in shared memory, so that its two reads of four
+// meet no bank twice.
 constexpr int kSplitThreads = 192;
 
 template <typename T>
-__global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __grid_constant__ LinearArgs p) {
+__global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __grid_constant__ LinearArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], done;
     __shared__ uint32_t tmem_s;
@@ -193,6 +220,29 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
     const int32_t c0 = (int32_t)((int64_t)p.chunks * rank / p.splits);
     const int32_t n = (int32_t)((int64_t)p.chunks * (rank + 1) / p.splits) - c0;  // at least one
     pdl_enter();
+    // what a thread of the last four warps will write: rows r .. r + 7 of every
+    // eighth token of its CTA's share
+    constexpr int32_t kTokensAtATime = 8;
+    const bool writer = warp >= 2;
+    const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
+    const int32_t row8 = (threadIdx.x & 15) * 8;
+    const int64_t r = r0 + row8;
+    const int32_t real = p.rows - r < 8 ? (int32_t)(p.rows - r) : 8;
+    const int32_t first = tokens * (int32_t)rank / p.splits + ((int32_t)(threadIdx.x - 64) >> 4);
+    const int32_t last = tokens * (int32_t)(rank + 1) / p.splits;
+    float ws[8], bias[8], xs_next = 0.f;
+    Operands<T> ops{};
+    if (writer) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            ws[k] = k < real ? p.w_scale[r + k] : 0.f;
+            bias[k] = p.bias && k < real ? to_f32(static_cast<const T *>(p.bias)[r + k]) : 0.f;
+        }
+        if (first < last && real > 0) {
+            load_operands<T>(p, (int64_t)(t0 + first) * p.rows + r, ops);
+            xs_next = p.x_scale[t0 + first];
+        }
+    }
 
     if (warp == 0 && lane == 0) {  // ------------------------------ copies
         int s = 0;
@@ -247,54 +297,65 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
         for (int32_t c = copied_s > p.stages ? copied_s - p.stages : 0; c < copied_s; c++)
             mbar_wait(full0 + 8u * (c % p.stages), (uint32_t)((c / p.stages) & 1), nullptr);
     }
-    const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
-    if (warp >= 2 && !*failed) {  // this CTA's sums out of tensor memory
+    float *sums = reinterpret_cast<float *>(smem + (a_sa - shared_addr(smem)));
+    if (writer && !*failed) {  // this CTA's sums out of tensor memory
         const int row = 32 * (warp & 3) + lane;
-        const int64_t r = r0 + row;
-        const bool real = r < p.rows;
-        const float ws = real ? p.w_scale[r] : 0.f;
-        const float bias = real && p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f;
-        float *sums = reinterpret_cast<float *>(smem + (a_sa - shared_addr(smem)));
         for (int col = 0; col < tokens; col += 16) {
             uint32_t v[16];
             tmem_load(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)col, v);
-            if (p.splits > 1) {
 #pragma unroll
-                for (int k = 0; k < 16; k++) sums[(col + k) * 128 + row] = __uint_as_float(v[k]);
-            } else if (real) {
-#pragma unroll
-                for (int k = 0; k < 16; k++)
-                    if (col + k < tokens)
-                        write_out<T>(p, __uint_as_float(v[k]), ws, bias, p.x_scale[t0 + col + k], t0 + col + k, r);
-            }
+            for (int k = 0; k < 16; k++) sums[(col + k) * 128 + (row ^ (row >> 3 & 4))] = __uint_as_float(v[k]);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncwarp();
-    if (p.splits > 1) {
+    if (p.splits > 1)
         cluster_sync();
-        if (!*failed) {
-            const int32_t lo = tokens * (int32_t)rank / p.splits, hi = tokens * (int32_t)(rank + 1) / p.splits;
-            for (int32_t i = threadIdx.x; i < (hi - lo) * 128; i += kSplitThreads) {
-                const int32_t col = lo + (i >> 7), row = i & 127;
-                const int64_t r = r0 + row;
-                if (r >= p.rows) continue;
-                float a = 0.f;
-                for (int s = 0; s < p.splits; s++) {
-                    float v;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                 : "=f"(v)
-                                 : "r"(cluster_addr(a_sa, s) + (uint32_t)(col * 128 + row) * 4u));
-                    a += v;
-                }
-                write_out<T>(p, a, p.w_scale[r], p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f,
-                             p.x_scale[t0 + col], t0 + col, r);
+    else
+        __syncthreads();
+    if (writer && !*failed && real > 0) {
+        for (int32_t col = first; col < last; col += kTokensAtATime) {
+            const Operands<T> now = ops;
+            const float xs = xs_next;
+            const int64_t at = (int64_t)(t0 + col) * p.rows + r;
+            if (col + kTokensAtATime < last) {
+                load_operands<T>(p, at + kTokensAtATime * p.rows, ops);
+                xs_next = p.x_scale[t0 + col + kTokensAtATime];
             }
+            float v[8] = {};
+#pragma unroll
+            for (int s0 = 0; s0 < 8; s0 += 4) {  // four CTAs' loads at once
+                if (s0 >= p.splits) break;
+                float4 part[4][2];
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    if (s0 + s < p.splits) {
+                        const uint32_t from = cluster_addr(a_sa, s0 + s) + (uint32_t)(col * 128 + row8) * 4u;
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(part[s][h].x), "=f"(part[s][h].y), "=f"(part[s][h].z), "=f"(part[s][h].w)
+                                         : "r"(from + 16u * (h ^ (row8 >> 5 & 1)))
+                                         : "memory");
+                    }
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    if (s0 + s < p.splits) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+                            v[4 * h] += part[s][h].x, v[4 * h + 1] += part[s][h].y, v[4 * h + 2] += part[s][h].z,
+                                v[4 * h + 3] += part[s][h].w;
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __fmaf_rn(v[k] * ws[k], xs, bias[k]);
+            activate(v, p.act);
+            write_eight<T>(p, v, at, real, now);
         }
+    }
+    if (p.splits > 1) {
         __syncwarp();
         cluster_sync();  // no CTA leaves while another reads its sums
-    } else {
-        __syncthreads();
     }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;");
@@ -311,59 +372,9 @@ __global__ void __launch_bounds__(kSplitThreads) linear_split_kernel(const __gri
 // in each CTA write its 128 rows of one tile while the next is multiplied.
 // Tiles are taken in bands of eight token tiles, the row tiles in turn within
 // a band, so that the tiles in work at a time share their operands in L2.
-
-// A warp's 32 rows (one a lane) of n tokens from the accumulator columns at
-// `acc` on; mul, res and y point to the first token.  The operands of the next
-// 16 tokens are loaded while the present ones are worked out.  kFull: n is a
-// multiple of 16 and every lane's row is real.
-template <typename T, bool kFull>
-__device__ __forceinline__ void write_columns(const LinearArgs &p, uint32_t acc, int32_t n, float ws, float bias,
-                                              const float *x_scale, const T *mul, const T *res, T *y, bool real) {
-    const int lane = threadIdx.x & 31;
-    T mu[16], re[16];
-    float xs;
-    const auto load = [&](int32_t col) {
-        xs = col + (lane & 15) < n ? x_scale[col + (lane & 15)] : 0.f;
-        if (mul) {
-#pragma unroll
-            for (int k = 0; k < 16; k++)
-                if (kFull || (real && col + k < n)) mu[k] = mul[(int64_t)(col + k) * p.rows];
-        }
-        if (res) {
-#pragma unroll
-            for (int k = 0; k < 16; k++)
-                if (kFull || (real && col + k < n)) re[k] = res[(int64_t)(col + k) * p.rows];
-        }
-    };
-    load(0);
-    for (int32_t col = 0; col < n; col += 16) {
-        uint32_t raw[16];
-        tmem_load(acc + (uint32_t)col, raw);
-        float v[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-            v[k] = __fmaf_rn(__uint_as_float(raw[k]) * ws, __shfl_sync(0xffffffffu, xs, k), bias);
-        T mu_now[16], re_now[16];
-#pragma unroll
-        for (int k = 0; k < 16; k++) mu_now[k] = mu[k], re_now[k] = re[k];
-        if (col + 16 < n) load(col + 16);
-        activate(v, p.act);
-        if (mul) {
-#pragma unroll
-            for (int k = 0; k < 16; k++) v[k] *= to_f32(mu_now[k]);
-        }
-        if (res) {
-#pragma unroll
-            for (int k = 0; k < 16; k++) v[k] += to_f32(re_now[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-            if (kFull || (real && col + k < n)) y[(int64_t)(col + k) * p.rows] = from_f32<T>(v[k]);
-    }
-}
-
 constexpr int kPairThreads = 320;
 constexpr int kBand = 8;
+constexpr int kWarpFloats = 16 * 32 + 128;  // an epilogue warp's shared memory: 16 tokens x 32 rows, 128 scales
 
 template <typename T>
 __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __grid_constant__ LinearArgs p) {
@@ -492,7 +503,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
         if (!ok) give_up();
         if (it > 0 && !mbar_wait(accf0 + 8u * ((it - 1) & 1), ((it - 1) >> 1) & 1, nullptr)) give_up();
     } else if (warp >= 2) {  // ------------------------------------ epilogue
+        // Rows one a lane out of tensor memory; 16 tokens x 32 rows at a time
+        // change places in shared memory, so that four lanes write a token's 32 rows.
         const int quarter = warp & 3, half = (warp - 2) >> 2;
+        float *turned = reinterpret_cast<float *>(smem + (b_sa - shared_addr(smem)) + (uint32_t)p.stages * b_bytes) +
+                        (warp - 2) * kWarpFloats;
+        float *xs = turned + 512;
         int32_t it = 0;
         for (int32_t tile = blockIdx.x / 2; tile < tiles; tile += pairs, it++) {
             int32_t r0, t0;
@@ -501,25 +517,48 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             const bool real = r < p.rows;
             const float ws = real ? p.w_scale[r] : 0.f;
             const float bias = real && p.bias ? to_f32(static_cast<const T *>(p.bias)[r]) : 0.f;
+            const int64_t r8 = r - lane + lane % 4 * 8;
+            const int32_t real8 = p.rows - r8 < 8 ? (int32_t)(p.rows - r8) : 8;
+            const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
+            const int32_t begin = half * p.bn / 2, end = min(tokens, begin + p.bn / 2);
+            __syncwarp();
+            for (int32_t i = lane; i < p.bn / 2; i += 32) xs[i] = begin + i < end ? p.x_scale[t0 + begin + i] : 0.f;
+            __syncwarp();
             uint32_t ok = lane ? 1u : (uint32_t)mbar_wait(accf0 + 8u * (it & 1), (it >> 1) & 1, failed);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;");
-            const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
-            const int32_t end = min(tokens, (half + 1) * p.bn / 2);
-            const int32_t begin = half * p.bn / 2;
             const uint32_t acc = tmem + (uint32_t)((it & 1) * p.bn) + ((uint32_t)(32 * quarter) << 16);
-            if (begin < end) {
-                const int64_t at = (int64_t)(t0 + begin) * p.rows + r;
-                const T *mul = p.mul ? static_cast<const T *>(p.mul) + at : nullptr;
-                const T *res = p.residual ? static_cast<const T *>(p.residual) + at : nullptr;
-                T *y = static_cast<T *>(p.y) + at;
-                if (r - lane + 32 <= p.rows && (end - begin) % 16 == 0)
-                    write_columns<T, true>(p, acc + begin, end - begin, ws, bias, p.x_scale + t0 + begin, mul, res, y, true);
-                else
-                    write_columns<T, false>(p, acc + begin, end - begin, ws, bias, p.x_scale + t0 + begin, mul, res, y, real);
+            for (int32_t col = begin; col < end; col += 16) {
+                const int64_t at = (int64_t)(t0 + col + lane / 4) * p.rows + r8;
+                Operands<T> ops[2] = {};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (real8 > 0 && col + 8 * h + lane / 4 < end) load_operands<T>(p, at + 8 * h * p.rows, ops[h]);
+                uint32_t raw[16];
+                tmem_load(acc + (uint32_t)col, raw);
+                float v[16];
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(xs + col - begin + k);
+                    v[k] = __fmaf_rn(__uint_as_float(raw[k]) * ws, x.x, bias);
+                    v[k + 1] = __fmaf_rn(__uint_as_float(raw[k + 1]) * ws, x.y, bias);
+                    v[k + 2] = __fmaf_rn(__uint_as_float(raw[k + 2]) * ws, x.z, bias);
+                    v[k + 3] = __fmaf_rn(__uint_as_float(raw[k + 3]) * ws, x.w, bias);
+                }
+                activate(v, p.act);
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 16; k++) turned[k * 32 + lane] = v[k];
+                __syncwarp();
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float e[8];
+                    load8(turned + (8 * h + lane / 4) * 32 + lane % 4 * 8, e);
+                    if (real8 > 0 && col + 8 * h + lane / 4 < end) write_eight<T>(p, e, at + 8 * h * p.rows, real8, ops[h]);
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
             __syncwarp();
@@ -574,7 +613,7 @@ int e4m3_map(CUtensorMap *map, const uint8_t *p, int64_t rows, int64_t cols, int
 
 template <typename T>
 int launch_linear(const LinearArgs &p, bool pair, int sms, cudaStream_t st) {
-    const int smem = 1024 + p.stages * (int)(kTileA + p.bn * (pair ? 64 : 128));
+    const int smem = 1024 + p.stages * (int)(kTileA + p.bn * (pair ? 64 : 128)) + (pair ? 8 * kWarpFloats * 4 : 0);
     const auto kernel = pair ? linear_pair_kernel<T> : linear_split_kernel<T>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return launch_failed("linear_kernel", e);
@@ -613,13 +652,20 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
     p.rows = rows;
     p.chunks = (int32_t)ceil_div<int64_t>(cols, 128);
     p.act = act;
+    p.vec = rows % 8 == 0 && is_aligned(mul, 16) && is_aligned(residual, 16) && is_aligned(y, 16);
     p.status = status;
     int dev, sms;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return launch_failed("linear", e);
+    // The split form while its 128 x 128 tiles fit the card one an SM; above, the
+    // pair form, except where that needs a second round and the split form still
+    // fits two an SM.  Both, us, at K = 5120: [5120 x 5120], 256 tokens 16.7 split,
+    // 21.0 pair; [17408 x 5120], 256 tokens 33.6, 28.9; [10240 x 5120], 384 tokens
+    // 31.3, 38.2; 512 tokens 54.5, 38.6.
+    const int64_t split_tiles = ceil_div<int64_t>(rows, 128) * ceil_div<int64_t>(m, 128);
     const int64_t pair_tiles = ceil_div<int64_t>(rows, 256) * ceil_div<int64_t>(m, 256);
-    const bool pair = m > 128 && pair_tiles >= sms / 3;
+    const bool pair = m > 128 && split_tiles > sms && (pair_tiles <= sms / 2 || 100 * split_tiles > 185 * sms);
     int64_t row_tiles, token_tiles;
     if (pair) {
         p.bn = 256;
@@ -631,9 +677,17 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
         p.bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
         row_tiles = ceil_div<int64_t>(rows, 128);
         token_tiles = ceil_div<int64_t>(m, p.bn);
-        // two CTAs an SM, each with at least four chunks of columns
-        int64_t splits = 2 * sms / (row_tiles * token_tiles);
-        if (splits > p.chunks / 4) splits = p.chunks / 4;
+        // Up to 32 tokens: nearly two CTAs an SM, which keep more of w in flight
+        // (clusters do not fill every group of SMs: past 1.73 an SM a second round
+        // begins, 23 instead of 18 us at [5120 x 17408]).  Above, the exchange of
+        // the sums weighs more: about one an SM (64 tokens of [5120 x 5120]: 3
+        // splits 10.0 us, 6 12.0), but two splits wherever they fit
+        // (128 tokens of [17408 x 5120]: 1 split 26.7 us, 2 23.1).
+        const int64_t tiles = row_tiles * token_tiles;
+        int64_t splits = (m <= 32 ? 173 : 110) * sms / (100 * tiles);
+        if (m > 32 && splits < 2 && 2 * tiles * 100 <= 185 * sms) splits = 2;
+        const int32_t least = m <= 32 ? 4 : 8;  // chunks of a split
+        if (splits > p.chunks / least) splits = p.chunks / least;
         p.splits = (int32_t)(splits < 1 ? 1 : (splits > 8 ? 8 : splits));
         p.stages = (int32_t)((110 * 1024 - 1024) / (kTileA + p.bn * 128));
         if (p.stages > kMaxStages) p.stages = kMaxStages;
