@@ -1004,22 +1004,16 @@ int split_ctas(const Cache &c, int64_t max_pages, int64_t seqs, int64_t tiles, i
     return (int)(all < most ? all : most);
 }
 
-template <typename K>
-int prepare_attend(K kernel, int smem) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    return e == cudaSuccess ? TANS_B200_OK : launch_failed("attend_kernel", e);
-}
-
 template <typename T, int D>
 int launch_attend(const AttendArgs &p, int max_rows, int ctas, cudaStream_t st) {
     constexpr int smem = AttnLayout<D>::kBytes;
     if (!ctas) {
-        const int rc = prepare_attend(attend_kernel<T, D>, smem);
+        const int rc = allow_smem<attend_kernel<T, D>>("attend_kernel", smem);
         return rc ? rc
                   : launch_ex(attend_kernel<T, D>, dim3(ceil_div(max_rows, 16), p.cache.heads, p.seqs), dim3(kAttnWarps * 32), smem, 1, st,
                               "attend_kernel", p);
     }
-    int rc = prepare_attend(attend_split_kernel<T, D>, smem);
+    int rc = allow_smem<attend_split_kernel<T, D>>("attend_split_kernel", smem);
     if (!rc)
         rc = launch_ex(attend_split_kernel<T, D>, dim3(ctas), dim3(kAttnWarps * 32), smem, 1, st, "attend_split_kernel", p);
     return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, ceil_div(max_rows < 16 ? max_rows : 16, kJoinRows)),
@@ -1132,10 +1126,9 @@ int plan_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64_
     if (max_pages > INT32_MAX || (max_pages << c->page_log2) > INT32_MAX - 4096 ||
         most_new > INT32_MAX || most_new * (q_heads / c->heads) > (1 << 28))
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: a sequence holds at most 2^31-4097 tokens");
-    int dev, sms;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return launch_failed("kv4_attention", e);
+    int sms;
+    rc = current_sms("kv4_attention", &sms);
+    if (rc) return rc;
     *ctas = split_ctas(*c, max_pages, seqs, ceil_div<int64_t>(most_new * (q_heads / c->heads), 16), window, most_new, sms);
     return TANS_B200_OK;
 }

@@ -27,6 +27,7 @@ namespace {
 constexpr int kMaxStages = 8;
 constexpr uint32_t kWaitLimit = 1u << 16;  // polls per wait
 constexpr uint32_t kPollNs = 10000;        // suspend-time hint per poll: bound ~0.66 s
+constexpr int kMaxSmem = 225 * 1024;       // dynamic; the barriers' few bytes are static
 constexpr uint32_t kTileA = 128 * 128;     // bytes of 128 rows x 128 columns
 
 struct LinearArgs {
@@ -614,15 +615,15 @@ int e4m3_map(CUtensorMap *map, const uint8_t *p, int64_t rows, int64_t cols, int
 template <typename T>
 int launch_linear(const LinearArgs &p, bool pair, int sms, cudaStream_t st) {
     const int smem = 1024 + p.stages * (int)(kTileA + p.bn * (pair ? 64 : 128)) + (pair ? 8 * kWarpFloats * 4 : 0);
-    const auto kernel = pair ? linear_pair_kernel<T> : linear_split_kernel<T>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return launch_failed("linear_kernel", e);
+    int rc = pair ? allow_smem<linear_pair_kernel<T>>("linear_pair_kernel", kMaxSmem)
+                  : allow_smem<linear_split_kernel<T>>("linear_split_kernel", kMaxSmem);
+    if (rc) return rc;
     if (pair) {
         const int tiles = p.row_tiles * p.token_tiles, pairs = sms / 2;
-        return launch_ex(kernel, dim3(2u * (tiles < pairs ? tiles : pairs)), dim3(kPairThreads), smem, 2, st,
+        return launch_ex(linear_pair_kernel<T>, dim3(2u * (tiles < pairs ? tiles : pairs)), dim3(kPairThreads), smem, 2, st,
                          "linear_pair_kernel", p);
     }
-    return launch_ex(kernel, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)p.token_tiles), dim3(kSplitThreads), smem,
+    return launch_ex(linear_split_kernel<T>, dim3((unsigned)(p.row_tiles * p.splits), (unsigned)p.token_tiles), dim3(kSplitThreads), smem,
                      p.splits, st, "linear_split_kernel", p);
 }
 
@@ -654,10 +655,9 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
     p.act = act;
     p.vec = rows % 8 == 0 && is_aligned(mul, 16) && is_aligned(residual, 16) && is_aligned(y, 16);
     p.status = status;
-    int dev, sms;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return launch_failed("linear", e);
+    int sms;
+    int rc = current_sms("linear", &sms);
+    if (rc) return rc;
     // The split form while its 128 x 128 tiles fit the card one an SM; above, the
     // pair form, except where that needs a second round and the split form still
     // fits two an SM.  Both, us, at K = 5120: [5120 x 5120], 256 tokens 16.7 split,
@@ -696,7 +696,7 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
         return fail(TANS_B200_ERR_INVALID, "linear: m and rows are too large");
     p.row_tiles = (int32_t)row_tiles;
     p.token_tiles = (int32_t)token_tiles;
-    int rc = e4m3_map(&p.wmap, w, rows, cols, 128);
+    rc = e4m3_map(&p.wmap, w, rows, cols, 128);
     if (!rc) rc = e4m3_map(&p.xmap, x, m, cols, pair ? p.bn / 2 : p.bn);
     if (rc) return rc;
     return dispatch_half(dtype, "linear", [&](auto t) { return launch_linear<decltype(t)>(p, pair, sms, (cudaStream_t)stream); });

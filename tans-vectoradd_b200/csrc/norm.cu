@@ -196,11 +196,8 @@ int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
     if (!vec) {
         const int threads = p.cols >= 1024 ? 512 : (p.cols >= 256 ? 128 : 32);
         const int smem = p.cols * 4;
-        if (smem > 48 * 1024) {
-            const cudaError_t e =
-                cudaFuncSetAttribute(norm_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (e != cudaSuccess) return launch_failed("norm_any_kernel", e);
-        }
+        const int rc = allow_smem<norm_any_kernel<T>>("norm_any_kernel", kMaxCols * 4);
+        if (rc) return rc;
         return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
     }
     const int vecs = p.cols / 8;

@@ -7,7 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -53,6 +53,41 @@ int launch_ex(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, int clus
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
     return e == cudaSuccess ? TANS_B200_OK : launch_failed(name, e);
+}
+
+constexpr int kMaxDevices = 64;
+
+// The current device and its SM count (asked for once per device).
+inline int current_sms(const char *what, int *sms) {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) e = cudaErrorInvalidDevice;
+    if (e != cudaSuccess) return launch_failed(what, e);
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return launch_failed(what, e);
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return TANS_B200_OK;
+}
+
+// Lets `kernel` use up to `bytes` of dynamic shared memory on the current
+// device, which has to be the same for every call: done once per device.
+template <auto kernel>
+int allow_smem(const char *what, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) e = cudaErrorInvalidDevice;
+    if (e != cudaSuccess) return launch_failed(what, e);
+    if (done.load(std::memory_order_relaxed) >> dev & 1) return TANS_B200_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return launch_failed(what, e);
+    done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return TANS_B200_OK;
 }
 
 inline bool is_aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

@@ -7,6 +7,7 @@ reference's L = 4096) is loaded on first use by `lib_for_table(2048)`.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -127,22 +128,26 @@ def check(rc: int, lib: ctypes.CDLL | None = None) -> None:
         raise RuntimeError(msg or f"libtans_b200 error {rc}")
 
 
-class _Here:
-    """Context for a call on the device that is already current."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_CTX = _Here()
+_HERE = contextlib.nullcontext()
 
 
 def on_device(dev: torch.device):
-    """A device guard for `dev`; free of cost where `dev` is already current."""
-    return _HERE_CTX if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    """A device guard for `dev`; nothing to enter where `dev` is already current."""
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+def raw_stream(dev: torch.device) -> int:
+    """The cudaStream_t of torch's current stream on `dev`."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def new(shape: tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    """A dense tensor, uninitialised (torch.empty at half its cost on the host)."""
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=dev)
 
 
 def version() -> str:

@@ -15,51 +15,54 @@ from __future__ import annotations
 
 import torch
 
-from ._C import _post_check, _req, _status, _stream
-from ._lib import LIB, check, on_device
+from ._C import _post_check, _status
+from ._lib import LIB, check, new, on_device, raw_stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
 
 
-def _rows(name: str, t: torch.Tensor, shape=None, dtype=None, device=None) -> int:
+def _rows(name: str, t: torch.Tensor) -> int:
     """Checks [rows, cols] with a dense last dimension; the stride between rows."""
-    _req(t.is_cuda and t.dim() == 2 and t.dtype in _TYPES and (t.stride(1) == 1 or t.shape[1] == 1 or not t.numel()),
-         f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor with dense rows")
-    if shape is not None:
-        _req(t.shape == shape and t.dtype == dtype and t.device == device,
-             f"{name} must have x's shape, type and device")
+    if not t.is_cuda or t.dim() != 2 or t.dtype not in _TYPES or (
+            not t.is_contiguous() and t.stride(1) != 1 and t.shape[1] != 1):
+        raise RuntimeError(f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor with dense rows")
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _like_x(name: str, t: torch.Tensor, x: torch.Tensor) -> int:
+    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+        raise RuntimeError(f"{name} must have x's shape, type and device")
+    return _rows(name, t)
 
 
 def _norm(x, weight, residual, eps, residual_out, quantize):
     xs = _rows("x", x)
     R, C = x.shape
     dev, dt = x.device, x.dtype
-    _req(weight.shape == (C,) and weight.is_contiguous() and weight.device == dev
-         and weight.dtype in (dt, torch.float32), "weight must be a contiguous [cols] tensor of x's type or float32")
+    wt = weight.dtype
+    if (weight.dim() != 1 or weight.shape[0] != C or not weight.is_contiguous() or weight.device != dev
+            or (wt != dt and wt != torch.float32)):
+        raise RuntimeError("weight must be a contiguous [cols] tensor of x's type or float32")
     rs = hs = 0
-    h = residual_out
+    h, r_ptr, h_ptr = x, None, None
+    if residual is not None:
+        rs, r_ptr = _like_x("residual", residual, x), residual.data_ptr()
+    elif residual_out is not None:
+        raise RuntimeError("residual_out needs residual")
     with on_device(dev):
         if residual is not None:
-            rs = _rows("residual", residual, x.shape, dt, dev)
-            if h is None:
-                h = torch.empty((R, C), dtype=dt, device=dev)
-            hs = _rows("residual_out", h, x.shape, dt, dev)
-        else:
-            _req(h is None, "residual_out needs residual")
-        y = q = scale = None
+            h = new((R, C), dt, dev) if residual_out is None else residual_out
+            hs, h_ptr = _like_x("residual_out", h, x), h.data_ptr()
         if quantize:
-            q = torch.empty((R, C), dtype=torch.uint8, device=dev)
-            scale = torch.empty((R,), dtype=torch.float32, device=dev)
+            y, scale = new((R, C), torch.uint8, dev), new((R,), torch.float32, dev)
+            out = (None, y.data_ptr(), scale.data_ptr())
         else:
-            y = torch.empty((R, C), dtype=dt, device=dev)
-        check(LIB.tans_b200_add_rms_norm(
-            x.data_ptr(), xs, None if residual is None else residual.data_ptr(), rs, weight.data_ptr(),
-            _TYPES[weight.dtype], eps, None if h is None else h.data_ptr(), hs, None if y is None else y.data_ptr(),
-            None if q is None else q.data_ptr(), None if scale is None else scale.data_ptr(), R, C, _TYPES[dt],
-            _stream(dev)))
-    return y, q, scale, x if h is None else h
+            y, scale = new((R, C), dt, dev), None
+            out = (y.data_ptr(), None, None)
+        check(LIB.tans_b200_add_rms_norm(x.data_ptr(), xs, r_ptr, rs, weight.data_ptr(), _TYPES[wt], eps, h_ptr, hs,
+                                         *out, R, C, _TYPES[dt], raw_stream(dev)))
+    return y, scale, h
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, *,
@@ -69,7 +72,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     + eps) * weight, both [rows, cols] in x's type (bf16, f16 or f32; f32
     inside, the norm of the unrounded sum).  residual_out may be x or residual:
     then h replaces it."""
-    y, _, _, h = _norm(x, weight, residual, eps, residual_out, False)
+    y, _, h = _norm(x, weight, residual, eps, residual_out, False)
     return y, h
 
 
@@ -78,8 +81,7 @@ def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(q, scale, h): add_rms_norm with y as e4m3 (uint8 [rows, cols]) and one
     f32 scale a row, max|y| -> 448."""
-    _, q, scale, h = _norm(x, weight, residual, eps, residual_out, True)
-    return q, scale, h
+    return _norm(x, weight, residual, eps, residual_out, True)
 
 
 def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -88,10 +90,9 @@ def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     R, C = x.shape
     dev = x.device
     with on_device(dev):
-        q = torch.empty((R, C), dtype=torch.uint8, device=dev)
-        scale = torch.empty((R,), dtype=torch.float32, device=dev)
+        q, scale = new((R, C), torch.uint8, dev), new((R,), torch.float32, dev)
         check(LIB.tans_b200_quantize_tokens(x.data_ptr(), xs, q.data_ptr(), scale.data_ptr(), R, C, _TYPES[x.dtype],
-                                            _stream(dev)))
+                                            raw_stream(dev)))
     return q, scale
 
 
@@ -107,30 +108,33 @@ def linear(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: t
     "silu" or "gelu_tanh".  f32 accumulation, one rounding.  `out` may be mul or
     residual."""
     dev = x8.device
-    _req(x8.is_cuda and x8.dim() == 2 and x8.dtype == torch.uint8 and x8.is_contiguous(),
-         "x8 must be a contiguous CUDA uint8 [tokens, cols] tensor of e4m3 bits")
+    if not x8.is_cuda or x8.dim() != 2 or x8.dtype != torch.uint8 or not x8.is_contiguous():
+        raise RuntimeError("x8 must be a contiguous CUDA uint8 [tokens, cols] tensor of e4m3 bits")
     M, K = x8.shape
-    _req(w8.dim() == 2 and w8.dtype == torch.uint8 and w8.is_contiguous() and w8.device == dev and w8.shape[1] == K,
-         "w8 must be a contiguous uint8 [rows, cols] tensor of e4m3 bits with x8's columns and device")
+    if (w8.dim() != 2 or w8.dtype != torch.uint8 or not w8.is_contiguous() or w8.device != dev
+            or w8.shape[1] != K):
+        raise RuntimeError("w8 must be a contiguous uint8 [rows, cols] tensor of e4m3 bits with x8's columns and device")
     N = w8.shape[0]
-    f32 = torch.float32
-    _req(x_scale.dtype == f32 and x_scale.shape == (M,) and x_scale.is_contiguous() and x_scale.device == dev
-         and w_scale.dtype == f32 and w_scale.shape == (N,) and w_scale.is_contiguous() and w_scale.device == dev,
-         "x_scale must be contiguous f32 [tokens] and w_scale [rows]")
-    _req(act in _ACTS, f"act must be one of {', '.join(_ACTS)}")
-    _req(dtype in (torch.bfloat16, torch.float16), "dtype must be bfloat16 or float16")
+    for t, n in ((x_scale, M), (w_scale, N)):
+        if (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()
+                or t.device != dev):
+            raise RuntimeError("x_scale must be contiguous f32 [tokens] and w_scale [rows]")
+    if act not in _ACTS:
+        raise RuntimeError(f"act must be one of {', '.join(_ACTS)}")
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise RuntimeError("dtype must be bfloat16 or float16")
     for name, t, shape in (("bias", bias, (N,)), ("mul", mul, (M, N)), ("residual", residual, (M, N)),
                            ("out", out, (M, N))):
-        _req(t is None or (t.shape == shape and t.dtype == dtype and t.is_contiguous() and t.device == dev),
-             f"{name} must be a contiguous {dtype} tensor of shape {shape} on x8's device")
+        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != dev):
+            raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on x8's device")
     with on_device(dev):
         if out is None:
-            out = torch.empty((M, N), dtype=dtype, device=dev)
+            out = new((M, N), dtype, dev)
         check(LIB.tans_b200_linear(
             x8.data_ptr(), x_scale.data_ptr(), w8.data_ptr(), w_scale.data_ptr(),
             None if bias is None else bias.data_ptr(), _ACTS[act], None if mul is None else mul.data_ptr(),
             None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, _TYPES[dtype],
-            _status(dev).data_ptr(), _stream(dev)))
+            _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return out
 

@@ -17,12 +17,13 @@ never followed and shows in `rans_vectoradd._C.data_status()` (bit 16).
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
 
-from ._C import _post_check, _req, _status, _stream
-from ._lib import LIB, KV4, check, on_device
+from ._C import _post_check, _req, _status
+from ._lib import LIB, KV4, check, new, on_device, raw_stream
 
 _HALF = {torch.bfloat16: 0, torch.float16: 1}
 _FLOAT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -92,18 +93,20 @@ class KV4Cache:
 
 def _heads(name: str, t: torch.Tensor, cache: KV4Cache, dtype: torch.dtype) -> int:
     """Checks [tokens, heads, dim] with dense heads; the stride between tokens."""
-    D = cache.head_dim
-    _req(t.dim() == 3 and t.shape[2] == D and t.dtype == dtype and t.device == cache.device,
-         f"{name} must be [tokens, heads, {D}] {dtype} on the cache's device")
+    D = cache._c.dim
+    if t.dim() != 3 or t.shape[2] != D or t.dtype != dtype or t.device != cache.k_codes.device:
+        raise RuntimeError(f"{name} must be [tokens, heads, {D}] {dtype} on the cache's device")
+    if t.is_contiguous():
+        return t.shape[1] * D
     st = t.stride()
-    _req((st[2] == 1 and (st[1] == D or t.shape[1] == 1)) or t.numel() == 0,
-         f"{name}'s heads must be dense (strides {D} and 1)")
+    if st[2] != 1 or (st[1] != D and t.shape[1] != 1):
+        raise RuntimeError(f"{name}'s heads must be dense (strides {D} and 1)")
     return st[0] if t.shape[0] > 1 else t.shape[1] * D
 
 
 def _index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: torch.device) -> int:
-    _req(t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == dev,
-         f"{name} must be a contiguous {dtype} tensor of {n} on the cache's device")
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of {n} on the cache's device")
     return t.data_ptr()
 
 
@@ -117,7 +120,8 @@ def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
     [max_position, half] (pairs (i, i + half), or (2i, 2i+1) if interleaved;
     2 * half <= dim).  Returns q [tokens, q_heads, dim] rotated alike, if given."""
     dt, dev = k.dtype, cache.device
-    _req(dt in _HALF, "k must be bfloat16 or float16")
+    if dt not in _HALF:
+        raise RuntimeError("k must be bfloat16 or float16")
     ks, vs = _heads("k", k, cache, dt), _heads("v", v, cache, dt)
     T = k.shape[0]
     _req(k.shape[1] == cache.heads and v.shape == k.shape, "k and v must have the cache's heads")
@@ -138,11 +142,11 @@ def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
         _req(q.shape[0] == T, "q must have k's tokens")
     with on_device(dev):
         if q is not None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
+            out = new(q.shape, dt, dev)
         check(LIB.tans_b200_kv4_append(
             cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, _index("slots", slots, T, torch.int64, dev),
             None if q is None else q.data_ptr(), qs, qh, None if out is None else out.data_ptr(), pos_p, cos_p,
-            sin_p, top, half, int(interleaved), T, _HALF[dt], _status(dev).data_ptr(), _stream(dev)))
+            sin_p, top, half, int(interleaved), T, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return out
 
@@ -154,12 +158,23 @@ def read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat
     _req(dtype in _FLOAT, "dtype must be bfloat16, float16 or float32")
     dev, T = cache.device, slots.shape[0]
     with on_device(dev):
-        k = torch.empty((T, cache.heads, cache.head_dim), dtype=dtype, device=dev)
+        k = new((T, cache._c.heads, cache._c.dim), dtype, dev)
         v = torch.empty_like(k)
         check(LIB.tans_b200_kv4_read(cache._ref, _index("slots", slots, T, torch.int64, dev), k.data_ptr(),
-                                     v.data_ptr(), T, _FLOAT[dtype], _status(dev).data_ptr(), _stream(dev)))
+                                     v.data_ptr(), T, _FLOAT[dtype], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return k, v
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_workspace_bytes(heads: int, page_size: int, head_dim: int, q_heads: int, max_pages: int, seqs: int,
+                              tokens: int, most_new: int, window: int, device: torch.device) -> int:
+    """Bytes of `attention`'s workspace: it follows from the sizes and the device alone."""
+    c, n = KV4(256, 256, 256, 256, None, None, 1, heads, page_size, head_dim), ctypes.c_int64()
+    with on_device(device):
+        check(LIB.tans_b200_kv4_attention_workspace_bytes(ctypes.addressof(c), q_heads, max_pages, seqs, tokens,
+                                                          most_new, window, ctypes.byref(n)))
+    return n.value
 
 
 def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
@@ -177,30 +192,30 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
     least `attention_workspace_bytes`, else allocated."""
     dt, dev = q.dtype, cache.device
-    _req(dt in _HALF, "q must be bfloat16 or float16")
+    if dt not in _HALF:
+        raise RuntimeError("q must be bfloat16 or float16")
     qs = _heads("q", q, cache, dt)
     T, H, D = q.shape
     B = lens.shape[0] if lens.dim() == 1 else -1
-    _req(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] == B and table.device == dev
-         and (table.stride(1) == 1 or table.shape[1] <= 1), "table must be int32 [seqs, max_pages], rows dense")
+    if (table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B or table.device != dev
+            or not (table.is_contiguous() or table.stride(1) == 1 or table.shape[1] <= 1)):
+        raise RuntimeError("table must be int32 [seqs, max_pages], rows dense")
     lens_p = _index("lens", lens, B, torch.int32, dev)
     starts_p = None if starts is None else _index("starts", starts, B + 1, torch.int32, dev)
     P = table.shape[1]
     with on_device(dev):
-        out = torch.empty(q.shape, dtype=dt, device=dev)
-        lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
-        need = ctypes.c_int64()
-        check(LIB.tans_b200_kv4_attention_workspace_bytes(cache._ref, H, P, B, T, most_new, window,
-                                                          ctypes.byref(need)))
-        if need.value and workspace is None:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        out = new(q.shape, dt, dev)
+        lse = new((T, H), torch.float32, dev) if return_lse else None
+        need = attention_workspace_bytes(cache.heads, cache.page_size, D, H, P, B, T, most_new, window, dev)
+        if need and workspace is None:
+            workspace = new((need,), torch.uint8, dev)
         ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
         check(LIB.tans_b200_kv4_attention(
             cache._ref, q.data_ptr(), qs, H, table.data_ptr(), table.stride(0), P, lens_p, starts_p, B, T, most_new,
             D ** -0.5 if scale is None else scale, window, out.data_ptr(), None if lse is None else lse.data_ptr(),
-            ws, ws_bytes, _HALF[dt], _status(dev).data_ptr(), _stream(dev)))
+            ws, ws_bytes, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return (out, lse) if return_lse else out
 
 
-__all__ = ["KV4Cache", "append", "read", "attention"]
+__all__ = ["KV4Cache", "append", "read", "attention", "attention_workspace_bytes"]

@@ -160,7 +160,8 @@ def check_linear(x8, xs, w8, ws, bias=None, act="none", mul=None, residual=None,
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 128, 128), (1, 5120, 1024), (2, 129, 144), (15, 77, 4096),
                                    (17, 640, 5120), (33, 1000, 272), (64, 5120, 17408), (65, 256, 128),
                                    (129, 384, 1040), (200, 130, 2064), (257, 1024, 512), (512, 2048, 512),
-                                   (700, 1111, 784), (1025, 300, 2048)])
+                                   (700, 1111, 784), (1025, 300, 2048), (300, 6500, 272), (129, 12700, 144),
+                                   (2000, 1700, 512), (1500, 5001, 400), (4100, 2600, 16), (384, 10240, 1024)])
 def test_linear_matches_formula(cuda, m, n, k):
     x8, xs = quantized(m, k, m + n, cuda)
     w8, ws = quantized(n, k, k, cuda, 0.02)
