@@ -58,114 +58,191 @@ struct AppendArgs {
     const int64_t *positions;              // rows of cos and sin
     const float *cos, *sin;                // [max_position][half]
     int64_t max_position;
-    int32_t tokens, q_heads, dim, half;    // 2 * half elements of a head are rotated
+    int32_t tokens, q_heads, dim, dim_log2, half;  // 2 * half elements of a head are rotated
+    int32_t per;                                   // heads of a thread
     bool interleaved;
     int32_t *status;
 };
 
-// Sixteen elements e0 .. e0 + 15 of one head, rotated by its token's angle.
-// The products and the sum round one by one.
-template <typename T>
-__device__ __forceinline__ void load_rotated(const T *head, int e0, const float *cs, const float *sn, int half,
-                                             bool interleaved, float (&x)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 8) load8(head + e0 + i, reinterpret_cast<float(&)[8]>(x[i]));
-    if (e0 >= 2 * half || !cs) return;
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int e = e0 + i;
-        if (e < 2 * half) {
-            const bool second = interleaved ? (e & 1) : e >= half;
-            const int pair = interleaved ? e >> 1 : (second ? e - half : e);
-            const int other = interleaved ? e ^ 1 : (second ? e - half : e + half);
-            const float o = to_f32(head[other]), c = cs[pair], s = sn[pair];
-            x[i] = second ? __fadd_rn(__fmul_rn(x[i], c), __fmul_rn(o, s))
-                          : __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(o, s));
-        }
-    }
-}
+// How a call's rotation lies to a thread's eight elements: none; pairs (i,
+// i + half), the partners eight in a row as well (half a multiple of 8); pairs
+// of neighbours (interleaved, half a multiple of 4); anything else.
+enum Rotation { kNoTurn, kHalves, kNeighbours, kMixed };
 
-// Codes (8 bytes) and scale byte of sixteen values.
-__device__ __forceinline__ uint2 quantize16(const float (&x)[16], uint32_t &scale) {
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) amax = max_nan(amax, fabsf(x[i]));
-    scale = e4m3x2(amax / 6.f, 0.f);
-    scale &= 0xFFu;
-    const float s = e4m3_f32(scale);
-    uint32_t w[2] = {0u, 0u};
-    if (s != 0.f) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            uint32_t b;
-            asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\n\t"
-                "mov.b32 %0, {b, 0, 0, 0};\n\t}"
-                : "=r"(b)
-                : "f"(x[i + 1] / s), "f"(x[i] / s));
-            w[i >> 3] |= (b & 0xFFu) << (4 * (i & 7));
-        }
-    }
-    return make_uint2(w[0], w[1]);
-}
+// The angles of elements e0 .. e0 + 7 of a head, kept for all heads of a
+// token: a rotated element becomes x * c + partner * s, each product and the
+// sum rounded (s negative for the first of a pair).
+template <Rotation R>
+struct Turn {
+    float c[8], s[8];
+    uint32_t rotated;  // bit i: element i is (all or none but for kMixed)
+    int partner;       // kHalves: where the partners lie
 
-// One thread per 16 elements: key groups, value groups, then query groups of
-// a token.
-template <typename T>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
-    pdl_enter();
-    const int groups = p.dim / 16;
-    const int kv = p.cache.heads * groups, per_token = 2 * kv + (p.q ? p.q_heads * groups : 0);
-    const int64_t total = (int64_t)p.tokens * per_token;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int token = (int)(i / per_token);
-        int rest = (int)(i - (int64_t)token * per_token);
-        const float *cs = nullptr, *sn = nullptr;
-        if (p.half && !(rest >= kv && rest < 2 * kv)) {
-            const int64_t pos = p.positions[token];
-            if (pos < 0 || pos >= p.max_position) {
-                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            } else {
-                cs = p.cos + pos * p.half;
-                sn = p.sin + pos * p.half;
+    __device__ __forceinline__ void set(const float *cs, const float *sn, int e0, int half, bool interleaved) {
+        if (e0 >= 2 * half) return;
+        if constexpr (R == kNeighbours) {
+            const float4 a = *reinterpret_cast<const float4 *>(cs + e0 / 2), b = *reinterpret_cast<const float4 *>(sn + e0 / 2);
+            c[0] = c[1] = a.x, c[2] = c[3] = a.y, c[4] = c[5] = a.z, c[6] = c[7] = a.w;
+            s[0] = -b.x, s[1] = b.x, s[2] = -b.y, s[3] = b.y, s[4] = -b.z, s[5] = b.z, s[6] = -b.w, s[7] = b.w;
+            rotated = 0xFFu;
+        } else if constexpr (R == kHalves) {
+            const bool first = e0 < half;
+            load8(cs + (first ? e0 : e0 - half), c);
+            load8(sn + (first ? e0 : e0 - half), s);
+            if (first) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[i] = -s[i];
+            }
+            partner = first ? half : -half;
+            rotated = 0xFFu;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int e = e0 + i;
+                if (e < 2 * half) {
+                    const bool second = interleaved ? (e & 1) : e >= half;
+                    const int pair = interleaved ? e >> 1 : (second ? e - half : e);
+                    rotated |= 1u << i;
+                    c[i] = cs[pair];
+                    s[i] = second ? sn[pair] : -sn[pair];
+                }
             }
         }
-        float x[16];
-        if (rest >= 2 * kv) {
-            rest -= 2 * kv;
-            const T *head = static_cast<const T *>(p.q) + token * p.q_stride + (int64_t)(rest / groups) * p.dim;
-            load_rotated(head, rest % groups * 16, cs, sn, p.half, p.interleaved, x);
-            T *out = static_cast<T *>(p.q_out) + ((int64_t)token * p.q_heads * groups + rest) * 16;
+    }
+};
+
+// A thread's eight elements of one head, and their partners.
+template <typename T, Rotation R>
+struct Loaded {
+    Eight<T> own, other;
+    __device__ __forceinline__ void load(const T *at, const Turn<R> &t) {
+        own = load_eight(at);
+        if constexpr (R == kHalves) other = load_eight(at + t.partner);
+    }
+    // at: where they lie, for kMixed
+    __device__ __forceinline__ void turn(const Turn<R> &t, const T *at, int e0, int half, bool interleaved, float (&x)[8]) const {
+        own.to(x);
+        if constexpr (R == kNoTurn) return;
+        float o[8];
+        if constexpr (R == kHalves) {
+            other.to(o);
+        } else if constexpr (R == kNeighbours) {
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) store8(out + j, reinterpret_cast<float(&)[8]>(x[j]));
-            continue;
+            for (int i = 0; i < 8; i++) o[i] = x[i ^ 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                o[i] = t.rotated >> i & 1 ? to_f32(at[interleaved ? i ^ 1 : (e0 + i < half ? i + half : i - half)]) : 0.f;
         }
-        const int64_t slot = p.slots[token];
-        if (slot < 0) continue;
-        if (slot >= (p.cache.pages << p.cache.page_log2)) {
-            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            continue;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float y = __fadd_rn(__fmul_rn(x[i], t.c[i]), __fmul_rn(o[i], t.s[i]));
+            x[i] = (R == kMixed ? t.rotated >> i & 1 : t.rotated) ? y : x[i];
         }
-        const bool value = rest >= kv;
-        if (value) rest -= kv;
-        const int head = rest / groups, g = rest % groups;
-        const T *src = static_cast<const T *>(value ? p.v : p.k) + token * (value ? p.v_stride : p.k_stride) +
-                       (int64_t)head * p.dim;
-        if (value)
-            load_rotated(src, g * 16, nullptr, nullptr, 0, false, x);
-        else
-            load_rotated(src, g * 16, cs, sn, p.half, p.interleaved, x);
-        const float *gain = value ? p.cache.v_gain : p.cache.k_gain;
+    }
+};
+
+// Codes (4 bytes) of eight values and the scale byte of the sixteen of them
+// and of the neighbouring lane (lane ^ 1, which runs along).
+__device__ __forceinline__ uint32_t quantize(const float (&x)[8], uint32_t &scale) {
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) amax = max_nan(amax, fabsf(x[i]));
+    amax = max_nan(amax, __shfl_xor_sync(3u << (threadIdx.x & 30), amax, 1));
+    scale = e4m3x2(amax / 6.f, 0.f) & 0xFFu;
+    const float s = e4m3_f32(scale);
+    uint32_t w = 0;
+    if (s != 0.f) {
+        asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+            "mov.b32 %0, {a, b, c, d};\n\t}"
+            : "=r"(w)
+            : "f"(x[0] / s), "f"(x[1] / s), "f"(x[2] / s), "f"(x[3] / s), "f"(x[4] / s), "f"(x[5] / s), "f"(x[6] / s),
+              "f"(x[7] / s));
+    }
+    return w;
+}
+
+// Heads h0 .. h1 - 1 of keys or values into the cache; src: this thread's
+// elements of head 0, at: its group of head 0 in the cache, in units of 8.
+template <typename T, Rotation R>
+__device__ __forceinline__ void store_heads(const AppendArgs &p, const T *src, int h0, int h1, const Turn<R> &turn, int e0,
+                                            const float *gain, uint8_t *codes, uint8_t *scales, int64_t at,
+                                            int64_t head_step) {
+    src += (int64_t)h0 << p.dim_log2;
+    at += h0 * head_step;
+    Loaded<T, R> next;
+    next.load(src, turn);
+    for (int h = h0; h < h1; h++, src += p.dim, at += head_step) {
+        const Loaded<T, R> now = next;
+        if (h + 1 < h1) next.load(src + p.dim, turn);
+        float x[8];
+        now.turn(turn, src, e0, p.half, p.interleaved, x);
         if (gain) {
-            const float d = gain[head];
+            const float d = gain[h];
 #pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = x[j] / d;
+            for (int j = 0; j < 8; j++) x[j] = x[j] / d;
         }
         uint32_t scale;
-        const uint2 codes = quantize16(x, scale);
-        const int64_t at = token_at(p.cache, slot >> p.cache.page_log2, head,
-                                    (int)(slot & ((1 << p.cache.page_log2) - 1))) * groups + g;
-        reinterpret_cast<uint2 *>(value ? p.cache.v_codes : p.cache.k_codes)[at] = codes;
-        (value ? p.cache.v_scales : p.cache.k_scales)[at] = (uint8_t)scale;
+        reinterpret_cast<uint32_t *>(codes)[at] = quantize(x, scale);
+        if (!(e0 & 8)) scales[at / 2] = (uint8_t)scale;
+    }
+}
+
+// A thread has eight elements of one token, for p.per of its heads in turn
+// (keys, values, then queries; blockIdx.y is which), the next head's loaded
+// while the present one's are worked out; the angles are read once for them.
+// A warp's lanes lie side by side in a head.
+template <typename T, Rotation R>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
+    pdl_enter();
+    const int kv = p.cache.heads, heads = 2 * kv + p.q_heads, groups_log2 = p.dim_log2 - 3;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int token = i >> groups_log2, group = i & ((1 << groups_log2) - 1), e0 = 8 * group;
+    if (token >= p.tokens) return;
+    const int h0 = (int)blockIdx.y * p.per, h1 = min(heads, h0 + p.per);
+    Turn<R> turn;
+    turn.rotated = 0;
+    turn.partner = 0;
+    if (R != kNoTurn && !(h0 >= kv && h1 <= 2 * kv)) {
+        const int64_t pos = p.positions[token];
+        if (pos < 0 || pos >= p.max_position) {
+            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+        } else {
+            turn.set(p.cos + pos * p.half, p.sin + pos * p.half, e0, p.half, p.interleaved);
+        }
+    }
+    if (h0 < 2 * kv) {
+        const int64_t slot = p.slots[token];
+        if (slot >= (p.cache.pages << p.cache.page_log2)) {
+            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+        } else if (slot >= 0) {
+            const int64_t at = (token_at(p.cache, slot >> p.cache.page_log2, 0, (int)(slot & ((1 << p.cache.page_log2) - 1)))
+                                << groups_log2) + group;
+            const int64_t head_step = (int64_t)1 << (p.cache.page_log2 + groups_log2);
+            if (h0 < kv)
+                store_heads<T, R>(p, static_cast<const T *>(p.k) + token * p.k_stride + e0, h0, min(h1, kv), turn, e0,
+                                  p.cache.k_gain, p.cache.k_codes, p.cache.k_scales, at, head_step);
+            if (h1 > kv)
+                store_heads<T, kNoTurn>(p, static_cast<const T *>(p.v) + token * p.v_stride + e0, max(h0 - kv, 0),
+                                        min(h1 - kv, kv), Turn<kNoTurn>{}, e0, p.cache.v_gain, p.cache.v_codes,
+                                        p.cache.v_scales, at, head_step);
+        }
+    }
+    if (h1 > 2 * kv) {
+        const int q0 = max(h0 - 2 * kv, 0), q1 = h1 - 2 * kv;
+        const T *src = static_cast<const T *>(p.q) + token * p.q_stride + ((int64_t)q0 << p.dim_log2) + e0;
+        T *dst = static_cast<T *>(p.q_out) + (((int64_t)token * p.q_heads + q0) << p.dim_log2) + e0;
+        Loaded<T, R> next;
+        next.load(src, turn);
+        for (int h = q0; h < q1; h++, src += p.dim, dst += p.dim) {
+            const Loaded<T, R> now = next;
+            if (h + 1 < q1) next.load(src + p.dim, turn);
+            float x[8];
+            now.turn(turn, src, e0, p.half, p.interleaved, x);
+            store8(dst, x);
+        }
     }
 }
 
@@ -1064,9 +1141,9 @@ extern "C" int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, i
     if (half < 0 || 2 * half > cache->dim || (half && (!positions || !cos || !sin || max_position < 1)))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_append: half must be 0..dim/2, with positions, cos and sin where it is not 0");
-    if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(q, 16) || !is_aligned(q_out, 16) || k_stride % 8 ||
+    if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(q, 16) || !is_aligned(q_out, 16) || !is_aligned(cos, 16) || !is_aligned(sin, 16) || k_stride % 8 ||
         v_stride % 8 || (q && q_stride % 8))
-        return fail(TANS_B200_ERR_INVALID, "kv4_append: q, k and v must be 16-byte aligned, their strides multiples of 8");
+        return fail(TANS_B200_ERR_INVALID, "kv4_append: q, k, v, cos and sin must be 16-byte aligned, the strides multiples of 8");
     p.q = q;
     p.k = k;
     p.v = v;
@@ -1085,10 +1162,30 @@ extern "C" int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, i
     p.half = (int32_t)half;
     p.interleaved = interleaved != 0;
     p.status = status;
-    const int64_t total = tokens * (2 * (int64_t)p.cache.heads + p.q_heads) * (p.dim / 16);
+    int sms;
+    rc = current_sms("kv4_append", &sms);
+    if (rc) return rc;
+    // as many heads a thread as leave 1024 threads an SM, at most 8
+    const int64_t heads = 2 * (int64_t)p.cache.heads + p.q_heads, groups = p.dim / 8;
+    if (tokens * groups > INT32_MAX - 256) return fail(TANS_B200_ERR_INVALID, "kv4_append: too many tokens for one call");
+    const int64_t per = tokens * groups * heads / (1024 * (int64_t)sms);
+    p.per = (int32_t)(per < 1 ? 1 : (per > 8 ? 8 : per));
+    p.dim_log2 = __builtin_ctz((unsigned)p.dim);
+    const dim3 grid((unsigned)ceil_div<int64_t>(tokens * groups, 256), (unsigned)ceil_div<int64_t>(heads, p.per));
+    if (grid.y > 65535) return fail(TANS_B200_ERR_INVALID, "kv4_append: too many heads");
+    const Rotation r = p.half == 0 ? kNoTurn
+                                   : (p.interleaved ? (p.half % 4 ? kMixed : kNeighbours) : (p.half % 8 ? kMixed : kHalves));
     return dispatch_half(dtype, "kv4_append", [&](auto t) {
-        return launch_ex(append_kernel<decltype(t)>, dim3(flat_grid(total)), dim3(256), 0, 1, (cudaStream_t)stream,
-                         "append_kernel", p);
+        using T = decltype(t);
+        const auto launch = [&](auto kernel) {
+            return launch_ex(kernel, grid, dim3(256), 0, 1, (cudaStream_t)stream, "append_kernel", p);
+        };
+        switch (r) {
+            case kNoTurn: return launch(append_kernel<T, kNoTurn>);
+            case kHalves: return launch(append_kernel<T, kHalves>);
+            case kNeighbours: return launch(append_kernel<T, kNeighbours>);
+            default: return launch(append_kernel<T, kMixed>);
+        }
     });
 }
 

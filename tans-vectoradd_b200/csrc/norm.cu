@@ -53,94 +53,88 @@ __device__ __forceinline__ void block_reduce(float &a, float &b, float2 *buf) {
     }
 }
 
-// The row's factor and quantisation scale from its sum of squares and max|s * w|.
-__device__ __forceinline__ void row_factors(const NormArgs &p, float sumsq, float amax, float &inv,
-                                            float &scale) {
-    inv = p.norm ? rsqrtf(sumsq / (float)p.cols + p.eps) : 1.f;
+// From a row's sum of squares and max|s * w|: what brings s * w to y, or to
+// y / scale when quantising, and the scale.  There the root cancels, y / scale
+// = s * w * 448 / max|s * w|, one rounding less; sizes far out of range (and
+// NaN) take the long way.
+__device__ __forceinline__ float row_factor(const NormArgs &p, float sumsq, float amax, float &scale) {
+    const float inv = p.norm ? rsqrtf(sumsq / (float)p.cols + p.eps) : 1.f;
+    if (!p.q) return inv;
     const float top = amax * inv;
     scale = top == 0.f ? 1.f : max_nan(top / 448.f, 1.17549435e-38f);
+    return amax > 1e-30f && amax < 1e30f && top > 1e-30f ? 448.f / amax : inv / scale;
 }
 
 // Rows of whole 8-element vectors, 16-byte aligned everywhere: thread t holds
 // vectors t, t + blockDim, ...
-template <typename T, int VPT>
-__global__ void __launch_bounds__(1024) norm_vec_kernel(const NormArgs p) {
+template <typename T, int VPT, int kMost>
+__global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     __shared__ float2 buf[32];
     pdl_enter();
     const int64_t row = blockIdx.x;
     const int vecs = p.cols / 8;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
-    float s[VPT][8];
+    // every load of the row before the first use of one
+    Eight<T> xv[VPT], rv[VPT], wv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int v = threadIdx.x + i * blockDim.x;
-        if (v < vecs) load8(x + 8 * v, s[i]);
-    }
-    if (r) {
-        T *h = static_cast<T *>(p.h) + row * p.h_stride;
-#pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int v = threadIdx.x + i * blockDim.x;
-            if (v < vecs) {
-                float a[8];
-                load8(r + 8 * v, a);
-#pragma unroll
-                for (int k = 0; k < 8; k++) s[i][k] += a[k];
-                store8(h + 8 * v, s[i]);
-            }
+        if (v < vecs) {
+            xv[i] = load_eight(x + 8 * v);
+            if (r) rv[i] = load_eight(r + 8 * v);
+            if (p.norm && !p.weight_f32) wv[i] = load_eight(static_cast<const T *>(p.weight) + 8 * v);
         }
     }
+    float s[VPT][8];
     float sumsq = 0.f, amax = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < vecs) {
-            float w[8];
-            if (!p.norm) {
+            xv[i].to(s[i]);
+            if (r) {
+                float a[8];
+                rv[i].to(a);
 #pragma unroll
-                for (int k = 0; k < 8; k++) w[k] = 1.f;
-            } else if (p.weight_f32) {
-                load8(static_cast<const float *>(p.weight) + 8 * v, w);
-            } else {
-                load8(static_cast<const T *>(p.weight) + 8 * v, w);
+                for (int k = 0; k < 8; k++) s[i][k] += a[k];
+                store8(static_cast<T *>(p.h) + row * p.h_stride + 8 * v, s[i]);
             }
+            if (p.norm) {
+                float w[8];
+                if (p.weight_f32)
+                    load8(static_cast<const float *>(p.weight) + 8 * v, w);
+                else
+                    wv[i].to(w);
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                sumsq += s[i][k] * s[i][k];
-                s[i][k] *= w[k];
-                amax = max_nan(amax, fabsf(s[i][k]));
+                for (int k = 0; k < 8; k++) {
+                    sumsq = __fmaf_rn(s[i][k], s[i][k], sumsq);
+                    s[i][k] *= w[k];
+                }
+            }
+            if (p.q) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) amax = max_nan(amax, fabsf(s[i][k]));
             }
         }
     }
     block_reduce(sumsq, amax, buf);
-    float inv, scale;
-    row_factors(p, sumsq, amax, inv, scale);
-    if (p.q) {
-        if (threadIdx.x == 0) p.scale[row] = scale;
-        uint8_t *q = p.q + row * p.cols;
+    float scale;
+    const float f = row_factor(p, sumsq, amax, scale);
+    if (p.q && threadIdx.x == 0) p.scale[row] = scale;
 #pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int v = threadIdx.x + i * blockDim.x;
-            if (v < vecs) {
-                float y[8];
+    for (int i = 0; i < VPT; i++) {
+        const int v = threadIdx.x + i * blockDim.x;
+        if (v < vecs) {
 #pragma unroll
-                for (int k = 0; k < 8; k++) y[k] = s[i][k] * inv / scale;
+            for (int k = 0; k < 8; k++) s[i][k] *= f;
+            if (p.q) {
                 uint2 u;
-                u.x = e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16;
-                u.y = e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16;
-                *reinterpret_cast<uint2 *>(q + 8 * v) = u;
-            }
-        }
-    } else {
-        T *y = static_cast<T *>(p.y) + row * p.cols;
-#pragma unroll
-        for (int i = 0; i < VPT; i++) {
-            const int v = threadIdx.x + i * blockDim.x;
-            if (v < vecs) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) s[i][k] *= inv;
-                store8(y + 8 * v, s[i]);
+                u.x = e4m3x2(s[i][0], s[i][1]) | e4m3x2(s[i][2], s[i][3]) << 16;
+                u.y = e4m3x2(s[i][4], s[i][5]) | e4m3x2(s[i][6], s[i][7]) << 16;
+                *reinterpret_cast<uint2 *>(p.q + row * p.cols + 8 * v) = u;
+            } else {
+                store8(static_cast<T *>(p.y) + row * p.cols + 8 * v, s[i]);
             }
         }
     }
@@ -170,13 +164,13 @@ __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
         srow[c] = s;
     }
     block_reduce(sumsq, amax, buf);
-    float inv, scale;
-    row_factors(p, sumsq, amax, inv, scale);
+    float scale;
+    const float f = row_factor(p, sumsq, amax, scale);
     if (p.q && threadIdx.x == 0) p.scale[row] = scale;
     for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-        const float y = srow[c] * inv;
+        const float y = srow[c] * f;
         if (p.q)
-            p.q[row * p.cols + c] = (uint8_t)e4m3x2(y / scale, 0.f);
+            p.q[row * p.cols + c] = (uint8_t)e4m3x2(y, 0.f);
         else
             static_cast<T *>(p.y)[row * p.cols + c] = from_f32<T>(y);
     }
@@ -201,11 +195,15 @@ int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
         return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
     }
     const int vecs = p.cols / 8;
-    // four vectors a thread keep a row's loads in flight at once with many rows resident
+    // four vectors a thread: a row's loads are in flight at once, with many rows resident
     const int threads = ceil_div(ceil_div(vecs, 4), 32) * 32;
-    if (vecs <= threads) return launch_ex(norm_vec_kernel<T, 1>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
-    if (vecs <= 2 * threads) return launch_ex(norm_vec_kernel<T, 2>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
-    return launch_ex(norm_vec_kernel<T, 4>, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
+    const auto launch = [&](auto kernel) {
+        return launch_ex(kernel, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
+    };
+    if (vecs <= threads) return launch(norm_vec_kernel<T, 1, 32>);
+    if (vecs <= 2 * threads) return launch(norm_vec_kernel<T, 2, 32>);
+    if (threads <= 256) return launch(norm_vec_kernel<T, 4, 256>);
+    return launch(norm_vec_kernel<T, 4, 1024>);
 }
 
 int check_rows(const char *what, int64_t rows, int64_t cols) {

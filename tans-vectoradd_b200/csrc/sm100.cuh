@@ -148,6 +148,24 @@ __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
     }
 }
 
+// Eight consecutive values as they lie in memory, 16-byte aligned.
+template <typename T>
+struct Eight {
+    uint4 u[sizeof(T) / 2];
+    __device__ __forceinline__ void to(float (&v)[8]) const {
+        const T *e = reinterpret_cast<const T *>(u);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
+    }
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *p) {
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.u[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
+}
+
 // Two e4m3 bytes (low byte = lo), round to nearest even, clamped to +-448;
 // NaN becomes 0x7F.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
