@@ -67,6 +67,7 @@ struct AppendArgs {
 // How a call's rotation lies to a thread's eight elements: none; pairs (i,
 // i + half), the partners eight in a row as well (half a multiple of 8); pairs
 // of neighbours (interleaved, half a multiple of 4); anything else.
+constexpr int kBatch = 4;  // heads whose loads are in flight together
 enum Rotation { kNoTurn, kHalves, kNeighbours, kMixed };
 
 // The angles of elements e0 .. e0 + 7 of a head, kept for all heads of a
@@ -172,28 +173,32 @@ __device__ __forceinline__ void store_heads(const AppendArgs &p, const T *src, i
                                             int64_t head_step) {
     src += (int64_t)h0 << p.dim_log2;
     at += h0 * head_step;
-    Loaded<T, R> next;
-    next.load(src, turn);
-    for (int h = h0; h < h1; h++, src += p.dim, at += head_step) {
-        const Loaded<T, R> now = next;
-        if (h + 1 < h1) next.load(src + p.dim, turn);
-        float x[8];
-        now.turn(turn, src, e0, p.half, p.interleaved, x);
-        if (gain) {
-            const float d = gain[h];
+    for (int h = h0; h < h1; h += kBatch, src += kBatch * p.dim, at += kBatch * head_step) {
+        Loaded<T, R> l[kBatch];
 #pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = x[j] / d;
+        for (int b = 0; b < kBatch; b++)
+            if (h + b < h1) l[b].load(src + b * p.dim, turn);
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) {
+            if (h + b >= h1) break;
+            float x[8];
+            l[b].turn(turn, src + b * p.dim, e0, p.half, p.interleaved, x);
+            if (gain) {
+                const float d = gain[h + b];
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = x[j] / d;
+            }
+            uint32_t scale;
+            reinterpret_cast<uint32_t *>(codes)[at + b * head_step] = quantize(x, scale);
+            if (!(e0 & 8)) scales[(at + b * head_step) / 2] = (uint8_t)scale;
         }
-        uint32_t scale;
-        reinterpret_cast<uint32_t *>(codes)[at] = quantize(x, scale);
-        if (!(e0 & 8)) scales[at / 2] = (uint8_t)scale;
     }
 }
 
-// A thread has eight elements of one token, for p.per of its heads in turn
-// (keys, values, then queries; blockIdx.y is which), the next head's loaded
-// while the present one's are worked out; the angles are read once for them.
-// A warp's lanes lie side by side in a head.
+// A thread has eight elements of one token, for p.per of its heads (keys,
+// values, then queries; blockIdx.y is which), four heads' loads at a time to
+// keep memory busy; the angles are read once for them.  A warp's lanes lie
+// side by side in a head.
 template <typename T, Rotation R>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
     pdl_enter();
@@ -234,14 +239,18 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
         const int q0 = max(h0 - 2 * kv, 0), q1 = h1 - 2 * kv;
         const T *src = static_cast<const T *>(p.q) + token * p.q_stride + ((int64_t)q0 << p.dim_log2) + e0;
         T *dst = static_cast<T *>(p.q_out) + (((int64_t)token * p.q_heads + q0) << p.dim_log2) + e0;
-        Loaded<T, R> next;
-        next.load(src, turn);
-        for (int h = q0; h < q1; h++, src += p.dim, dst += p.dim) {
-            const Loaded<T, R> now = next;
-            if (h + 1 < q1) next.load(src + p.dim, turn);
-            float x[8];
-            now.turn(turn, src, e0, p.half, p.interleaved, x);
-            store8(dst, x);
+        for (int h = q0; h < q1; h += kBatch, src += kBatch * p.dim, dst += kBatch * p.dim) {
+            Loaded<T, R> l[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; b++)
+                if (h + b < q1) l[b].load(src + b * p.dim, turn);
+#pragma unroll
+            for (int b = 0; b < kBatch; b++) {
+                if (h + b >= q1) break;
+                float x[8];
+                l[b].turn(turn, src + b * p.dim, e0, p.half, p.interleaved, x);
+                store8(dst + b * p.dim, x);
+            }
         }
     }
 }
