@@ -67,8 +67,13 @@ struct AppendArgs {
 // How a call's rotation lies to a thread's eight elements: none; pairs (i,
 // i + half), the partners eight in a row as well (half a multiple of 8); pairs
 // of neighbours (interleaved, half a multiple of 4); anything else.
-constexpr int kBatch = 4;  // heads whose loads are in flight together
 enum Rotation { kNoTurn, kHalves, kNeighbours, kMixed };
+
+// Heads whose loads are in flight together: two with a load for the partners
+// (halves of 128 elements, 16383 tokens: 106 us against 118 with four), else
+// four (neighbours: 93 us, 103 with two).
+template <Rotation R>
+constexpr int kBatch = R == kHalves || R == kMixed ? 2 : 4;
 
 // The angles of elements e0 .. e0 + 7 of a head, kept for all heads of a
 // token: a rotated element becomes x * c + partner * s, each product and the
@@ -173,13 +178,13 @@ __device__ __forceinline__ void store_heads(const AppendArgs &p, const T *src, i
                                             int64_t head_step) {
     src += (int64_t)h0 << p.dim_log2;
     at += h0 * head_step;
-    for (int h = h0; h < h1; h += kBatch, src += kBatch * p.dim, at += kBatch * head_step) {
-        Loaded<T, R> l[kBatch];
+    for (int h = h0; h < h1; h += kBatch<R>, src += kBatch<R> * p.dim, at += kBatch<R> * head_step) {
+        Loaded<T, R> l[kBatch<R>];
 #pragma unroll
-        for (int b = 0; b < kBatch; b++)
+        for (int b = 0; b < kBatch<R>; b++)
             if (h + b < h1) l[b].load(src + b * p.dim, turn);
 #pragma unroll
-        for (int b = 0; b < kBatch; b++) {
+        for (int b = 0; b < kBatch<R>; b++) {
             if (h + b >= h1) break;
             float x[8];
             l[b].turn(turn, src + b * p.dim, e0, p.half, p.interleaved, x);
@@ -196,11 +201,11 @@ __device__ __forceinline__ void store_heads(const AppendArgs &p, const T *src, i
 }
 
 // A thread has eight elements of one token, for p.per of its heads (keys,
-// values, then queries; blockIdx.y is which), four heads' loads at a time to
+// values, then queries; blockIdx.y is which), the loads of several at a time to
 // keep memory busy; the angles are read once for them.  A warp's lanes lie
 // side by side in a head.
 template <typename T, Rotation R>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
+__global__ void __launch_bounds__(256, 4) append_kernel(const AppendArgs p) {
     pdl_enter();
     const int kv = p.cache.heads, heads = 2 * kv + p.q_heads, groups_log2 = p.dim_log2 - 3;
     const int i = blockIdx.x * 256 + threadIdx.x;
@@ -239,13 +244,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
         const int q0 = max(h0 - 2 * kv, 0), q1 = h1 - 2 * kv;
         const T *src = static_cast<const T *>(p.q) + token * p.q_stride + ((int64_t)q0 << p.dim_log2) + e0;
         T *dst = static_cast<T *>(p.q_out) + (((int64_t)token * p.q_heads + q0) << p.dim_log2) + e0;
-        for (int h = q0; h < q1; h += kBatch, src += kBatch * p.dim, dst += kBatch * p.dim) {
-            Loaded<T, R> l[kBatch];
+        for (int h = q0; h < q1; h += kBatch<R>, src += kBatch<R> * p.dim, dst += kBatch<R> * p.dim) {
+            Loaded<T, R> l[kBatch<R>];
 #pragma unroll
-            for (int b = 0; b < kBatch; b++)
+            for (int b = 0; b < kBatch<R>; b++)
                 if (h + b < q1) l[b].load(src + b * p.dim, turn);
 #pragma unroll
-            for (int b = 0; b < kBatch; b++) {
+            for (int b = 0; b < kBatch<R>; b++) {
                 if (h + b >= q1) break;
                 float x[8];
                 l[b].turn(turn, src + b * p.dim, e0, p.half, p.interleaved, x);
@@ -258,40 +263,54 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
 // --------------------------------------------------------------------- read
 
 // k, v [tokens][heads][D] from the cache's slots; a negative slot gives zeros.
+// A thread has eight elements of one token, for `per` of its key and value
+// heads, four heads' loads at a time.
 template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t *slots, T *k, T *v, int32_t tokens,
-                                                   int32_t dim, int32_t *status) {
+                                                   int32_t groups_log2, int32_t per, int32_t *status) {
+    constexpr int kAtATime = 4;
     pdl_enter();
-    const int groups = dim / 16, kv = c.heads * groups;
-    const int64_t total = (int64_t)tokens * 2 * kv;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int token = (int)(i / (2 * kv));
-        int rest = (int)(i - (int64_t)token * 2 * kv);
-        const bool value = rest >= kv;
-        if (value) rest -= kv;
-        const int head = rest / groups, g = rest % groups;
-        const int64_t slot = slots[token];
-        float x[16] = {};
-        if (slot >= (c.pages << c.page_log2)) {
-            if (status) atomicOr(status, TANS_B200_DATA_BAD_INDEX);
-        } else if (slot >= 0) {
-            const int64_t at =
-                token_at(c, slot >> c.page_log2, head, (int)(slot & ((1 << c.page_log2) - 1))) * groups + g;
-            const uint2 u = reinterpret_cast<const uint2 *>(value ? c.v_codes : c.k_codes)[at];
-            float s = e4m3_f32((value ? c.v_scales : c.k_scales)[at]);
-            const float *gain = value ? c.v_gain : c.k_gain;
-            if (gain) s *= gain[head];
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int token = i >> groups_log2, group = i & ((1 << groups_log2) - 1);
+    if (token >= tokens) return;
+    int64_t slot = slots[token];
+    if (slot >= (c.pages << c.page_log2)) {
+        if (status) atomicOr(status, TANS_B200_DATA_BAD_INDEX);
+        slot = -1;
+    }
+    const int64_t at0 = slot < 0 ? 0
+                                 : (token_at(c, slot >> c.page_log2, 0, (int)(slot & ((1 << c.page_log2) - 1))) << groups_log2) + group;
+    const int64_t head_step = (int64_t)1 << (c.page_log2 + groups_log2);
+    const int h1 = min(2 * c.heads, ((int)blockIdx.y + 1) * per);
+    for (int h0 = blockIdx.y * per; h0 < h1; h0 += kAtATime) {
+        uint32_t codes[kAtATime], scale[kAtATime];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t h2 = e2m1x2_f16(((j < 4 ? u.x : u.y) >> (8 * (j & 3))) & 0xFFu);
+        for (int b = 0; b < kAtATime; b++) {
+            const int h = h0 + b;
+            codes[b] = scale[b] = 0;
+            if (h >= h1 || slot < 0) continue;
+            const int64_t at = at0 + (h < c.heads ? h : h - c.heads) * head_step;
+            codes[b] = reinterpret_cast<const uint32_t *>(h < c.heads ? c.k_codes : c.v_codes)[at];
+            scale[b] = (h < c.heads ? c.k_scales : c.v_scales)[at / 2];
+        }
+#pragma unroll
+        for (int b = 0; b < kAtATime; b++) {
+            const int h = h0 + b;
+            if (h >= h1) break;
+            const bool value = h >= c.heads;
+            const int head = value ? h - c.heads : h;
+            const float *gain = value ? c.v_gain : c.k_gain;
+            const float s = e4m3_f32(scale[b]) * (gain ? gain[head] : 1.f);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t h2 = e2m1x2_f16(codes[b] >> (8 * j) & 0xFFu);
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
                 x[2 * j] = f.x * s;
                 x[2 * j + 1] = f.y * s;
             }
+            store8((value ? v : k) + ((((int64_t)token * c.heads + head) << groups_log2) + group) * 8, x);
         }
-        T *out = (value ? v : k) + ((int64_t)token * kv + rest) * 16;
-#pragma unroll
-        for (int j = 0; j < 16; j += 8) store8(out + j, reinterpret_cast<float(&)[8]>(x[j]));
     }
 }
 
@@ -1106,11 +1125,6 @@ int launch_attend(const AttendArgs &p, int max_rows, int ctas, cudaStream_t st) 
                                dim3(kJoinRows * kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
 }
 
-int flat_grid(int64_t total) {
-    const int64_t blocks = ceil_div<int64_t>(total, 256);
-    return (int)(blocks < (1 << 20) ? blocks : (1 << 20));
-}
-
 int check_cache(const char *what, const tans_b200_kv4 *c, Cache *out) {
     if (!c || !c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales)
         return fail(TANS_B200_ERR_INVALID, "%s: null cache array", what);
@@ -1174,11 +1188,11 @@ extern "C" int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, i
     int sms;
     rc = current_sms("kv4_append", &sms);
     if (rc) return rc;
-    // as many heads a thread as leave 1024 threads an SM, at most 8
+    // as many heads a thread as leave 1024 threads an SM, at most 16
     const int64_t heads = 2 * (int64_t)p.cache.heads + p.q_heads, groups = p.dim / 8;
     if (tokens * groups > INT32_MAX - 256) return fail(TANS_B200_ERR_INVALID, "kv4_append: too many tokens for one call");
     const int64_t per = tokens * groups * heads / (1024 * (int64_t)sms);
-    p.per = (int32_t)(per < 1 ? 1 : (per > 8 ? 8 : per));
+    p.per = (int32_t)(per < 1 ? 1 : (per > 16 ? 16 : per));
     p.dim_log2 = __builtin_ctz((unsigned)p.dim);
     const dim3 grid((unsigned)ceil_div<int64_t>(tokens * groups, 256), (unsigned)ceil_div<int64_t>(heads, p.per));
     if (grid.y > 65535) return fail(TANS_B200_ERR_INVALID, "kv4_append: too many heads");
@@ -1208,12 +1222,21 @@ extern "C" int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slo
     if (tokens == 0) return TANS_B200_OK;
     if (!slots || !k || !v || !is_aligned(k, 16) || !is_aligned(v, 16))
         return fail(TANS_B200_ERR_INVALID, "kv4_read: slots, and k and v 16-byte aligned, are needed");
-    const int64_t total = tokens * 2 * (int64_t)c.heads * (cache->dim / 16);
+    int sms;
+    rc = current_sms("kv4_read", &sms);
+    if (rc) return rc;
+    const int64_t heads = 2 * (int64_t)c.heads, groups = cache->dim / 8;
+    if (tokens * groups > INT32_MAX - 256) return fail(TANS_B200_ERR_INVALID, "kv4_read: too many tokens for one call");
+    // as many heads a thread as leave 1024 threads an SM, at most 8
+    const int64_t most = tokens * groups * heads / (1024 * (int64_t)sms);
+    const int32_t per = (int32_t)(most < 1 ? 1 : (most > 8 ? 8 : most));
+    const dim3 grid((unsigned)ceil_div<int64_t>(tokens * groups, 256), (unsigned)ceil_div<int64_t>(heads, per));
+    if (grid.y > 65535) return fail(TANS_B200_ERR_INVALID, "kv4_read: too many heads");
     return dispatch_float(dtype, "kv4_read", [&](auto t) {
         using T = decltype(t);
-        return launch_ex(read_kernel<T>, dim3(flat_grid(total)), dim3(256), 0, 1, (cudaStream_t)stream, "read_kernel",
-                         c, slots, static_cast<T *>(k), static_cast<T *>(v), (int32_t)tokens, (int32_t)cache->dim,
-                         status);
+        return launch_ex(read_kernel<T>, grid, dim3(256), 0, 1, (cudaStream_t)stream, "read_kernel", c, slots,
+                         static_cast<T *>(k), static_cast<T *>(v), (int32_t)tokens, (int32_t)__builtin_ctz((unsigned)groups),
+                         per, status);
     });
 }
 
