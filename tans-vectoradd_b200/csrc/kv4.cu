@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 
 constexpr int kAttnWarps = 4;
 constexpr int kUnit = 16 * kAttnWarps;  // keys
-constexpr int kStages = 4;              // 16-key blocks in a warp's ring
+constexpr int kStages = 5;              // 16-key blocks in a warp's ring: two in work, three on their way
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
@@ -502,7 +502,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     constexpr int kVS = (D + 127) / 128;   // scales of an eighth
     constexpr int kKS = D / 64;            // scales of a quarter
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int head = x.head, k1 = x.k1, lo_all = x.lo_all, hi_all = x.hi_all;
+    const int head = x.head, k1 = x.k1, lo_all = x.lo_all;
+    const int kend = min(x.hi_all, k1 - 1);  // the piece's last key
     const uint8_t *ring = smem + warp * (kStages * L::kBlock);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
 
@@ -519,60 +520,61 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
     const uint32_t k_dst = ring_sa + lane / (D / 32) * (D / 2) + 16 * L::k_chunk(lane / (D / 32), c16);
     const uint32_t v_dst = ring_sa + L::kCodes + lane / (D / 32) * (D / 2) + 16 * L::v_chunk(lane / (D / 32), c16);
-    // blocks within one page whose keys all exist: first .. first + span
+    // blocks within one page whose keys all belong to the piece: first .. first + span
     const bool whole_pages = page_log2 >= 4;
-    const int easy = lo_all, easy_span = whole_pages ? hi_all - 15 - lo_all : -1;
+    const int easy_span = whole_pages ? kend - 15 - lo_all : -1;
     // the page of key base + r16, or with whole pages of the block, loaded ahead of its use
     const auto page_of = [&](int base) -> int {
-        return base < k1 ? table[max(lo_all, min(whole_pages ? base : base + r16, hi_all)) >> page_log2] : 0;
+        return base <= kend ? table[max(lo_all, min(whole_pages ? base : base + r16, kend)) >> page_log2] : 0;
     };
-    // start the copies of the block at `base`, its keys' pages in `page`, `at` bytes into the ring
+    // start the copies of the block at `base`, its keys' pages in `page`, `at`
+    // bytes into the ring; keys past the piece become zeros
     const auto fetch = [&](int base, int page, uint32_t at) {
-        if (base < k1) {
-            if ((uint32_t)page >= (uint32_t)p.cache.pages) {
-                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-                page = 0;
-            }
-            const uint32_t s_dst = ring_sa + 2 * L::kCodes + lane * (D / 16) + at;
-            if (base >= easy && base - easy <= easy_span) {
-                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(base & in_page);
+        if ((uint32_t)page >= (uint32_t)p.cache.pages) {
+            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+            page = 0;
+        }
+        const uint32_t s_dst = ring_sa + 2 * L::kCodes + lane * (D / 16) + at;
+        if (base >= lo_all && base - lo_all <= easy_span) {
+            const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(base & in_page);
 #pragma unroll
-                for (int i = 0; i < D / 64; i++) {
-                    copy_async<16>(k_dst + at + 512 * i, k_src + tok * (D / 2) + 512 * i, true);
-                    copy_async<16>(L::kSameChunks ? v_dst + at + 512 * i
-                                                  : ring_sa + at + L::kCodes + (lane + 32 * i) / (D / 32) * (D / 2) +
-                                                        16 * L::v_chunk((lane + 32 * i) / (D / 32), c16),
-                                   v_src + tok * (D / 2) + 512 * i, true);
-                }
-                copy_async<D / 16>(s_dst, s_src + tok * (D / 16), true);
-            } else {
-#pragma unroll 1
-                for (int i = 0; i < D / 64; i++) {
-                    const int r = (lane + 32 * i) / (D / 32), key = base + r;
-                    const bool real = key >= lo_all && key <= hi_all;
-                    const uint32_t pg = (uint32_t)__shfl_sync(0xffffffffu, page, r);
-                    const uint64_t tok = head_at + (uint64_t)pg * page_tokens + (uint32_t)(key & in_page);
-                    const uint64_t off = real ? tok * (D / 2) + 16 * c16 : 0;
-                    copy_async<16>(ring_sa + at + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
-                    copy_async<16>(ring_sa + at + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16),
-                                   p.cache.v_codes + off, real);
-                }
-                const int key = base + r16;
-                const bool real = key >= lo_all && key <= hi_all;
-                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(key & in_page);
-                // s_src stands r16 tokens into the head's first page
-                copy_async<D / 16>(s_dst, s_src + (real ? (int64_t)(tok - r16) * (D / 16) : 0), real);
+            for (int i = 0; i < D / 64; i++) {
+                copy_async<16>(k_dst + at + 512 * i, k_src + tok * (D / 2) + 512 * i, true);
+                copy_async<16>(L::kSameChunks ? v_dst + at + 512 * i
+                                              : ring_sa + at + L::kCodes + (lane + 32 * i) / (D / 32) * (D / 2) +
+                                                    16 * L::v_chunk((lane + 32 * i) / (D / 32), c16),
+                               v_src + tok * (D / 2) + 512 * i, true);
             }
+            copy_async<D / 16>(s_dst, s_src + tok * (D / 16), true);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < D / 64; i++) {
+                const int r = (lane + 32 * i) / (D / 32), key = base + r;
+                const bool real = key >= lo_all && key <= kend;
+                const uint32_t pg = (uint32_t)__shfl_sync(0xffffffffu, page, r);
+                const uint64_t tok = head_at + (uint64_t)pg * page_tokens + (uint32_t)(key & in_page);
+                const uint64_t off = real ? tok * (D / 2) + 16 * c16 : 0;
+                copy_async<16>(ring_sa + at + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
+                copy_async<16>(ring_sa + at + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), p.cache.v_codes + off, real);
+            }
+            const int key = base + r16;
+            const bool real = key >= lo_all && key <= kend;
+            const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(key & in_page);
+            // s_src stands r16 tokens into the head's first page
+            copy_async<D / 16>(s_dst, s_src + (real ? (int64_t)(tok - r16) * (D / 16) : 0), real);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int base = x.k0 + 16 * warp;
-    int page = page_of(base);
+    int page[2] = {page_of(base), page_of(base + kUnit)};
+    if (base < k1) {
 #pragma unroll 1
-    for (int i = 0; i < kStages - 1; i++) {
-        const int now = page;
-        page = page_of(base + (i + 1) * kUnit);
-        fetch(base + i * kUnit, now, i * L::kBlock);
+        for (int i = 0; i < kStages; i++) {
+            const int now = page[0];
+            page[0] = page[1];
+            page[1] = page_of(base + (i + 2) * kUnit);
+            fetch(base + i * kUnit, now, i * L::kBlock);
+        }
     }
 
     // ---- Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
@@ -621,35 +623,33 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         }
     }
     __syncthreads();
-    const int inner = x.lo_in, inner_span = x.hi_in - 15 - x.lo_in;  // blocks that every row sees whole
+    // pairs of blocks that every row sees whole
+    const int inner = x.lo_in, inner_span = min(x.hi_in, kend) - 15 - kUnit - x.lo_in;
 
     float o[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     // scores up to this need no new maximum; what is subtracted; the sums
     float limit[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-    uint32_t at = 0;  // the block's place in the ring, in bytes
+    uint32_t at = 0;  // the first block's place in the ring, in bytes
 #pragma unroll 1
-    for (; base < k1; base += kUnit) {
+    for (; base < k1; base += 2 * kUnit) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
-        {
-            const int now = page;
-            page = page_of(base + kStages * kUnit);
-            fetch(base + (kStages - 1) * kUnit, now, at == 0 ? (kStages - 1) * L::kBlock : at - L::kBlock);
-        }
-        const uint8_t *blk = ring + at;
-        at = at == (kStages - 1) * L::kBlock ? 0 : at + L::kBlock;
+        // the blocks at base and base + kUnit, their places in the ring, the place after them
+        const uint32_t at1 = at == (kStages - 1) * L::kBlock ? 0 : at + L::kBlock;
+        const uint32_t after = at1 == (kStages - 1) * L::kBlock ? 0 : at1 + L::kBlock;
+        const uint8_t *blk[2] = {ring + at, ring + at1};
         // Column n of an 8-key half is key n ^ (n >> 1 & 1): the V reads of
         // lanes t = 0..3 then fall on rows of both parities.
-        // ---- scores of 16 keys
-        float s[2][4] = {};
+        // ---- scores of 2 x 16 keys; half h is half h % 2 of block h / 2
+        float s[4][4] = {};
         {
-            uint32_t w[2][D / 32], f[2][kKS];
+            uint32_t w[4][D / 32], f[4][kKS];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int r = 8 * h + (g ^ (g >> 1 & 1));
-                const uint8_t *kp = blk + r * (D / 2);
+            for (int h = 0; h < 4; h++) {
+                const int r = 8 * (h & 1) + (g ^ (g >> 1 & 1));
+                const uint8_t *kp = blk[h / 2] + r * (D / 2);
                 if constexpr (D == 64) {
                     const uint2 v = *reinterpret_cast<const uint2 *>(kp + 8 * t);
                     w[h][0] = v.x, w[h][1] = v.y;
@@ -660,7 +660,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                         w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
                     }
                 }
-                const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
+                const uint8_t *sp = blk[h / 2] + 2 * L::kCodes + r * (D / 16) + t * kKS;
                 if constexpr (kKS == 1) {
                     f[h][0] = e4m3x2_h2(*sp * 0x101u);
                 } else {
@@ -676,7 +676,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
             for (int j = 0; j < kSteps; j += 2) {
                 const uint4 qa = qs[j * 32 + lane], qb = qs[(j + 1) * 32 + lane];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < 4; h++) {
                     uint32_t b[4];
                     e2m1x8_h2(w[h][j / 2], b);
 #pragma unroll
@@ -691,18 +691,24 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int hi = x.hi[g + 8 * i], lo = first_seen(p, hi);
+                const int last = x.hi[g + 8 * i], lo = first_seen(p, last), hi = min(last, kend);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int key = base + 8 * (c >> 1) + ((2 * t + (c & 1)) ^ (t & 1));
-                    if (key < lo || key > hi) s[c >> 1][2 * i + (c & 1)] = -INFINITY;
-                }
+                for (int h = 0; h < 4; h++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int key = base + kUnit * (h >> 1) + 8 * (h & 1) + ((2 * t + c) ^ (t & 1));
+                        if (key < lo || key > hi) s[h][2 * i + c] = -INFINITY;
+                    }
             }
         }
         float m[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            m[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1])) * to_log2[i];
+        for (int i = 0; i < 2; i++) {
+            m[i] = s[0][2 * i];
+#pragma unroll
+            for (int k = 1; k < 8; k++) m[i] = fmaxf(m[i], s[k / 2][2 * i + (k & 1)]);
+            m[i] *= to_log2[i];
+        }
         if (__any_sync(0xffffffffu, m[0] > limit[0] || m[1] > limit[1])) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -721,97 +727,112 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                 }
             }
         }
+        uint4 pf[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int h = 0; h < 4; h++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 s[h][c] = exp2_fast(__fmaf_rn(s[h][c], to_log2[c >> 1], -less[c >> 1]));
                 sum[c >> 1] += s[h][c];
             }
-        const uint4 pf = make_uint4(h2_of(s[0][0], s[0][1]), h2_of(s[0][2], s[0][3]), h2_of(s[1][0], s[1][1]),
-                                    h2_of(s[1][2], s[1][3]));
-        // ---- values of the lane's four keys
-        uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int r = 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-            const uint8_t *vp = blk + L::kCodes + r * (D / 2);
-            if constexpr (D == 64) {
-                w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
-            } else if constexpr (D == 128) {
-                const uint2 v = *reinterpret_cast<const uint2 *>(vp + 16 * L::v_chunk(r, g >> 1) + 8 * (g & 1));
-                w[k][0] = v.x, w[k][1] = v.y;
-            } else {
-                const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * L::v_chunk(r, g));
-                w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
-            }
+        for (int b = 0; b < 2; b++)
+            pf[b] = make_uint4(h2_of(s[2 * b][0], s[2 * b][1]), h2_of(s[2 * b][2], s[2 * b][3]),
+                               h2_of(s[2 * b + 1][0], s[2 * b + 1][1]), h2_of(s[2 * b + 1][2], s[2 * b + 1][3]));
+        // ---- values of the lane's four keys of each block
 #pragma unroll
-            for (int i = 0; i < kVS; i++)
-                sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
-        }
-        // A NaN scale on a key that only some rows see must not reach the
-        // others as 0 * NaN: its values count as 0 here and are added below.
-        uint32_t nan_keys = 0;
-        if (edge) {
+        for (int y = 0; y < 2; y++) {
+            uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 4; k++) {
+                const int r = 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                const uint8_t *vp = blk[y] + L::kCodes + r * (D / 2);
+                if constexpr (D == 64) {
+                    w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
+                } else if constexpr (D == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + 16 * L::v_chunk(r, g >> 1) + 8 * (g & 1));
+                    w[k][0] = v.x, w[k][1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * L::v_chunk(r, g));
+                    w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+                }
 #pragma unroll
                 for (int i = 0; i < kVS; i++)
-                    if ((sc[k][i] & 0x7Fu) == 0x7Fu) {
-                        nan_keys |= 1u << (k * kVS + i);
-                        sc[k][i] = 0;
-                    }
-        }
-#pragma unroll
-        for (int i = 0; i < kVS; i++) {
-            const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
-            constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
-#pragma unroll
-            for (int j = 0; j < kPer; j += 8) {
-                const int word = (i * 16 + j) / 8;
-                uint32_t even[2][4], odd[2][4];
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
-                    e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
-                    e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    mma_f16(o[i * 16 + j + 2 * e], pf, mul_h2(even[0][e], f[0]), mul_h2(even[1][e], f[1]));
-                    mma_f16(o[i * 16 + j + 2 * e + 1], pf, mul_h2(odd[0][e], f[0]), mul_h2(odd[1][e], f[1]));
-                }
+                    sc[k][i] = blk[y][2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
             }
-        }
-        if (edge && __any_sync(0xffffffffu, nan_keys)) {
-            uint32_t seen[4];
+            // A NaN scale on a key that only some rows see must not reach the
+            // others as 0 * NaN: its values count as 0 here and are added below.
+            uint32_t nan_keys = 0;
+            if (edge) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int hi = x.hi[g + 8 * i], lo = first_seen(p, hi);
+                for (int k = 0; k < 4; k++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int a = base + 8 * h + ((2 * t) ^ (t & 1)), b = base + 8 * h + ((2 * t + 1) ^ (t & 1));
-                    seen[2 * h + i] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
-                }
+                    for (int i = 0; i < kVS; i++)
+                        if ((sc[k][i] & 0x7Fu) == 0x7Fu) {
+                            nan_keys |= 1u << (k * kVS + i);
+                            sc[k][i] = 0;
+                        }
             }
 #pragma unroll
             for (int i = 0; i < kVS; i++) {
-                uint32_t b[2];
+                const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
+                constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-                    b[x] = h2_of(nan_keys >> (2 * x * kVS + i) & 1 ? 1.f : 0.f,
-                                 nan_keys >> ((2 * x + 1) * kVS + i) & 1 ? 1.f : 0.f);
-                float n[4] = {};
-                mma_f16(n, make_uint4(seen[0], seen[1], seen[2], seen[3]), b[0], b[1]);
-                constexpr int kPer = kE < 16 ? kE : 16;
+                for (int j = 0; j < kPer; j += 8) {
+                    const int word = (i * 16 + j) / 8;
+                    uint32_t even[2][4], odd[2][4];
 #pragma unroll
-                for (int j = 0; j < kPer; j++)
+                    for (int b = 0; b < 2; b++) {
+                        const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
+                        e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
+                        e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
+                    }
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if (n[c] > 0.f) o[i * 16 + j][c] = NAN;
+                    for (int e = 0; e < 4; e++) {
+                        mma_f16(o[i * 16 + j + 2 * e], pf[y], mul_h2(even[0][e], f[0]), mul_h2(even[1][e], f[1]));
+                        mma_f16(o[i * 16 + j + 2 * e + 1], pf[y], mul_h2(odd[0][e], f[0]), mul_h2(odd[1][e], f[1]));
+                    }
+                }
+            }
+            if (edge && __any_sync(0xffffffffu, nan_keys)) {
+                uint32_t seen[4];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int last = x.hi[g + 8 * i], lo = first_seen(p, last), hi = min(last, kend);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int a = base + kUnit * y + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
+                        seen[2 * h + i] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kVS; i++) {
+                    uint32_t b[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        b[k] = h2_of(nan_keys >> (2 * k * kVS + i) & 1 ? 1.f : 0.f,
+                                     nan_keys >> ((2 * k + 1) * kVS + i) & 1 ? 1.f : 0.f);
+                    float n[4] = {};
+                    mma_f16(n, make_uint4(seen[0], seen[1], seen[2], seen[3]), b[0], b[1]);
+                    constexpr int kPer = kE < 16 ? kE : 16;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            if (n[c] > 0.f) o[i * 16 + j][c] = NAN;
+                }
             }
         }
-        __syncwarp();  // the block is read before its place in the ring is filled again
+        // ---- the next copies into the two places just read
+        __syncwarp();
+        {
+            const int now[2] = {page[0], page[1]};
+            page[0] = page_of(base + (kStages + 2) * kUnit);
+            page[1] = page_of(base + (kStages + 3) * kUnit);
+            fetch(base + kStages * kUnit, now[0], at);
+            fetch(base + (kStages + 1) * kUnit, now[1], at1);
+        }
+        at = after;
     }
 
     // ---- the warps' results, side by side
