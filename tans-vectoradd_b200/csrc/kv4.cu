@@ -322,11 +322,12 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 // The rows of one KV head are its new tokens times the query heads that share
 // it (row = token * group + head in group); 16 of them are the M of an
 // m16n8k16 MMA and make a tile.  The keys of a (sequence, head, tile) are cut
-// into units of 64, 16 for each of a CTA's four warps, which keep a running
+// into units of 128, 32 for each of a CTA's four warps, which keep a running
 // maximum and sum each and join at the end.
 //
-// Codes go from shared memory (a ring of asynchronous copies per warp) to MMA
-// operands in registers:
+// A block's codes and scales lie together in its page, so four bulk copies
+// bring it (eight with pages of 16), the next block's while one is worked on.
+// From shared memory they go to MMA operands in registers:
 //  * S = Q K^T: the contraction runs over D in any order, so lane (g, t) takes
 //    one key of each 8-key half and the t-th quarter of its D codes, D/8
 //    contiguous bytes; step j uses codes 4j .. 4j+3 of that quarter, and
@@ -340,8 +341,9 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 // element loses bits only below 2^-28 of that.
 
 constexpr int kAttnWarps = 4;
-constexpr int kUnit = 16 * kAttnWarps;  // keys
-constexpr int kStages = 5;              // 16-key blocks in a warp's ring: two in work, three on their way
+constexpr int kBlockKeys = 32;                  // keys a warp takes at a time
+constexpr int kUnit = kBlockKeys * kAttnWarps;  // keys
+constexpr int kStages = 2;                      // blocks in a warp's ring: one in work, one on its way
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
@@ -392,14 +394,27 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs &p, int seq) {
     return s;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t *src, bool real) {
-    const int n = real ? BYTES : 0;  // what is not read is filled with zeros
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
-                     : "memory");
+// Bulk copy of `bytes` (a multiple of 16, both ends aligned) into shared memory, counted on `bar`.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const uint8_t *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Waits for the phase of `bar` with the given parity.  Bounded: copies that do
+// not land within about a second set TANS_B200_DATA_TIMEOUT.
+__device__ __forceinline__ void wait_copies(uint32_t bar, uint32_t parity, int32_t *status) {
+    for (uint32_t i = 0; i < 1u << 16; i++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, 10000;\n\t"
+            "selp.b32 %0, 1, 0, P1;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return;
+    }
+    if (status) atomicOr(status, TANS_B200_DATA_TIMEOUT);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
@@ -443,7 +458,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 template <int D>
 struct AttnLayout {
-    static constexpr int kCodes = 16 * D / 2, kScales = 16 * D / 16;       // bytes of a 16-key block
+    static constexpr int kCodes = kBlockKeys * D / 2, kScales = kBlockKeys * D / 16;  // bytes of a block
     static constexpr int kBlock = 2 * (kCodes + kScales);                  // K codes, V codes, K scales, V scales
     static constexpr int kRing = kAttnWarps * kStages * kBlock;
     static constexpr int kRow = D + 8;                                     // floats of a row of O: no bank conflicts
@@ -452,11 +467,6 @@ struct AttnLayout {
     static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ;
     static constexpr int kCtas = D == 256 ? 2 : 4;                         // resident on an SM
     static constexpr int kPart = 16 * (D + 2);                             // floats of a partial result
-    // 16-byte chunk c of row r of a block's codes lies in chunk k_chunk(r, c) of
-    // that row (V: v_chunk), so that the lanes of a read meet different banks
-    static __device__ int k_chunk(int r, int c) { return D == 256 ? c ^ (r & 1) : c; }
-    static __device__ int v_chunk(int r, int c) { return D == 256 ? c ^ (r & 6) : (D == 128 ? c ^ (r >> 1 & 2) : c); }
-    static constexpr bool kSameChunks = D != 256;  // v_chunk of rows 512 bytes apart is the same
     // place of element e in a merged row: the order of the MMA's columns
     static __device__ int place(int e) { return e % (D / 8) * 8 + e / (D / 8); }
 };
@@ -491,10 +501,12 @@ __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
     }
 }
 
-// Runs a piece (set by the caller, before a block barrier): afterwards the four
+// Runs a piece (set by the caller, before a block barrier).  s_bars: the rings'
+// barriers, whose parities this warp keeps in `phases`.  Afterwards the four
 // warps' results lie in `smem` as [warp][16][kRow] O, [warp][16] maxima and sums.
 template <typename T, int D>
-__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem) {
+__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem, uint64_t *s_bars,
+                                             uint32_t &phases) {
     using L = AttnLayout<D>;
     constexpr int kSteps = D / 16;         // MMA steps of S
     constexpr int kTiles = D / 8;          // MMA column tiles of O
@@ -504,77 +516,84 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int head = x.head, k1 = x.k1, lo_all = x.lo_all;
     const int kend = min(x.hi_all, k1 - 1);  // the piece's last key
-    const uint8_t *ring = smem + warp * (kStages * L::kBlock);
+    uint8_t *ring = smem + warp * (kStages * L::kBlock);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
 
-    // ---- copies of 16-key blocks into the warp's ring
+    // ---- copies of the warp's blocks into its ring
     const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
     const int32_t *table = p.table + (int64_t)x.seq * p.table_stride;
-    const int c16 = lane % (D / 32);                                // this lane's 16-byte chunk of a token's codes
-    const int r16 = lane & 15;                                      // the token whose scales it copies
     const int64_t head_at = (int64_t)head << page_log2;
-    const uint8_t *k_src = p.cache.k_codes + head_at * (D / 2) + 16 * lane;
-    const uint8_t *v_src = p.cache.v_codes + head_at * (D / 2) + 16 * lane;
-    const uint8_t *s_src = (lane < 16 ? p.cache.k_scales : p.cache.v_scales) + (head_at + r16) * (D / 16);
     const uint32_t page_tokens = (uint32_t)p.cache.heads << page_log2;
     const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
-    const uint32_t k_dst = ring_sa + lane / (D / 32) * (D / 2) + 16 * L::k_chunk(lane / (D / 32), c16);
-    const uint32_t v_dst = ring_sa + L::kCodes + lane / (D / 32) * (D / 2) + 16 * L::v_chunk(lane / (D / 32), c16);
-    // blocks within one page whose keys all belong to the piece: first .. first + span
-    const bool whole_pages = page_log2 >= 4;
-    const int easy_span = whole_pages ? kend - 15 - lo_all : -1;
-    // the page of key base + r16, or with whole pages of the block, loaded ahead of its use
-    const auto page_of = [&](int base) -> int {
-        return base <= kend ? table[max(lo_all, min(whole_pages ? base : base + r16, kend)) >> page_log2] : 0;
-    };
-    // start the copies of the block at `base`, its keys' pages in `page`, `at`
-    // bytes into the ring; keys past the piece become zeros
-    const auto fetch = [&](int base, int page, uint32_t at) {
+    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(s_bars) + 8u * kStages * warp;
+    // Pages of 16 and more: lanes 0..3 copy K codes, V codes, K scales and V
+    // scales of the block (of its first 16 keys, and lanes 4..7 of the others,
+    // where a page holds 16).
+    const int sets = page_log2 == 4 ? 2 : 1;
+    const bool codes = !(lane & 2), copies = page_log2 >= 4 && lane < 4 * sets;
+    const int set_key = lane >> 2 << 4;  // the first key of a lane's copy in the block
+    const uint32_t row_bytes = codes ? D / 2 : D / 16, copy_bytes = row_bytes * kBlockKeys / sets;
+    const uint8_t *src = (codes ? (lane & 1 ? p.cache.v_codes : p.cache.k_codes)
+                                : (lane & 1 ? p.cache.v_scales : p.cache.k_scales)) + head_at * row_bytes;
+    const uint32_t dst = ring_sa + (codes ? (lane & 1) * L::kCodes : 2 * L::kCodes + (lane & 1) * L::kScales) +
+                         set_key * row_bytes;
+    const auto page_at = [&](int key) {  // of a key within the piece
+        int page = table[key >> page_log2];
         if ((uint32_t)page >= (uint32_t)p.cache.pages) {
             if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
             page = 0;
         }
-        const uint32_t s_dst = ring_sa + 2 * L::kCodes + lane * (D / 16) + at;
-        if (base >= lo_all && base - lo_all <= easy_span) {
-            const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(base & in_page);
-#pragma unroll
-            for (int i = 0; i < D / 64; i++) {
-                copy_async<16>(k_dst + at + 512 * i, k_src + tok * (D / 2) + 512 * i, true);
-                copy_async<16>(L::kSameChunks ? v_dst + at + 512 * i
-                                              : ring_sa + at + L::kCodes + (lane + 32 * i) / (D / 32) * (D / 2) +
-                                                    16 * L::v_chunk((lane + 32 * i) / (D / 32), c16),
-                               v_src + tok * (D / 2) + 512 * i, true);
-            }
-            copy_async<D / 16>(s_dst, s_src + tok * (D / 16), true);
-        } else {
-#pragma unroll 1
-            for (int i = 0; i < D / 64; i++) {
-                const int r = (lane + 32 * i) / (D / 32), key = base + r;
-                const bool real = key >= lo_all && key <= kend;
-                const uint32_t pg = (uint32_t)__shfl_sync(0xffffffffu, page, r);
-                const uint64_t tok = head_at + (uint64_t)pg * page_tokens + (uint32_t)(key & in_page);
-                const uint64_t off = real ? tok * (D / 2) + 16 * c16 : 0;
-                copy_async<16>(ring_sa + at + r * (D / 2) + 16 * L::k_chunk(r, c16), p.cache.k_codes + off, real);
-                copy_async<16>(ring_sa + at + L::kCodes + r * (D / 2) + 16 * L::v_chunk(r, c16), p.cache.v_codes + off, real);
-            }
-            const int key = base + r16;
-            const bool real = key >= lo_all && key <= kend;
-            const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)(key & in_page);
-            // s_src stands r16 tokens into the head's first page
-            copy_async<D / 16>(s_dst, s_src + (real ? (int64_t)(tok - r16) * (D / 16) : 0), real);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        return (uint32_t)page;
     };
-    int base = x.k0 + 16 * warp;
-    int page[2] = {page_of(base), page_of(base + kUnit)};
-    if (base < k1) {
+    // this lane's page of the block at `base`, asked for a block ahead of its use
+    const auto page_of = [&](int base) -> int {
+        return copies && base < k1 ? table[max(lo_all, min(base + set_key, kend)) >> page_log2] : 0;
+    };
+    const auto fetch = [&](int base, int page, int stage) {
+        if (base >= k1) return;
+        const uint32_t bar = bars + 8u * stage;
+        if (page_log2 >= 4) {
+            if (lane == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(L::kBlock) : "memory");
+            if (copies) {
+                if ((uint32_t)page >= (uint32_t)p.cache.pages) {
+                    if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+                    page = 0;
+                }
+                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)((base + set_key) & in_page);
+                copy_bulk(dst + stage * L::kBlock, src + tok * row_bytes, copy_bytes, bar);
+            }
+        } else {  // smaller pages: a lane brings one key itself
+            const int key = base + lane;
+            const bool real = key >= lo_all && key <= kend;
+            const int64_t tok = real ? head_at + (int64_t)page_at(key) * page_tokens + (key & in_page) : 0;
+            uint8_t *at = ring + stage * L::kBlock;
 #pragma unroll 1
-        for (int i = 0; i < kStages; i++) {
-            const int now = page[0];
-            page[0] = page[1];
-            page[1] = page_of(base + (i + 2) * kUnit);
-            fetch(base + i * kUnit, now, i * L::kBlock);
+            for (int i = 0; i < D / 32; i++) {
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(at + lane * (D / 2) + 16 * i) =
+                    real ? *reinterpret_cast<const uint4 *>(p.cache.k_codes + tok * (D / 2) + 16 * i) : zero;
+                *reinterpret_cast<uint4 *>(at + L::kCodes + lane * (D / 2) + 16 * i) =
+                    real ? *reinterpret_cast<const uint4 *>(p.cache.v_codes + tok * (D / 2) + 16 * i) : zero;
+            }
+#pragma unroll 1
+            for (int i = 0; i < D / 64; i++) {
+                uint32_t *ks = reinterpret_cast<uint32_t *>(at + 2 * L::kCodes + lane * (D / 16) + 4 * i);
+                ks[0] = real ? *reinterpret_cast<const uint32_t *>(p.cache.k_scales + tok * (D / 16) + 4 * i) : 0u;
+                ks[L::kScales / 4] = real ? *reinterpret_cast<const uint32_t *>(p.cache.v_scales + tok * (D / 16) + 4 * i) : 0u;
+            }
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
         }
+    };
+    // what was written here by ordinary stores comes before the copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    int base = x.k0 + kBlockKeys * warp;
+    int page = page_of(base);
+    {
+        const int now = page;
+        page = page_of(base + kUnit);
+        fetch(base, now, 0);
     }
 
     // ---- Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
@@ -623,44 +642,47 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         }
     }
     __syncthreads();
-    // pairs of blocks that every row sees whole
-    const int inner = x.lo_in, inner_span = min(x.hi_in, kend) - 15 - kUnit - x.lo_in;
+    // blocks that every row sees whole
+    const int inner = x.lo_in, inner_span = min(x.hi_in, kend) - (kBlockKeys - 1) - x.lo_in;
 
     float o[kTiles][4];
 #pragma unroll
     for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     // scores up to this need no new maximum; what is subtracted; the sums
     float limit[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
-    uint32_t at = 0;  // the first block's place in the ring, in bytes
+    int stage = 0;
 #pragma unroll 1
-    for (; base < k1; base += 2 * kUnit) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        __syncwarp();
-        // the blocks at base and base + kUnit, their places in the ring, the place after them
-        const uint32_t at1 = at == (kStages - 1) * L::kBlock ? 0 : at + L::kBlock;
-        const uint32_t after = at1 == (kStages - 1) * L::kBlock ? 0 : at1 + L::kBlock;
-        const uint8_t *blk[2] = {ring + at, ring + at1};
+    for (; base < k1; base += kUnit) {
+        {  // the next block into the other place
+            const int now = page;
+            page = page_of(base + 2 * kUnit);
+            fetch(base + kUnit, now, stage ^ 1);
+        }
+        wait_copies(bars + 8u * stage, phases >> stage & 1, p.status);
+        phases ^= 1u << stage;
+        const uint8_t *blk = ring + stage * L::kBlock;
+        stage ^= 1;
         // Column n of an 8-key half is key n ^ (n >> 1 & 1): the V reads of
         // lanes t = 0..3 then fall on rows of both parities.
-        // ---- scores of 2 x 16 keys; half h is half h % 2 of block h / 2
+        // ---- scores of 32 keys, eight at a time
         float s[4][4] = {};
         {
             uint32_t w[4][D / 32], f[4][kKS];
 #pragma unroll
             for (int h = 0; h < 4; h++) {
-                const int r = 8 * (h & 1) + (g ^ (g >> 1 & 1));
-                const uint8_t *kp = blk[h / 2] + r * (D / 2);
+                const int r = 8 * h + (g ^ (g >> 1 & 1));
+                const uint8_t *kp = blk + r * (D / 2);
                 if constexpr (D == 64) {
                     const uint2 v = *reinterpret_cast<const uint2 *>(kp + 8 * t);
                     w[h][0] = v.x, w[h][1] = v.y;
                 } else {
 #pragma unroll
                     for (int i = 0; i < D / 128; i++) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(kp + 16 * L::k_chunk(r, t * (D / 128) + i));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(kp + t * (D / 8) + 16 * i);
                         w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
                     }
                 }
-                const uint8_t *sp = blk[h / 2] + 2 * L::kCodes + r * (D / 16) + t * kKS;
+                const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
                 if constexpr (kKS == 1) {
                     f[h][0] = e4m3x2_h2(*sp * 0x101u);
                 } else {
@@ -696,7 +718,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                 for (int h = 0; h < 4; h++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const int key = base + kUnit * (h >> 1) + 8 * (h & 1) + ((2 * t + c) ^ (t & 1));
+                        const int key = base + 8 * h + ((2 * t + c) ^ (t & 1));
                         if (key < lo || key > hi) s[h][2 * i + c] = -INFINITY;
                     }
             }
@@ -739,39 +761,43 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         for (int b = 0; b < 2; b++)
             pf[b] = make_uint4(h2_of(s[2 * b][0], s[2 * b][1]), h2_of(s[2 * b][2], s[2 * b][3]),
                                h2_of(s[2 * b + 1][0], s[2 * b + 1][1]), h2_of(s[2 * b + 1][2], s[2 * b + 1][3]));
-        // ---- values of the lane's four keys of each block
+        // ---- values of the lane's four keys of each 16
 #pragma unroll
         for (int y = 0; y < 2; y++) {
             uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int r = 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-                const uint8_t *vp = blk[y] + L::kCodes + r * (D / 2);
+                const int r = 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                const uint8_t *vp = blk + L::kCodes + r * (D / 2);
                 if constexpr (D == 64) {
                     w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
                 } else if constexpr (D == 128) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + 16 * L::v_chunk(r, g >> 1) + 8 * (g & 1));
+                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + 8 * g);
                     w[k][0] = v.x, w[k][1] = v.y;
                 } else {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * L::v_chunk(r, g));
+                    const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
                     w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
                 }
 #pragma unroll
                 for (int i = 0; i < kVS; i++)
-                    sc[k][i] = blk[y][2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
+                    sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
             }
-            // A NaN scale on a key that only some rows see must not reach the
-            // others as 0 * NaN: its values count as 0 here and are added below.
+            // Keys outside the piece hold anything: their values count as 0.  A NaN
+            // scale on a key that only some rows see must not reach the others
+            // as 0 * NaN: its values count as 0 here and are added below.
             uint32_t nan_keys = 0;
             if (edge) {
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int k = 0; k < 4; k++) {
+                    const int key = base + 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                    const bool real = key >= lo_all && key <= kend;
 #pragma unroll
-                    for (int i = 0; i < kVS; i++)
-                        if ((sc[k][i] & 0x7Fu) == 0x7Fu) {
-                            nan_keys |= 1u << (k * kVS + i);
-                            sc[k][i] = 0;
-                        }
+                    for (int i = 0; i < kVS; i++) {
+                        const bool nan = (sc[k][i] & 0x7Fu) == 0x7Fu;
+                        if (nan && real) nan_keys |= 1u << (k * kVS + i);
+                        if (nan || !real) sc[k][i] = 0;
+                    }
+                }
             }
 #pragma unroll
             for (int i = 0; i < kVS; i++) {
@@ -801,7 +827,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                     const int last = x.hi[g + 8 * i], lo = first_seen(p, last), hi = min(last, kend);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const int a = base + kUnit * y + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
+                        const int a = base + 16 * y + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
                         seen[2 * h + i] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
                     }
                 }
@@ -823,20 +849,10 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                 }
             }
         }
-        // ---- the next copies into the two places just read
-        __syncwarp();
-        {
-            const int now[2] = {page[0], page[1]};
-            page[0] = page_of(base + (kStages + 2) * kUnit);
-            page[1] = page_of(base + (kStages + 3) * kUnit);
-            fetch(base + kStages * kUnit, now[0], at);
-            fetch(base + (kStages + 1) * kUnit, now[1], at1);
-        }
-        at = after;
+        __syncwarp();  // all lanes have read the block before its place is filled again
     }
 
     // ---- the warps' results, side by side
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float *merge = reinterpret_cast<float *>(smem);
     float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
@@ -915,12 +931,22 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, 
     }
 }
 
+// Called by all threads, before a block barrier.
+__device__ __forceinline__ void init_bars(uint64_t *bars) {
+    if (threadIdx.x < kAttnWarps * kStages)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(bars + threadIdx.x)));
+    asm volatile("fence.mbarrier_init.release.cluster;");
+}
+
 // One CTA a (tile, head, sequence), over all its keys.
 template <typename T, int D>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
     __shared__ Piece x;
+    __shared__ __align__(8) uint64_t bars[kAttnWarps * kStages];
+    uint32_t phases = 0;
+    init_bars(bars);
     const Sequence q = sequence(p, blockIdx.z);
     if ((int)blockIdx.x * 16 >= q.news * p.group) return;
     if (threadIdx.x < 32) {
@@ -934,16 +960,18 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
         set_rows(p, x);
     }
     __syncthreads();
-    attend_piece<T, D>(p, x, smem);
+    attend_piece<T, D>(p, x, smem, bars, phases);
     join_warps<T, D>(p, x, smem, nullptr);
 }
 
 // Split form: the units of all tiles in a row (sequence, head, tile, unit),
-// cut into equal stretches, one a CTA, whatever the sequences' lengths.  A
-// CTA's first tile may have begun in an earlier one (part 0 of its
+// with kTileCost idle ones before each tile for what a tile costs besides its
+// keys, cut into equal stretches, one a CTA, whatever the sequences' lengths.
+// A CTA's first tile may have begun in an earlier one (part 0 of its
 // workspace), its last may go on in the next (part 1); those are joined by
 // attend_join_kernel, whose CTA c takes the tile that begins in stretch c
 // and does not end there, as `head` describes it.
+constexpr int kTileCost = 1;
 struct SplitHead {
     int32_t pieces;  // 0: none
     int32_t seq, head, row0, rows, first;
@@ -962,6 +990,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
     __shared__ int found_seq, left, take;
     __shared__ bool begins;
     __shared__ Piece x;
+    __shared__ __align__(8) uint64_t bars[kAttnWarps * kStages];
+    uint32_t phases = 0;
+    init_bars(bars);
     constexpr int kThreads = kAttnWarps * 32;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -971,7 +1002,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
     const auto units_of = [&](int seq) -> int64_t {
         if (seq >= p.seqs) return 0;
         const Sequence s = sequence(p, seq);
-        return (int64_t)s.tiles * s.units * p.cache.heads;
+        return (int64_t)s.tiles * (s.units + kTileCost) * p.cache.heads;
     };
     int64_t total = 0;
     for (int b = tid; b < p.seqs; b += kThreads) total += units_of(b);
@@ -1017,37 +1048,46 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
         left = (int)(u_end - u);
     }
     __syncthreads();
-    while (left > 0) {
+    while (true) {
         if (tid < 32) {
             if (tid == 0) {
-                while (at >= (int64_t)x.q.tiles * x.q.units * p.cache.heads) {
-                    at -= (int64_t)x.q.tiles * x.q.units * p.cache.heads;
-                    x.q = sequence(p, ++x.seq);
+                take = 0;
+                while (left > 0) {
+                    const int span = x.q.units + kTileCost;
+                    if (at >= (int64_t)x.q.tiles * span * p.cache.heads) {
+                        at -= (int64_t)x.q.tiles * span * p.cache.heads;
+                        x.q = sequence(p, ++x.seq);
+                        continue;
+                    }
+                    const int pair = (int)(at / span), pos = (int)(at - (int64_t)pair * span);
+                    const int step = min(left, span - pos);
+                    at += step;
+                    left -= step;
+                    const int u0 = max(pos - kTileCost, 0), u1 = pos + step - kTileCost;
+                    if (u1 <= 0) continue;
+                    take = u1 - u0;
+                    begins = u0 == 0;
+                    x.head = pair / x.q.tiles;
+                    x.row0 = pair % x.q.tiles * 16;
+                    x.k0 = (x.q.lo & ~(kUnit - 1)) + u0 * kUnit;
+                    x.k1 = x.k0 + take * kUnit;
+                    if (begins && u1 < x.q.units)
+                        *info = SplitHead{1 + (int)ceil_div<int64_t>(x.q.units - u1, per), x.seq, x.head, x.row0,
+                                          min(16, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
+                    break;
                 }
-                const int pair = (int)(at / x.q.units), unit = (int)(at % x.q.units);
-                take = min(left, x.q.units - unit);
-                begins = unit == 0;
-                x.head = pair / x.q.tiles;
-                x.row0 = pair % x.q.tiles * 16;
-                x.k0 = (x.q.lo & ~(kUnit - 1)) + unit * kUnit;
-                x.k1 = x.k0 + take * kUnit;
-                if (begins && take < x.q.units)
-                    *info = SplitHead{1 + (int)ceil_div<int64_t>(x.q.units - take, per), x.seq, x.head, x.row0,
-                                      min(16, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
             }
             __syncwarp();
-            set_rows(p, x);
+            if (take) set_rows(p, x);
         }
         __syncthreads();
-        attend_piece<T, D>(p, x, smem);
+        if (take == 0) return;
+        attend_piece<T, D>(p, x, smem, bars, phases);
         join_warps<T, D>(p, x, smem,
                          begins && take == x.q.units ? nullptr
                                                      : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D>::kPart : 0));
-        __syncthreads();
-        if (tid == 0) {
-            at += take;
-            left -= take;
-        }
+        // the next piece's copies come after what was written and read here
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
     }
 }
@@ -1124,7 +1164,7 @@ int split_ctas(const Cache &c, int64_t max_pages, int64_t seqs, int64_t tiles, i
     int64_t keys = max_pages << c.page_log2;
     if (window > 0 && window + most_new < keys) keys = window + most_new;
     const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
-    if (units <= 8) return 0;
+    if (units <= 5) return 0;
     const int64_t all = seqs * c.heads * tiles * units;
     const int64_t most = (c.dim == 256 ? AttnLayout<256>::kCtas : AttnLayout<128>::kCtas) * (int64_t)sms;
     return (int)(all < most ? all : most);
