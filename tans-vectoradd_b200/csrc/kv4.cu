@@ -326,7 +326,8 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 // maximum and sum each and join at the end.
 //
 // A block's codes and scales lie together in its page, so four bulk copies
-// bring it (eight with pages of 16), the next block's while one is worked on.
+// bring it (eight with pages of 16), the next block's while one is worked on;
+// with smaller pages the lanes load a key each.
 // From shared memory they go to MMA operands in registers:
 //  * S = Q K^T: the contraction runs over D in any order, so lane (g, t) takes
 //    one key of each 8-key half and the t-th quarter of its D codes, D/8
@@ -526,17 +527,6 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     const uint32_t page_tokens = (uint32_t)p.cache.heads << page_log2;
     const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
     const uint32_t bars = (uint32_t)__cvta_generic_to_shared(s_bars) + 8u * kStages * warp;
-    // Pages of 16 and more: lanes 0..3 copy K codes, V codes, K scales and V
-    // scales of the block (of its first 16 keys, and lanes 4..7 of the others,
-    // where a page holds 16).
-    const int sets = page_log2 == 4 ? 2 : 1;
-    const bool codes = !(lane & 2), copies = page_log2 >= 4 && lane < 4 * sets;
-    const int set_key = lane >> 2 << 4;  // the first key of a lane's copy in the block
-    const uint32_t row_bytes = codes ? D / 2 : D / 16, copy_bytes = row_bytes * kBlockKeys / sets;
-    const uint8_t *src = (codes ? (lane & 1 ? p.cache.v_codes : p.cache.k_codes)
-                                : (lane & 1 ? p.cache.v_scales : p.cache.k_scales)) + head_at * row_bytes;
-    const uint32_t dst = ring_sa + (codes ? (lane & 1) * L::kCodes : 2 * L::kCodes + (lane & 1) * L::kScales) +
-                         set_key * row_bytes;
     const auto page_at = [&](int key) {  // of a key within the piece
         int page = table[key >> page_log2];
         if ((uint32_t)page >= (uint32_t)p.cache.pages) {
@@ -545,23 +535,27 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         }
         return (uint32_t)page;
     };
-    // this lane's page of the block at `base`, asked for a block ahead of its use
-    const auto page_of = [&](int base) -> int {
-        return copies && base < k1 ? table[max(lo_all, min(base + set_key, kend)) >> page_log2] : 0;
-    };
-    const auto fetch = [&](int base, int page, int stage) {
+    const uint64_t page_first = (uint64_t)head_at;  // this head's first token in a page
+    const auto fetch = [&](int base, uint32_t page0, uint32_t page1, int stage) {
         if (base >= k1) return;
-        const uint32_t bar = bars + 8u * stage;
+        const uint32_t bar = bars + 8u * stage, to = ring_sa + stage * L::kBlock;
         if (page_log2 >= 4) {
-            if (lane == 0)
+            if (lane == 0) {
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(L::kBlock) : "memory");
-            if (copies) {
-                if ((uint32_t)page >= (uint32_t)p.cache.pages) {
-                    if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-                    page = 0;
+                const auto copy = [&](uint32_t page, int first, uint32_t keys) {
+                    const uint64_t tok = page_first + (uint64_t)page * page_tokens + (uint32_t)((base + first) & in_page);
+                    copy_bulk(to + first * (D / 2), p.cache.k_codes + tok * (D / 2), keys * (D / 2), bar);
+                    copy_bulk(to + L::kCodes + first * (D / 2), p.cache.v_codes + tok * (D / 2), keys * (D / 2), bar);
+                    copy_bulk(to + 2 * L::kCodes + first * (D / 16), p.cache.k_scales + tok * (D / 16), keys * (D / 16), bar);
+                    copy_bulk(to + 2 * L::kCodes + L::kScales + first * (D / 16), p.cache.v_scales + tok * (D / 16),
+                              keys * (D / 16), bar);
+                };
+                if (page_log2 >= 5) {
+                    copy(page0, 0, 32);
+                } else {
+                    copy(page0, 0, 16);
+                    copy(page1, 16, 16);
                 }
-                const uint64_t tok = (uint64_t)(uint32_t)page * page_tokens + (uint32_t)((base + set_key) & in_page);
-                copy_bulk(dst + stage * L::kBlock, src + tok * row_bytes, copy_bytes, bar);
             }
         } else {  // smaller pages: a lane brings one key itself
             const int key = base + lane;
@@ -586,15 +580,20 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
             if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
         }
     };
+    // the pages of a block's first and last 16 keys, asked for a block ahead of
+    // their use; a key outside the piece stands for the nearest inside it
+    const auto pages_of = [&](int base, uint32_t &page0, uint32_t &page1) {
+        if (page_log2 < 4 || base >= k1) return;
+        page0 = page_at(max(lo_all, min(base, kend)));
+        if (page_log2 == 4) page1 = page_at(max(lo_all, min(base + 16, kend)));
+    };
     // what was written here by ordinary stores comes before the copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     int base = x.k0 + kBlockKeys * warp;
-    int page = page_of(base);
-    {
-        const int now = page;
-        page = page_of(base + kUnit);
-        fetch(base, now, 0);
-    }
+    uint32_t page0 = 0, page1 = 0;
+    pages_of(base, page0, page1);
+    fetch(base, page0, page1, 0);
+    pages_of(base + kUnit, page0, page1);
 
     // ---- Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
     float to_log2[2];  // positive: its sign goes into Q, and 0 becomes a number that lifts no score above 2^-20
@@ -653,11 +652,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     int stage = 0;
 #pragma unroll 1
     for (; base < k1; base += kUnit) {
-        {  // the next block into the other place
-            const int now = page;
-            page = page_of(base + 2 * kUnit);
-            fetch(base + kUnit, now, stage ^ 1);
-        }
+        fetch(base + kUnit, page0, page1, stage ^ 1);  // the next block, into the other place
+        pages_of(base + 2 * kUnit, page0, page1);
         wait_copies(bars + 8u * stage, phases >> stage & 1, p.status);
         phases ^= 1u << stage;
         const uint8_t *blk = ring + stage * L::kBlock;
@@ -971,7 +967,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
 // workspace), its last may go on in the next (part 1); those are joined by
 // attend_join_kernel, whose CTA c takes the tile that begins in stretch c
 // and does not end there, as `head` describes it.
-constexpr int kTileCost = 1;
+constexpr int kTileCost = 2;
 struct SplitHead {
     int32_t pieces;  // 0: none
     int32_t seq, head, row0, rows, first;
