@@ -1242,6 +1242,8 @@ extern "C" int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, i
     p.half = (int32_t)half;
     p.interleaved = interleaved != 0;
     p.status = status;
+    if (dtype != TANS_B200_BF16 && dtype != TANS_B200_F16)
+        return fail(TANS_B200_ERR_INVALID, "kv4_append: unsupported element type %d", dtype);
     int sms;
     rc = current_sms("kv4_append", &sms);
     if (rc) return rc;
@@ -1299,9 +1301,9 @@ extern "C" int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slo
 
 namespace {
 
-// Checks what the workspace depends on; CTAs of the split form in *ctas.
-int plan_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t tokens,
-                   int64_t most_new, int64_t window, int *ctas) {
+// Checks what the launch form depends on.
+int check_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t tokens,
+                    int64_t most_new, int64_t window) {
     int rc = check_cache("kv4_attention", cache, c);
     if (rc) return rc;
     if (seqs < 0 || seqs > 65535 || tokens < 0 || tokens > INT32_MAX || q_heads < 1 || q_heads % c->heads ||
@@ -1312,10 +1314,16 @@ int plan_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64_
     if (max_pages > INT32_MAX || (max_pages << c->page_log2) > INT32_MAX - 4096 ||
         most_new > INT32_MAX || most_new * (q_heads / c->heads) > (1 << 28))
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: a sequence holds at most 2^31-4097 tokens");
+    return TANS_B200_OK;
+}
+
+// CTAs of the split form, 0 for the whole form.
+int plan_attention(const Cache &c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t most_new, int64_t window,
+                   int *ctas) {
     int sms;
-    rc = current_sms("kv4_attention", &sms);
+    const int rc = current_sms("kv4_attention", &sms);
     if (rc) return rc;
-    *ctas = split_ctas(*c, max_pages, seqs, ceil_div<int64_t>(most_new * (q_heads / c->heads), 16), window, most_new, sms);
+    *ctas = split_ctas(c, max_pages, seqs, ceil_div<int64_t>(most_new * (q_heads / c.heads), 16), window, most_new, sms);
     return TANS_B200_OK;
 }
 
@@ -1332,7 +1340,8 @@ extern "C" int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cach
     if (!bytes) return fail(TANS_B200_ERR_INVALID, "kv4_attention: null pointer");
     Cache c;
     int ctas = 0;
-    const int rc = plan_attention(cache, &c, q_heads, max_pages, seqs, tokens, most_new, window, &ctas);
+    int rc = check_attention(cache, &c, q_heads, max_pages, seqs, tokens, most_new, window);
+    if (!rc) rc = plan_attention(c, q_heads, max_pages, seqs, most_new, window, &ctas);
     if (rc) return rc;
     *bytes = ctas * workspace_floats(cache->dim) * 4;
     return TANS_B200_OK;
@@ -1348,13 +1357,15 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     if (tokens == 0 || seqs == 0) return TANS_B200_OK;
     AttendArgs p{};
     int ctas = 0;
-    int rc = plan_attention(cache, &p.cache, q_heads, max_pages, seqs, tokens, most_new, window, &ctas);
+    int rc = check_attention(cache, &p.cache, q_heads, max_pages, seqs, tokens, most_new, window);
     if (rc) return rc;
     if (!starts && tokens != seqs)
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: one new token a sequence without starts");
     if (!q || !out || !lens || (!table && max_pages) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_attention: q, out (16-byte aligned, q's stride a multiple of 8), lens and table are needed");
+    rc = plan_attention(p.cache, q_heads, max_pages, seqs, most_new, window, &ctas);
+    if (rc) return rc;
     if (workspace_bytes < ctas * workspace_floats(cache->dim) * 4 || (ctas && (!workspace || !is_aligned(workspace, 16))))
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: the workspace is too small or not 16-byte aligned");
     p.q = q;

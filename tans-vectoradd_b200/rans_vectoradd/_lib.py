@@ -141,13 +141,8 @@ def raw_stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def new(shape: tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
-    """A dense tensor, uninitialised (torch.empty at half its cost on the host)."""
-    strides, n = [], 1
-    for d in reversed(shape):
-        strides.append(n)
-        n *= d
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=dev)
+def ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def version() -> str:

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from ._C import _post_check, _status
-from ._lib import LIB, check, new, on_device, raw_stream
+from ._lib import LIB, check, on_device, ptr, raw_stream
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
@@ -24,10 +24,13 @@ _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
 
 def _rows(name: str, t: torch.Tensor) -> int:
     """Checks [rows, cols] with a dense last dimension; the stride between rows."""
-    if not t.is_cuda or t.dim() != 2 or t.dtype not in _TYPES or (
-            not t.is_contiguous() and t.stride(1) != 1 and t.shape[1] != 1):
-        raise RuntimeError(f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor with dense rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() != 2 or t.dtype not in _TYPES or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor")
+    if t.is_contiguous():
+        return t.shape[1]
+    if t.stride(1) != 1 and t.shape[1] != 1:
+        raise RuntimeError(f"{name} must have dense rows")
+    return t.stride(0)
 
 
 def _like_x(name: str, t: torch.Tensor, x: torch.Tensor) -> int:
@@ -39,29 +42,31 @@ def _like_x(name: str, t: torch.Tensor, x: torch.Tensor) -> int:
 def _norm(x, weight, residual, eps, residual_out, quantize):
     xs = _rows("x", x)
     R, C = x.shape
-    dev, dt = x.device, x.dtype
-    wt = weight.dtype
+    dev, dt, wt = x.device, x.dtype, weight.dtype
     if (weight.dim() != 1 or weight.shape[0] != C or not weight.is_contiguous() or weight.device != dev
             or (wt != dt and wt != torch.float32)):
         raise RuntimeError("weight must be a contiguous [cols] tensor of x's type or float32")
     rs = hs = 0
     h, r_ptr, h_ptr = x, None, None
-    if residual is not None:
-        rs, r_ptr = _like_x("residual", residual, x), residual.data_ptr()
-    elif residual_out is not None:
-        raise RuntimeError("residual_out needs residual")
     with on_device(dev):
         if residual is not None:
-            h = new((R, C), dt, dev) if residual_out is None else residual_out
-            hs, h_ptr = _like_x("residual_out", h, x), h.data_ptr()
+            rs, r_ptr = _like_x("residual", residual, x), residual.data_ptr()
+            if residual_out is None:
+                h, hs = torch.empty(R, C, dtype=dt, device=dev), C
+            else:
+                h, hs = residual_out, _like_x("residual_out", residual_out, x)
+            h_ptr = h.data_ptr()
+        elif residual_out is not None:
+            raise RuntimeError("residual_out needs residual")
         if quantize:
-            y, scale = new((R, C), torch.uint8, dev), new((R,), torch.float32, dev)
-            out = (None, y.data_ptr(), scale.data_ptr())
+            y = torch.empty(R, C, dtype=torch.uint8, device=dev)
+            scale = torch.empty(R, dtype=torch.float32, device=dev)
+            y_ptr, q_ptr, s_ptr = None, y.data_ptr(), scale.data_ptr()
         else:
-            y, scale = new((R, C), dt, dev), None
-            out = (y.data_ptr(), None, None)
+            y, scale = torch.empty(R, C, dtype=dt, device=dev), None
+            y_ptr, q_ptr, s_ptr = y.data_ptr(), None, None
         check(LIB.tans_b200_add_rms_norm(x.data_ptr(), xs, r_ptr, rs, weight.data_ptr(), _TYPES[wt], eps, h_ptr, hs,
-                                         *out, R, C, _TYPES[dt], raw_stream(dev)))
+                                         y_ptr, q_ptr, s_ptr, R, C, _TYPES[dt], raw_stream(dev)))
     return y, scale, h
 
 
@@ -90,10 +95,16 @@ def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     R, C = x.shape
     dev = x.device
     with on_device(dev):
-        q, scale = new((R, C), torch.uint8, dev), new((R,), torch.float32, dev)
+        q = torch.empty(R, C, dtype=torch.uint8, device=dev)
+        scale = torch.empty(R, dtype=torch.float32, device=dev)
         check(LIB.tans_b200_quantize_tokens(x.data_ptr(), xs, q.data_ptr(), scale.data_ptr(), R, C, _TYPES[x.dtype],
                                             raw_stream(dev)))
     return q, scale
+
+
+def _check_operand(name, t, shape, dtype, dev):
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != dev:
+        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on x8's device")
 
 
 def linear(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor, *,
@@ -115,25 +126,28 @@ def linear(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: t
             or w8.shape[1] != K):
         raise RuntimeError("w8 must be a contiguous uint8 [rows, cols] tensor of e4m3 bits with x8's columns and device")
     N = w8.shape[0]
-    for t, n in ((x_scale, M), (w_scale, N)):
-        if (t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous()
-                or t.device != dev):
-            raise RuntimeError("x_scale must be contiguous f32 [tokens] and w_scale [rows]")
+    f32 = torch.float32
+    if (x_scale.dtype != f32 or x_scale.shape != (M,) or not x_scale.is_contiguous() or x_scale.device != dev
+            or w_scale.dtype != f32 or w_scale.shape != (N,) or not w_scale.is_contiguous() or w_scale.device != dev):
+        raise RuntimeError("x_scale must be contiguous f32 [tokens] and w_scale [rows]")
     if act not in _ACTS:
         raise RuntimeError(f"act must be one of {', '.join(_ACTS)}")
     if dtype != torch.bfloat16 and dtype != torch.float16:
         raise RuntimeError("dtype must be bfloat16 or float16")
-    for name, t, shape in (("bias", bias, (N,)), ("mul", mul, (M, N)), ("residual", residual, (M, N)),
-                           ("out", out, (M, N))):
-        if t is not None and (t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != dev):
-            raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on x8's device")
+    if bias is not None:
+        _check_operand("bias", bias, (N,), dtype, dev)
+    if mul is not None:
+        _check_operand("mul", mul, (M, N), dtype, dev)
+    if residual is not None:
+        _check_operand("residual", residual, (M, N), dtype, dev)
+    if out is not None:
+        _check_operand("out", out, (M, N), dtype, dev)
     with on_device(dev):
         if out is None:
-            out = new((M, N), dtype, dev)
+            out = torch.empty(M, N, dtype=dtype, device=dev)
         check(LIB.tans_b200_linear(
             x8.data_ptr(), x_scale.data_ptr(), w8.data_ptr(), w_scale.data_ptr(),
-            None if bias is None else bias.data_ptr(), _ACTS[act], None if mul is None else mul.data_ptr(),
-            None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K, _TYPES[dtype],
+            ptr(bias), _ACTS[act], ptr(mul), ptr(residual), out.data_ptr(), M, N, K, _TYPES[dtype],
             _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return out

@@ -23,7 +23,7 @@ from dataclasses import dataclass
 import torch
 
 from ._C import _post_check, _req, _status
-from ._lib import LIB, KV4, check, new, on_device, raw_stream
+from ._lib import LIB, KV4, check, on_device, ptr, raw_stream
 
 _HALF = {torch.bfloat16: 0, torch.float16: 1}
 _FLOAT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -41,25 +41,26 @@ class KV4Cache:
     v_gain: torch.Tensor | None = None
 
     def __post_init__(self):
-        shape = self.k_codes.shape
-        _req(len(shape) == 4 and shape[3] * 2 in (64, 128, 256),
-             "codes must be [pages, heads, page_size, dim/2] with dim 64, 128 or 256")
+        kc, ks, vc, vs = self.k_codes, self.k_scales, self.v_codes, self.v_scales
+        shape, u8 = kc.shape, torch.uint8
+        if len(shape) != 4 or shape[3] not in (32, 64, 128):
+            raise RuntimeError("codes must be [pages, heads, page_size, dim/2] with dim 64, 128 or 256")
         pages, heads, size, half = shape
-        _req(size > 0 and size & (size - 1) == 0, "page_size must be a power of two")
-        scales = (pages, heads, size, half // 8)
-        dev = self.k_codes.device
-        for t, want in ((self.k_codes, shape), (self.v_codes, shape), (self.k_scales, scales),
-                        (self.v_scales, scales)):
-            _req(t.dtype == torch.uint8 and t.is_cuda and t.is_contiguous() and t.shape == want
-                 and t.device == dev,
-                 "cache arrays must be contiguous CUDA uint8, codes [.., dim/2] and scales [.., dim/16], "
-                 "on one device")
+        if size < 1 or size & (size - 1):
+            raise RuntimeError("page_size must be a power of two")
+        dev, scales = kc.device, (pages, heads, size, half // 8)
+        if (not kc.is_cuda or vc.shape != shape or ks.shape != scales or vs.shape != scales
+                or kc.dtype != u8 or vc.dtype != u8 or ks.dtype != u8 or vs.dtype != u8
+                or vc.device != dev or ks.device != dev or vs.device != dev
+                or not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous())):
+            raise RuntimeError("cache arrays must be contiguous CUDA uint8, codes [.., dim/2] and scales [.., dim/16], "
+                               "on one device")
         for t in (self.k_gain, self.v_gain):
-            _req(t is None or (t.dtype == torch.float32 and t.shape == (heads,) and t.is_contiguous()
-                               and t.device == dev), "gains must be contiguous f32 [heads]")
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        self._c = KV4(ptr(self.k_codes), ptr(self.k_scales), ptr(self.v_codes), ptr(self.v_scales),
-                      ptr(self.k_gain), ptr(self.v_gain), pages, heads, size, 2 * half)
+            if t is not None:
+                _req(t.dtype == torch.float32 and t.shape == (heads,) and t.is_contiguous() and t.device == dev,
+                     "gains must be contiguous f32 [heads]")
+        self._c = KV4(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), ptr(self.k_gain), ptr(self.v_gain),
+                      pages, heads, size, 2 * half)
         self._ref = ctypes.addressof(self._c)
 
     @classmethod
@@ -142,10 +143,10 @@ def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
         _req(q.shape[0] == T, "q must have k's tokens")
     with on_device(dev):
         if q is not None:
-            out = new(q.shape, dt, dev)
+            out = torch.empty(*q.shape, dtype=dt, device=dev)
         check(LIB.tans_b200_kv4_append(
             cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, _index("slots", slots, T, torch.int64, dev),
-            None if q is None else q.data_ptr(), qs, qh, None if out is None else out.data_ptr(), pos_p, cos_p,
+            ptr(q), qs, qh, ptr(out), pos_p, cos_p,
             sin_p, top, half, int(interleaved), T, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return out
@@ -158,7 +159,7 @@ def read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat
     _req(dtype in _FLOAT, "dtype must be bfloat16, float16 or float32")
     dev, T = cache.device, slots.shape[0]
     with on_device(dev):
-        k = new((T, cache._c.heads, cache._c.dim), dtype, dev)
+        k = torch.empty(T, cache._c.heads, cache._c.dim, dtype=dtype, device=dev)
         v = torch.empty_like(k)
         check(LIB.tans_b200_kv4_read(cache._ref, _index("slots", slots, T, torch.int64, dev), k.data_ptr(),
                                      v.data_ptr(), T, _FLOAT[dtype], _status(dev).data_ptr(), raw_stream(dev)))
@@ -204,15 +205,15 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     starts_p = None if starts is None else _index("starts", starts, B + 1, torch.int32, dev)
     P = table.shape[1]
     with on_device(dev):
-        out = new(q.shape, dt, dev)
-        lse = new((T, H), torch.float32, dev) if return_lse else None
-        need = attention_workspace_bytes(cache.heads, cache.page_size, D, H, P, B, T, most_new, window, dev)
+        out = torch.empty(T, H, D, dtype=dt, device=dev)
+        lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
+        need = attention_workspace_bytes(cache._c.heads, cache._c.page_size, D, H, P, B, T, most_new, window, dev)
         if need and workspace is None:
-            workspace = new((need,), torch.uint8, dev)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
         check(LIB.tans_b200_kv4_attention(
             cache._ref, q.data_ptr(), qs, H, table.data_ptr(), table.stride(0), P, lens_p, starts_p, B, T, most_new,
-            D ** -0.5 if scale is None else scale, window, out.data_ptr(), None if lse is None else lse.data_ptr(),
+            D ** -0.5 if scale is None else scale, window, out.data_ptr(), ptr(lse),
             ws, ws_bytes, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return (out, lse) if return_lse else out
