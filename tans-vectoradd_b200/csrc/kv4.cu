@@ -320,22 +320,29 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //   lse = log(sum(exp(S)));  no visible key: O = 0, lse = -inf.
 //
 // The rows of one KV head are its new tokens times the query heads that share
-// it (row = token * group + head in group); 16 of them are the M of an
-// m16n8k16 MMA and make a tile.  The keys of a (sequence, head, tile) are cut
-// into units of 128, 32 for each of a CTA's four warps, which keep a running
-// maximum and sum each and join at the end.
+// it (row = token * group + head in group); 8, 16 or 32 of them make a tile.
+// The keys of a (sequence, head, tile) are cut into units of 128, 32 for each of
+// a CTA's four warps, which keep a running maximum and sum each and join at
+// the end.
+//
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T: the codes are the
+// A operand of m16n8k16 MMAs and the rows the N dimension, so few rows cost
+// an N of 8 and half the MMAs, sums and exponentials that an M of 16 would
+// (batch of 64, group 4: 93 us with rows as M).
 //
 // A block's codes and scales lie together in its page, so four bulk copies
 // bring it (eight with pages of 16), the next block's while one is worked on;
-// with smaller pages the lanes load a key each.
-// From shared memory they go to MMA operands in registers:
-//  * S = Q K^T: the contraction runs over D in any order, so lane (g, t) takes
-//    one key of each 8-key half and the t-th quarter of its D codes, D/8
-//    contiguous bytes; step j uses codes 4j .. 4j+3 of that quarter, and
-//    the Q fragments are laid out in the same order.
-//  * O = P V: lane (g, t) takes the g-th eighth of D of the four keys of its P
+// with smaller pages the lanes load a key each.  From shared memory they go to
+// MMA operands in registers:
+//  * S^T: the contraction runs over D in any order, so lane (g, t) takes keys g
+//    and g + 8 of 16 and the t-th quarter of their D codes, D/8 contiguous
+//    bytes; step j uses codes 4j .. 4j+3 of that quarter, and the Q fragments
+//    are laid out in the same order.
+//  * P^T: S^T comes out with a key a lane group, P^T goes in with a row a lane
+//    group: one 8 x 8 transposition across the warp per eight keys.
+//  * O^T: lane (g, t) takes the g-th eighth of D of the four keys of its P^T
 //    fragment; merging the nibbles of two keys gives bytes whose conversion is
-//    the f16 pair (key, other key) of one element.
+//    the f16 pair (key, other key) of one element, two elements a MMA.
 // code * scale is exact in f16; P enters in f16 relative to a maximum that may
 // lag by up to 2^8; sums, maxima and O stay in f32.  bf16 queries become f16
 // after a power of two per row that brings their largest element to 2^14: an
@@ -359,6 +366,7 @@ struct AttendArgs {
     float *lse;            // [tokens][q_heads], may be null
     float *parts;          // workspace of a split launch, else null
     int32_t tokens, seqs, group, max_pages, most_new, window;
+    int32_t tile_rows;     // 8, 16 or 32
     float scale;           // softmax scale
     int32_t *status;
 };
@@ -390,7 +398,7 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs &p, int seq) {
     s.hi = s.len - 1;
     const int last = s.len - s.news;  // the last key of the first new token
     s.lo = p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0;
-    s.tiles = ceil_div(s.news * p.group, 16);
+    s.tiles = ceil_div(s.news * p.group, p.tile_rows);
     s.units = max(1, ceil_div(s.hi + 1 - (s.lo & ~(kUnit - 1)), kUnit));
     return s;
 }
@@ -457,19 +465,22 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-template <int D>
+// NT: 8-row columns of a tile
+template <int D, int NT>
 struct AttnLayout {
+    static constexpr int kRows = 8 * NT;
     static constexpr int kCodes = kBlockKeys * D / 2, kScales = kBlockKeys * D / 16;  // bytes of a block
-    static constexpr int kBlock = 2 * (kCodes + kScales);                  // K codes, V codes, K scales, V scales
+    static constexpr int kBlock = 2 * (kCodes + kScales);            // K codes, V codes, K scales, V scales
     static constexpr int kRing = kAttnWarps * kStages * kBlock;
-    static constexpr int kRow = D + 8;                                     // floats of a row of O: no bank conflicts
-    static constexpr int kMerge = kAttnWarps * 16 * (kRow + 2) * 4;        // the warps' O, maxima and sums
-    static constexpr int kQ = D / 16 * 512;                                // Q fragments
-    static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ;
-    static constexpr int kCtas = D == 256 ? 2 : 4;                         // resident on an SM
-    static constexpr int kPart = 16 * (D + 2);                             // floats of a partial result
-    // place of element e in a merged row: the order of the MMA's columns
-    static __device__ int place(int e) { return e % (D / 8) * 8 + e / (D / 8); }
+    static constexpr int kEighth = D / 8 + 2;                        // floats of an eighth of a row of O
+    static constexpr int kRow = 8 * kEighth + 4;                     // of a row: no bank conflicts
+    static constexpr int kMerge = kAttnWarps * kRows * (kRow + 2) * 4;  // the warps' O, maxima and sums
+    static constexpr int kQ = NT * D * 16;                           // Q fragments
+    static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ + kRows * 4;
+    static constexpr int kCtas = D == 256 ? 2 : (NT == 4 ? 2 : (NT == 2 ? 4 : 5));  // resident on an SM
+    static constexpr int kPart = kRows * (D + 2);                    // floats of a partial result
+    // place of element e in a merged row
+    static __device__ int place(int e) { return e / (D / 8) * kEighth + e % (D / 8); }
 };
 
 // One piece of a tile's work, in shared memory.
@@ -479,19 +490,19 @@ struct Piece {
     int k0, k1;  // keys, multiples of kUnit
     // keys that some row of the tile sees, and those that every row sees
     int lo_all, hi_all, lo_in, hi_in;
-    int hi[16];  // the last key that each row sees
+    int hi[32];  // the last key that each row sees
 };
 
 __device__ __forceinline__ int first_seen(const AttendArgs &p, int last) {
     return p.window > 0 && last + 1 > p.window ? last + 1 - p.window : 0;
 }
 
-// Fills in what follows from q, row0, k0 and k1; called by one whole warp, lane r < 16 for row r.
+// Fills in what follows from q, row0, k0 and k1; called by one whole warp, lane r for row r.
 __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
     const int lane = threadIdx.x & 31;
-    const int end = min(x.row0 + 16, x.q.news * p.group) - 1;
+    const int end = min(x.row0 + p.tile_rows, x.q.news * p.group) - 1;
     const auto last_key = [&](int row) { return x.q.len - x.q.news + row / p.group; };
-    if (lane < 16) x.hi[lane] = last_key(min(x.row0 + lane, end));
+    x.hi[lane] = last_key(min(x.row0 + lane, end));
     if (lane == 0) {
         x.hi_in = last_key(x.row0);
         x.hi_all = last_key(end);
@@ -504,21 +515,23 @@ __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
 
 // Runs a piece (set by the caller, before a block barrier).  s_bars: the rings'
 // barriers, whose parities this warp keeps in `phases`.  Afterwards the four
-// warps' results lie in `smem` as [warp][16][kRow] O, [warp][16] maxima and sums.
-template <typename T, int D>
+// warps' results lie in `smem` as [warp][kRows][kRow] O, [warp][kRows] maxima and sums.
+template <typename T, int D, int NT>
 __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem, uint64_t *s_bars,
                                              uint32_t &phases) {
-    using L = AttnLayout<D>;
-    constexpr int kSteps = D / 16;         // MMA steps of S
-    constexpr int kTiles = D / 8;          // MMA column tiles of O
-    constexpr int kE = D / 8;              // elements of an eighth of a head
-    constexpr int kVS = (D + 127) / 128;   // scales of an eighth
-    constexpr int kKS = D / 64;            // scales of a quarter
+    using L = AttnLayout<D, NT>;
+    constexpr int kSteps = D / 16;        // MMA steps of S
+    constexpr int kTiles = D / 16;        // MMA row tiles of O
+    constexpr int kE = D / 8;             // elements of an eighth of a head
+    constexpr int kVS = (D + 127) / 128;  // scales of an eighth
+    constexpr int kKS = D / 64;           // scales of a quarter
+    constexpr int kTogether = NT > 1 ? 1 : 2;  // halves of 16 keys worked on together
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int head = x.head, k1 = x.k1, lo_all = x.lo_all;
     const int kend = min(x.hi_all, k1 - 1);  // the piece's last key
     uint8_t *ring = smem + warp * (kStages * L::kBlock);
-    uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ);
+    uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ - L::kRows * 4);
+    float *factors = reinterpret_cast<float *>(smem + L::kBytes - L::kRows * 4);
 
     // ---- copies of the warp's blocks into its ring
     const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
@@ -595,60 +608,68 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     fetch(base, page0, page1, 0);
     pages_of(base + kUnit, page0, page1);
 
-    // ---- Q: step j, lane (g, t): elements 4j..4j+3 of quarter t of rows g and g + 8
-    float to_log2[2];  // positive: its sign goes into Q, and 0 becomes a number that lifts no score above 2^-20
-    {
+    // ---- Q: steps 2i and 2i + 1, lane (g, t): elements 8i .. 8i + 7 of quarter t of
+    // row g.  A row's factor brings its scores to base 2; it is positive: its sign
+    // goes into Q, and 0 becomes a number that lifts no score above 2^-20.
+    for (int n = warp; n < NT; n += kAttnWarps) {
         const float c = p.scale * kLog2e * (p.cache.k_gain ? p.cache.k_gain[head] : 1.f);
-        const int end = min(x.row0 + 16, x.q.news * p.group) - 1;
-        uint2 u[2][kSteps];
+        const int end = min(x.row0 + L::kRows, x.q.news * p.group) - 1, row = min(x.row0 + 8 * n + g, end);
+        const T *from = static_cast<const T *>(p.q) + (int64_t)(x.q.first + row / p.group) * p.q_stride +
+                        ((int64_t)head * p.group + row % p.group) * D + t * (D / 4);
+        uint4 u[kSteps / 2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int row = min(x.row0 + g + 8 * i, end);
-            const T *src = static_cast<const T *>(p.q) + (int64_t)(x.q.first + row / p.group) * p.q_stride +
-                           ((int64_t)head * p.group + row % p.group) * D + t * (D / 4);
+        for (int i = 0; i < kSteps / 2; i++) u[i] = *reinterpret_cast<const uint4 *>(from + 8 * i);
+        float factor = fabsf(c);
+        const uint32_t flip = c < 0.f ? 0x80008000u : 0u;
+        if constexpr (!std::is_same_v<T, __half>) {
+            float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < kSteps; j++) u[i][j] = *reinterpret_cast<const uint2 *>(src + 4 * j);
-            to_log2[i] = fabsf(c);
-            const uint32_t flip = c < 0.f ? 0x80008000u : 0u;
-            if constexpr (!std::is_same_v<T, __half>) {
-                float top = 0.f;
+            for (int i = 0; i < kSteps / 2; i++) {
+                const T *e = reinterpret_cast<const T *>(&u[i]);
 #pragma unroll
-                for (int j = 0; j < kSteps; j++) {
-                    const T *e = reinterpret_cast<const T *>(&u[i][j]);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) top = fmaxf(top, fabsf(to_f32(e[k])));
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // top * 2^k in [2^14, 2^15)
-                k = top == 0.f || top > 3.4e38f ? 0 : min(k, 100);
-                const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-                to_log2[i] *= __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-                for (int j = 0; j < kSteps; j++) {
-                    const T *e = reinterpret_cast<const T *>(&u[i][j]);
-                    u[i][j] = make_uint2(h2_of(to_f32(e[0]) * up, to_f32(e[1]) * up),
-                                         h2_of(to_f32(e[2]) * up, to_f32(e[3]) * up));
-                }
+                for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(to_f32(e[k])));
             }
-            to_log2[i] = max_nan(to_log2[i], 1e-37f);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int k = 14 - ((int)(__float_as_uint(top) >> 23) - 127);  // top * 2^k in [2^14, 2^15)
+            k = top == 0.f || top > 3.4e38f ? 0 : min(k, 100);
+            const float up = __uint_as_float((uint32_t)(127 + k) << 23);
+            factor *= __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
-            for (int j = 0; j < kSteps; j++) u[i][j].x ^= flip, u[i][j].y ^= flip;
+            for (int i = 0; i < kSteps / 2; i++) {
+                const T *e = reinterpret_cast<const T *>(&u[i]);
+                u[i] = make_uint4(h2_of(to_f32(e[0]) * up, to_f32(e[1]) * up), h2_of(to_f32(e[2]) * up, to_f32(e[3]) * up),
+                                  h2_of(to_f32(e[4]) * up, to_f32(e[5]) * up), h2_of(to_f32(e[6]) * up, to_f32(e[7]) * up));
+            }
         }
-        if (warp == 0) {
 #pragma unroll
-            for (int j = 0; j < kSteps; j++) qs[j * 32 + lane] = make_uint4(u[0][j].x, u[1][j].x, u[0][j].y, u[1][j].y);
-        }
+        for (int i = 0; i < kSteps / 2; i++)
+            qs[(n * (kSteps / 2) + i) * 32 + lane] =
+                make_uint4(u[i].x ^ flip, u[i].y ^ flip, u[i].z ^ flip, u[i].w ^ flip);
+        if (t == 0) factors[8 * n + g] = max_nan(factor, 1e-37f);
     }
     __syncthreads();
+    float2 to_log2[NT];  // of this lane's rows 8n + 2t and 8n + 2t + 1
+#pragma unroll
+    for (int n = 0; n < NT; n++) to_log2[n] = *reinterpret_cast<const float2 *>(factors + 8 * n + 2 * t);
     // blocks that every row sees whole
     const int inner = x.lo_in, inner_span = min(x.hi_in, kend) - (kBlockKeys - 1) - x.lo_in;
 
-    float o[kTiles][4];
+    // O^T: row tile j, elements 2j and 2j + 1 of this lane's eighth, rows 2t and 2t + 1
+    float o[kTiles][NT][4];
 #pragma unroll
-    for (int j = 0; j < kTiles; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    // scores up to this need no new maximum; what is subtracted; the sums
-    float limit[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+    for (int j = 0; j < kTiles; j++)
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
+    // scores up to `limit` need no new maximum; `less` is subtracted; the sums are this lane's keys'
+    float limit[NT][2], less[NT][2], sum[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) limit[n][i] = -INFINITY, less[n][i] = sum[n][i] = 0.f;
+    // Of eight keys the m-th is m ^ (m >> 1 & 1): the V reads of lanes t = 0..3
+    // then fall on rows of both parities.
+    const int own_key = g ^ (g >> 1 & 1);
     int stage = 0;
 #pragma unroll 1
     for (; base < k1; base += kUnit) {
@@ -658,190 +679,209 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         phases ^= 1u << stage;
         const uint8_t *blk = ring + stage * L::kBlock;
         stage ^= 1;
-        // Column n of an 8-key half is key n ^ (n >> 1 & 1): the V reads of
-        // lanes t = 0..3 then fall on rows of both parities.
-        // ---- scores of 32 keys, eight at a time
-        float s[4][4] = {};
-        {
-            uint32_t w[4][D / 32], f[4][kKS];
-#pragma unroll
-            for (int h = 0; h < 4; h++) {
-                const int r = 8 * h + (g ^ (g >> 1 & 1));
-                const uint8_t *kp = blk + r * (D / 2);
-                if constexpr (D == 64) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(kp + 8 * t);
-                    w[h][0] = v.x, w[h][1] = v.y;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < D / 128; i++) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(kp + t * (D / 8) + 16 * i);
-                        w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
-                    }
-                }
-                const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
-                if constexpr (kKS == 1) {
-                    f[h][0] = e4m3x2_h2(*sp * 0x101u);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kKS; i += 2) {
-                        const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
-                        f[h][i] = __byte_perm(two, two, 0x1010);
-                        f[h][i + 1] = __byte_perm(two, two, 0x3232);
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kSteps; j += 2) {
-                const uint4 qa = qs[j * 32 + lane], qb = qs[(j + 1) * 32 + lane];
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    uint32_t b[4];
-                    e2m1x8_h2(w[h][j / 2], b);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) b[i] = mul_h2(b[i], f[h][j / 4]);
-                    mma_f16(s[h], qa, b[0], b[1]);
-                    mma_f16(s[h], qb, b[2], b[3]);
-                }
-            }
-        }
-        // ---- the running maximum and the weights
         const bool edge = base < inner || base - inner > inner_span;
-        if (edge) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int last = x.hi[g + 8 * i], lo = first_seen(p, last), hi = min(last, kend);
+        for (int y0 = 0; y0 < 2; y0 += kTogether) {
+            // ---- scores of the keys base + 16 y ..
+            float s[kTogether][NT][4];
 #pragma unroll
-                for (int h = 0; h < 4; h++)
+            for (int y = 0; y < kTogether; y++) {
+                uint32_t w[2][D / 32], f[2][kKS];
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int key = base + 8 * h + ((2 * t + c) ^ (t & 1));
-                        if (key < lo || key > hi) s[h][2 * i + c] = -INFINITY;
+                for (int h = 0; h < 2; h++) {
+                    const int r = 16 * (y0 + y) + 8 * h + own_key;
+                    const uint8_t *kp = blk + r * (D / 2) + t * (D / 8);
+                    if constexpr (D == 64) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+                        w[h][0] = v.x, w[h][1] = v.y;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < D / 128; i++) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(kp + 16 * i);
+                            w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
+                        }
                     }
-            }
-        }
-        float m[2];
+                    const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
+                    if constexpr (kKS == 1) {
+                        f[h][0] = e4m3x2_h2(*sp * 0x101u);
+                    } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            m[i] = s[0][2 * i];
-#pragma unroll
-            for (int k = 1; k < 8; k++) m[i] = fmaxf(m[i], s[k / 2][2 * i + (k & 1)]);
-            m[i] *= to_log2[i];
-        }
-        if (__any_sync(0xffffffffu, m[0] > limit[0] || m[1] > limit[1])) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float top = limit[i] == -INFINITY ? -INFINITY : less[i];
-                float n = fmaxf(m[i], top);
-                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 1));
-                n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 2));
-                limit[i] = n + 8.f;
-                less[i] = n == -INFINITY ? 0.f : n;
-                const float f = exp2f(top - less[i]);  // nothing to scale yet while top is -inf
-                sum[i] *= f;
-#pragma unroll
-                for (int j = 0; j < kTiles; j++) {
-                    o[j][2 * i] *= f;
-                    o[j][2 * i + 1] *= f;
-                }
-            }
-        }
-        uint4 pf[2];
-#pragma unroll
-        for (int h = 0; h < 4; h++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                s[h][c] = exp2_fast(__fmaf_rn(s[h][c], to_log2[c >> 1], -less[c >> 1]));
-                sum[c >> 1] += s[h][c];
-            }
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-            pf[b] = make_uint4(h2_of(s[2 * b][0], s[2 * b][1]), h2_of(s[2 * b][2], s[2 * b][3]),
-                               h2_of(s[2 * b + 1][0], s[2 * b + 1][1]), h2_of(s[2 * b + 1][2], s[2 * b + 1][3]));
-        // ---- values of the lane's four keys of each 16
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-            uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int r = 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-                const uint8_t *vp = blk + L::kCodes + r * (D / 2);
-                if constexpr (D == 64) {
-                    w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
-                } else if constexpr (D == 128) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + 8 * g);
-                    w[k][0] = v.x, w[k][1] = v.y;
-                } else {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
-                    w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
-                }
-#pragma unroll
-                for (int i = 0; i < kVS; i++)
-                    sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
-            }
-            // Keys outside the piece hold anything: their values count as 0.  A NaN
-            // scale on a key that only some rows see must not reach the others
-            // as 0 * NaN: its values count as 0 here and are added below.
-            uint32_t nan_keys = 0;
-            if (edge) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int key = base + 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-                    const bool real = key >= lo_all && key <= kend;
-#pragma unroll
-                    for (int i = 0; i < kVS; i++) {
-                        const bool nan = (sc[k][i] & 0x7Fu) == 0x7Fu;
-                        if (nan && real) nan_keys |= 1u << (k * kVS + i);
-                        if (nan || !real) sc[k][i] = 0;
+                        for (int i = 0; i < kKS; i += 2) {
+                            const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
+                            f[h][i] = __byte_perm(two, two, 0x1010);
+                            f[h][i + 1] = __byte_perm(two, two, 0x3232);
+                        }
                     }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < kVS; i++) {
-                const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
-                constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
+                for (int n = 0; n < NT; n++) s[y][n][0] = s[y][n][1] = s[y][n][2] = s[y][n][3] = 0.f;
 #pragma unroll
-                for (int j = 0; j < kPer; j += 8) {
-                    const int word = (i * 16 + j) / 8;
-                    uint32_t even[2][4], odd[2][4];
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
-                        e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
-                        e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        mma_f16(o[i * 16 + j + 2 * e], pf[y], mul_h2(even[0][e], f[0]), mul_h2(even[1][e], f[1]));
-                        mma_f16(o[i * 16 + j + 2 * e + 1], pf[y], mul_h2(odd[0][e], f[0]), mul_h2(odd[1][e], f[1]));
-                    }
-                }
-            }
-            if (edge && __any_sync(0xffffffffu, nan_keys)) {
-                uint32_t seen[4];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int last = x.hi[g + 8 * i], lo = first_seen(p, last), hi = min(last, kend);
+                for (int i = 0; i < kSteps / 2; i++) {
+                    uint32_t a[2][4];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const int a = base + 16 * y + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
-                        seen[2 * h + i] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
+                        e2m1x8_h2(w[h][i], a[h]);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) a[h][k] = mul_h2(a[h][k], f[h][i / 2]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 q = qs[(n * (kSteps / 2) + i) * 32 + lane];
+                        mma_f16(s[y][n], make_uint4(a[0][0], a[1][0], a[0][1], a[1][1]), q.x, q.y);
+                        mma_f16(s[y][n], make_uint4(a[0][2], a[1][2], a[0][3], a[1][3]), q.z, q.w);
                     }
                 }
+            }
+            // ---- the running maximum and the weights
+            if (edge) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int last = x.hi[8 * n + 2 * t + i], lo = first_seen(p, last), hi = min(last, kend);
+#pragma unroll
+                        for (int y = 0; y < kTogether; y++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int key = base + 16 * (y0 + y) + 8 * h + own_key;
+                                if (key < lo || key > hi) s[y][n][2 * h + i] = -INFINITY;
+                            }
+                    }
+            }
+            float m[NT][2];
+            bool grew = false;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    m[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
+                    if (kTogether == 2) m[n][i] = fmaxf(m[n][i], fmaxf(s[kTogether - 1][n][i], s[kTogether - 1][n][2 + i]));
+                    m[n][i] *= i ? to_log2[n].y : to_log2[n].x;
+                    grew |= m[n][i] > limit[n][i];
+                }
+            if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float top = limit[n][i] == -INFINITY ? -INFINITY : less[n][i];
+                        float v = fmaxf(m[n][i], top);
+#pragma unroll
+                        for (int lanes = 4; lanes < 32; lanes *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
+                        limit[n][i] = v + 8.f;
+                        less[n][i] = v == -INFINITY ? 0.f : v;
+                        const float f = exp2f(top - less[n][i]);  // nothing to scale yet while top is -inf
+                        sum[n][i] *= f;
+#pragma unroll
+                        for (int j = 0; j < kTiles; j++) {
+                            o[j][n][i] *= f;
+                            o[j][n][2 + i] *= f;
+                        }
+                    }
+            }
+            uint32_t pt[kTogether][NT][2];  // P^T fragments
+#pragma unroll
+            for (int y = 0; y < kTogether; y++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        s[y][n][c] = exp2_fast(__fmaf_rn(s[y][n][c], c & 1 ? to_log2[n].y : to_log2[n].x, -less[n][c & 1]));
+                        sum[n][c & 1] += s[y][n][c];
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                            : "=r"(pt[y][n][h])
+                            : "r"(h2_of(s[y][n][2 * h], s[y][n][2 * h + 1])));
+                }
+            // ---- values of the lane's four keys of each 16
+#pragma unroll
+            for (int y = 0; y < kTogether; y++) {
+                uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int r = 16 * (y0 + y) + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                    const uint8_t *vp = blk + L::kCodes + r * (D / 2);
+                    if constexpr (D == 64) {
+                        w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
+                    } else if constexpr (D == 128) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(vp + 8 * g);
+                        w[k][0] = v.x, w[k][1] = v.y;
+                    } else {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
+                        w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+                    }
+#pragma unroll
+                    for (int i = 0; i < kVS; i++)
+                        sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
+                }
+                // Keys outside the piece hold anything: their values count as 0.  A NaN
+                // scale on a key that only some rows see must not reach the others
+                // as 0 * NaN: its values count as 0 here and are added below.
+                uint32_t nan_keys = 0;
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int key = base + 16 * (y0 + y) + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                        const bool real = key >= lo_all && key <= kend;
+#pragma unroll
+                        for (int i = 0; i < kVS; i++) {
+                            const bool nan = (sc[k][i] & 0x7Fu) == 0x7Fu;
+                            if (nan && real) nan_keys |= 1u << (k * kVS + i);
+                            if (nan || !real) sc[k][i] = 0;
+                        }
+                    }
+                }
+                constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
 #pragma unroll
                 for (int i = 0; i < kVS; i++) {
-                    uint32_t b[2];
+                    const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        b[k] = h2_of(nan_keys >> (2 * k * kVS + i) & 1 ? 1.f : 0.f,
-                                     nan_keys >> ((2 * k + 1) * kVS + i) & 1 ? 1.f : 0.f);
-                    float n[4] = {};
-                    mma_f16(n, make_uint4(seen[0], seen[1], seen[2], seen[3]), b[0], b[1]);
-                    constexpr int kPer = kE < 16 ? kE : 16;
+                    for (int j = 0; j < kPer; j += 8) {
+                        const int word = (i * 16 + j) / 8;
+                        uint32_t even[2][4], odd[2][4];
 #pragma unroll
-                    for (int j = 0; j < kPer; j++)
+                        for (int b = 0; b < 2; b++) {
+                            const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
+                            e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
+                            e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
+                        }
 #pragma unroll
-                        for (int c = 0; c < 4; c++)
-                            if (n[c] > 0.f) o[i * 16 + j][c] = NAN;
+                        for (int e = 0; e < 4; e++) {
+                            const uint4 a = make_uint4(mul_h2(even[0][e], f[0]), mul_h2(odd[0][e], f[0]),
+                                                       mul_h2(even[1][e], f[1]), mul_h2(odd[1][e], f[1]));
+#pragma unroll
+                            for (int n = 0; n < NT; n++) mma_f16(o[(i * 16 + j) / 2 + e][n], a, pt[y][n][0], pt[y][n][1]);
+                        }
+                    }
+                }
+                if (edge && __any_sync(0xffffffffu, nan_keys)) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const int last = x.hi[8 * n + g], lo = first_seen(p, last), hi = min(last, kend);
+                        uint32_t seen[2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int a = base + 16 * (y0 + y) + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
+                            seen[h] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kVS; i++) {
+                            uint32_t flag[2];
+#pragma unroll
+                            for (int k = 0; k < 2; k++)
+                                flag[k] = h2_of(nan_keys >> (2 * k * kVS + i) & 1 ? 1.f : 0.f,
+                                                nan_keys >> ((2 * k + 1) * kVS + i) & 1 ? 1.f : 0.f);
+                            float v[4] = {};
+                            mma_f16(v, make_uint4(flag[0], flag[0], flag[1], flag[1]), seen[0], seen[1]);
+#pragma unroll
+                            for (int j = 0; j < kPer / 2; j++)
+#pragma unroll
+                                for (int c = 0; c < 4; c++)
+                                    if (v[c] > 0.f) o[i * 8 + j][n][c] = NAN;
+                        }
+                    }
                 }
             }
         }
@@ -851,20 +891,23 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     // ---- the warps' results, side by side
     __syncthreads();
     float *merge = reinterpret_cast<float *>(smem);
-    float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
+    float *tops = merge + kAttnWarps * L::kRows * L::kRow, *sums = tops + kAttnWarps * L::kRows;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        if (t == 0) {
-            tops[warp * 16 + g + 8 * i] = limit[i] == -INFINITY ? -INFINITY : less[i];
-            sums[warp * 16 + g + 8 * i] = sum[i];
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int row = warp * L::kRows + 8 * n + 2 * t + i;
+#pragma unroll
+            for (int lanes = 4; lanes < 32; lanes *= 2) sum[n][i] += __shfl_xor_sync(0xffffffffu, sum[n][i], lanes);
+            if (g == 0) {
+                tops[row] = limit[n][i] == -INFINITY ? -INFINITY : less[n][i];
+                sums[row] = sum[n][i];
+            }
+#pragma unroll
+            for (int j = 0; j < kTiles; j++)
+                *reinterpret_cast<float2 *>(merge + row * L::kRow + g * L::kEighth + 2 * j) =
+                    make_float2(o[j][n][i], o[j][n][2 + i]);
         }
-#pragma unroll
-        for (int j = 0; j < kTiles; j++)  // tile j, columns 2t and 2t + 1
-            *reinterpret_cast<float2 *>(merge + (warp * 16 + g + 8 * i) * L::kRow + 8 * j + 2 * t) =
-                make_float2(o[j][2 * i], o[j][2 * i + 1]);
-    }
     __syncthreads();
 }
 
@@ -890,35 +933,35 @@ __device__ __forceinline__ void write_row(const AttendArgs &p, int head, int hea
 
 // Joins the four warps' results of a piece: into the output if the piece is
 // the tile's whole range, else into a part of the workspace.
-template <typename T, int D>
+template <typename T, int D, int NT>
 __device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, const uint8_t *smem, float *part) {
     const float *merge = reinterpret_cast<const float *>(smem);
-    using L = AttnLayout<D>;
-    const float *tops = merge + kAttnWarps * 16 * L::kRow, *sums = tops + kAttnWarps * 16;
+    using L = AttnLayout<D, NT>;
+    const float *tops = merge + kAttnWarps * L::kRows * L::kRow, *sums = tops + kAttnWarps * L::kRows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rows = min(16, x.q.news * p.group - x.row0);
+    const int rows = min(L::kRows, x.q.news * p.group - x.row0);
     for (int r = warp; r < rows; r += kAttnWarps) {
         float m = -INFINITY, l = 0.f, f[kAttnWarps], v[D / 32];
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, tops[w * 16 + r]);
+        for (int w = 0; w < kAttnWarps; w++) m = fmaxf(m, tops[w * L::kRows + r]);
 #pragma unroll
         for (int w = 0; w < kAttnWarps; w++) {
-            f[w] = part_factor(tops[w * 16 + r], sums[w * 16 + r], m);
-            l += f[w] * sums[w * 16 + r];
+            f[w] = part_factor(tops[w * L::kRows + r], sums[w * L::kRows + r], m);
+            l += f[w] * sums[w * L::kRows + r];
         }
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {
             v[i] = 0.f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; w++)
-                if (f[w] != 0.f) v[i] += f[w] * merge[(w * 16 + r) * L::kRow + L::place(lane + 32 * i)];
+                if (f[w] != 0.f) v[i] += f[w] * merge[(w * L::kRows + r) * L::kRow + L::place(lane + 32 * i)];
         }
         if (part) {
 #pragma unroll
             for (int i = 0; i < D / 32; i++) part[r * D + lane + 32 * i] = v[i];
             if (lane == 0) {
-                part[16 * D + r] = m;
-                part[16 * D + 16 + r] = l;
+                part[L::kRows * D + r] = m;
+                part[L::kRows * (D + 1) + r] = l;
             }
         } else {
             const int row = x.row0 + r;
@@ -935,8 +978,8 @@ __device__ __forceinline__ void init_bars(uint64_t *bars) {
 }
 
 // One CTA a (tile, head, sequence), over all its keys.
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_kernel(const AttendArgs p) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) attend_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
     __shared__ Piece x;
@@ -944,11 +987,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
     uint32_t phases = 0;
     init_bars(bars);
     const Sequence q = sequence(p, blockIdx.z);
-    if ((int)blockIdx.x * 16 >= q.news * p.group) return;
+    if ((int)blockIdx.x * p.tile_rows >= q.news * p.group) return;
     if (threadIdx.x < 32) {
         if (threadIdx.x == 0) {
             x.q = q;
-            x.seq = blockIdx.z, x.head = blockIdx.y, x.row0 = blockIdx.x * 16;
+            x.seq = blockIdx.z, x.head = blockIdx.y, x.row0 = blockIdx.x * p.tile_rows;
             x.k0 = q.lo & ~(kUnit - 1);
             x.k1 = x.k0 + q.units * kUnit;
         }
@@ -956,8 +999,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
         set_rows(p, x);
     }
     __syncthreads();
-    attend_piece<T, D>(p, x, smem, bars, phases);
-    join_warps<T, D>(p, x, smem, nullptr);
+    attend_piece<T, D, NT>(p, x, smem, bars, phases);
+    join_warps<T, D, NT>(p, x, smem, nullptr);
 }
 
 // Split form: the units of all tiles in a row (sequence, head, tile, unit),
@@ -974,13 +1017,13 @@ struct SplitHead {
     int32_t pad[2];
 };
 
-template <int D>
+template <int D, int NT>
 __host__ __device__ constexpr int64_t split_floats() {
-    return sizeof(SplitHead) / 4 + 2 * AttnLayout<D>::kPart;
+    return sizeof(SplitHead) / 4 + 2 * AttnLayout<D, NT>::kPart;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_split_kernel(const AttendArgs p) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) attend_split_kernel(const AttendArgs p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ int64_t warp_sum[kAttnWarps], found_at, at;
     __shared__ int found_seq, left, take;
@@ -992,7 +1035,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
     constexpr int kThreads = kAttnWarps * 32;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    float *mine = p.parts + blockIdx.x * split_floats<D>();
+    float *mine = p.parts + blockIdx.x * split_floats<D, NT>();
     SplitHead *info = reinterpret_cast<SplitHead *>(mine);
     if (tid == 0) info->pieces = 0;
     const auto units_of = [&](int seq) -> int64_t {
@@ -1064,12 +1107,12 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
                     take = u1 - u0;
                     begins = u0 == 0;
                     x.head = pair / x.q.tiles;
-                    x.row0 = pair % x.q.tiles * 16;
+                    x.row0 = pair % x.q.tiles * p.tile_rows;
                     x.k0 = (x.q.lo & ~(kUnit - 1)) + u0 * kUnit;
                     x.k1 = x.k0 + take * kUnit;
                     if (begins && u1 < x.q.units)
                         *info = SplitHead{1 + (int)ceil_div<int64_t>(x.q.units - u1, per), x.seq, x.head, x.row0,
-                                          min(16, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
+                                          min(p.tile_rows, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
                     break;
                 }
             }
@@ -1078,10 +1121,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
         }
         __syncthreads();
         if (take == 0) return;
-        attend_piece<T, D>(p, x, smem, bars, phases);
-        join_warps<T, D>(p, x, smem,
+        attend_piece<T, D, NT>(p, x, smem, bars, phases);
+        join_warps<T, D, NT>(p, x, smem,
                          begins && take == x.q.units ? nullptr
-                                                     : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D>::kPart : 0));
+                                                     : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D, NT>::kPart : 0));
         // the next piece's copies come after what was written and read here
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
@@ -1092,29 +1135,29 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D>::kCtas) attend_
 // it.  A CTA takes four rows, four warps each that take turns at the parts;
 // the parts' factors come first, so that the loads of O wait for nothing.
 constexpr int kJoinRows = 4, kJoinWarps = 4;
-template <typename T, int D>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
     constexpr int kMost = 512;  // parts whose factors are kept at a time
     __shared__ float factor[kJoinRows][kMost], o_of[kJoinRows][kJoinWarps][D];
     pdl_enter();
-    const float *at = p.parts + blockIdx.x * split_floats<D>();
+    const float *at = p.parts + blockIdx.x * split_floats<D, NT>();
     const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
     const int slot = threadIdx.x >> 7, turn = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31;
     const int r = blockIdx.y * kJoinRows + slot;
     if (h.pieces == 0 || (int)blockIdx.y * kJoinRows >= h.rows) return;
     const auto part = [&](int i) {
-        return at + i * split_floats<D>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D>::kPart);
+        return at + i * split_floats<D, NT>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D, NT>::kPart);
     };
     const bool real = r < h.rows;
     float m = -INFINITY, l = 0.f, v[D / 32] = {};
-    for (int i = lane; real && i < h.pieces; i += 32) m = fmaxf(m, part(i)[16 * D + r]);
+    for (int i = lane; real && i < h.pieces; i += 32) m = fmaxf(m, part(i)[8 * NT * D + r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     for (int i0 = 0; i0 < h.pieces; i0 += kMost) {
         const int n = min(kMost, h.pieces - i0);
         __syncthreads();
         for (int i = turn * 32 + lane; real && i < n; i += kJoinWarps * 32) {
-            const float s = part(i0 + i)[16 * D + 16 + r], f = part_factor(part(i0 + i)[16 * D + r], s, m);
+            const float s = part(i0 + i)[8 * NT * (D + 1) + r], f = part_factor(part(i0 + i)[8 * NT * D + r], s, m);
             factor[slot][i] = f;
             l += f * s;
         }
@@ -1153,33 +1196,65 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
 }
 
-// CTAs of the split form: 0 for the whole form.  Few (sequence, head, tile)s
-// with long ranges are split over the card; enough of them, or short ranges,
-// are not.
-int split_ctas(const Cache &c, int64_t max_pages, int64_t seqs, int64_t tiles, int64_t window, int64_t most_new, int sms) {
+// Rows of a tile.
+int rows_of_tile(int64_t rows, int64_t dim) { return rows <= 8 ? 8 : (rows <= 16 || dim == 256 ? 16 : 32); }
+
+// f(<D, NT>) for a head size and a tile's rows.
+template <typename F>
+auto dispatch_tile(int64_t dim, int tile_rows, F &&f) {
+    const auto with = [&](auto d) {
+        if (tile_rows == 8) return f(d, std::integral_constant<int, 1>{});
+        if constexpr (decltype(d)::value != 256)
+            if (tile_rows == 32) return f(d, std::integral_constant<int, 4>{});
+        return f(d, std::integral_constant<int, 2>{});
+    };
+    if (dim == 64) return with(std::integral_constant<int, 64>{});
+    if (dim == 128) return with(std::integral_constant<int, 128>{});
+    return with(std::integral_constant<int, 256>{});
+}
+
+// CTAs of the split form, and floats of its workspace for each; 0 for the
+// whole form: ranges of a few units, which are not worth the second launch.
+struct Plan {
+    int ctas, tile_rows, rows;  // rows of a sequence at most
+    int64_t floats;
+};
+int make_plan(const Cache &c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t most_new, int64_t window, Plan *plan) {
+    int sms;
+    const int rc = current_sms("kv4_attention", &sms);
+    if (rc) return rc;
+    plan->rows = (int)(most_new * (q_heads / c.heads));
+    plan->tile_rows = rows_of_tile(plan->rows, c.dim);
     int64_t keys = max_pages << c.page_log2;
     if (window > 0 && window + most_new < keys) keys = window + most_new;
     const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
-    if (units <= 5) return 0;
-    const int64_t all = seqs * c.heads * tiles * units;
-    const int64_t most = (c.dim == 256 ? AttnLayout<256>::kCtas : AttnLayout<128>::kCtas) * (int64_t)sms;
-    return (int)(all < most ? all : most);
+    const int64_t all = seqs * c.heads * ceil_div(plan->rows, plan->tile_rows) * units;
+    dispatch_tile(c.dim, plan->tile_rows, [&](auto d, auto nt) {
+        constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
+        const int64_t most = AttnLayout<D, NT>::kCtas * (int64_t)sms;
+        plan->ctas = units <= 5 ? 0 : (int)(all < most ? all : most);
+        plan->floats = plan->ctas * split_floats<D, NT>();
+        return 0;
+    });
+    return TANS_B200_OK;
 }
 
-template <typename T, int D>
-int launch_attend(const AttendArgs &p, int max_rows, int ctas, cudaStream_t st) {
-    constexpr int smem = AttnLayout<D>::kBytes;
-    if (!ctas) {
-        const int rc = allow_smem<attend_kernel<T, D>>("attend_kernel", smem);
+template <typename T, int D, int NT>
+int launch_attend(const AttendArgs &p, const Plan &plan, cudaStream_t st) {
+    using L = AttnLayout<D, NT>;
+    const dim3 block(kAttnWarps * 32);
+    if (!plan.ctas) {
+        const int rc = allow_smem<attend_kernel<T, D, NT>>("attend_kernel", L::kBytes);
         return rc ? rc
-                  : launch_ex(attend_kernel<T, D>, dim3(ceil_div(max_rows, 16), p.cache.heads, p.seqs), dim3(kAttnWarps * 32), smem, 1, st,
-                              "attend_kernel", p);
+                  : launch_ex(attend_kernel<T, D, NT>, dim3(ceil_div(plan.rows, L::kRows), p.cache.heads, p.seqs), block,
+                              L::kBytes, 1, st, "attend_kernel", p);
     }
-    int rc = allow_smem<attend_split_kernel<T, D>>("attend_split_kernel", smem);
-    if (!rc)
-        rc = launch_ex(attend_split_kernel<T, D>, dim3(ctas), dim3(kAttnWarps * 32), smem, 1, st, "attend_split_kernel", p);
-    return rc ? rc : launch_ex(attend_join_kernel<T, D>, dim3(ctas, ceil_div(max_rows < 16 ? max_rows : 16, kJoinRows)),
-                               dim3(kJoinRows * kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
+    int rc = allow_smem<attend_split_kernel<T, D, NT>>("attend_split_kernel", L::kBytes);
+    if (!rc) rc = launch_ex(attend_split_kernel<T, D, NT>, dim3(plan.ctas), block, L::kBytes, 1, st, "attend_split_kernel", p);
+    const int rows = plan.rows < L::kRows ? plan.rows : L::kRows;
+    return rc ? rc
+              : launch_ex(attend_join_kernel<T, D, NT>, dim3(plan.ctas, ceil_div(rows, kJoinRows)),
+                          dim3(kJoinRows * kJoinWarps * 32), 0, 1, st, "attend_join_kernel", p);
 }
 
 int check_cache(const char *what, const tans_b200_kv4 *c, Cache *out) {
@@ -1317,20 +1392,6 @@ int check_attention(const tans_b200_kv4 *cache, Cache *c, int64_t q_heads, int64
     return TANS_B200_OK;
 }
 
-// CTAs of the split form, 0 for the whole form.
-int plan_attention(const Cache &c, int64_t q_heads, int64_t max_pages, int64_t seqs, int64_t most_new, int64_t window,
-                   int *ctas) {
-    int sms;
-    const int rc = current_sms("kv4_attention", &sms);
-    if (rc) return rc;
-    *ctas = split_ctas(c, max_pages, seqs, ceil_div<int64_t>(most_new * (q_heads / c.heads), 16), window, most_new, sms);
-    return TANS_B200_OK;
-}
-
-int64_t workspace_floats(int64_t dim) {
-    return dim == 64 ? split_floats<64>() : (dim == 128 ? split_floats<128>() : split_floats<256>());
-}
-
 }  // namespace
 
 extern "C" int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cache, int64_t q_heads, int64_t max_pages,
@@ -1339,11 +1400,11 @@ extern "C" int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cach
     clear_error();
     if (!bytes) return fail(TANS_B200_ERR_INVALID, "kv4_attention: null pointer");
     Cache c;
-    int ctas = 0;
+    Plan plan;
     int rc = check_attention(cache, &c, q_heads, max_pages, seqs, tokens, most_new, window);
-    if (!rc) rc = plan_attention(c, q_heads, max_pages, seqs, most_new, window, &ctas);
+    if (!rc) rc = make_plan(c, q_heads, max_pages, seqs, most_new, window, &plan);
     if (rc) return rc;
-    *bytes = ctas * workspace_floats(cache->dim) * 4;
+    *bytes = plan.floats * 4;
     return TANS_B200_OK;
 }
 
@@ -1356,7 +1417,7 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     clear_error();
     if (tokens == 0 || seqs == 0) return TANS_B200_OK;
     AttendArgs p{};
-    int ctas = 0;
+    Plan plan;
     int rc = check_attention(cache, &p.cache, q_heads, max_pages, seqs, tokens, most_new, window);
     if (rc) return rc;
     if (!starts && tokens != seqs)
@@ -1364,9 +1425,9 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     if (!q || !out || !lens || (!table && max_pages) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_attention: q, out (16-byte aligned, q's stride a multiple of 8), lens and table are needed");
-    rc = plan_attention(p.cache, q_heads, max_pages, seqs, most_new, window, &ctas);
+    rc = make_plan(p.cache, q_heads, max_pages, seqs, most_new, window, &plan);
     if (rc) return rc;
-    if (workspace_bytes < ctas * workspace_floats(cache->dim) * 4 || (ctas && (!workspace || !is_aligned(workspace, 16))))
+    if (workspace_bytes < plan.floats * 4 || (plan.ctas && (!workspace || !is_aligned(workspace, 16))))
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: the workspace is too small or not 16-byte aligned");
     p.q = q;
     p.q_stride = q_stride;
@@ -1382,17 +1443,13 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     p.group = (int32_t)(q_heads / p.cache.heads);
     p.max_pages = (int32_t)max_pages;
     p.most_new = (int32_t)most_new;
+    p.tile_rows = plan.tile_rows;
     p.window = window > INT32_MAX - 1 ? 0 : (int32_t)window;
     p.scale = scale;
     p.status = status;
-    const int rows = (int)(most_new * p.group);
     return dispatch_half(dtype, "kv4_attention", [&](auto t) {
-        using T = decltype(t);
-        cudaStream_t st = (cudaStream_t)stream;
-        switch (cache->dim) {
-            case 64: return launch_attend<T, 64>(p, rows, ctas, st);
-            case 128: return launch_attend<T, 128>(p, rows, ctas, st);
-            default: return launch_attend<T, 256>(p, rows, ctas, st);
-        }
+        return dispatch_tile(cache->dim, plan.tile_rows, [&](auto d, auto nt) {
+            return launch_attend<decltype(t), decltype(d)::value, decltype(nt)::value>(p, plan, (cudaStream_t)stream);
+        });
     });
 }
