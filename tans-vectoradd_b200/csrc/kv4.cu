@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //   lse = log(sum(exp(S)));  no visible key: O = 0, lse = -inf.
 //
 // The rows of one KV head are its new tokens times the query heads that share
-// it (row = token * group + head in group); 8, 16 or 32 of them make a tile.
+// it (row = token * group + head in group); 8 or 16 of them make a tile.
 // The keys of a (sequence, head, tile) are cut into units of 128, 32 for each of
 // a CTA's four warps, which keep a running maximum and sum each and join at
 // the end.
@@ -330,10 +330,10 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 // an N of 8 and half the MMAs, sums and exponentials that an M of 16 would
 // (batch of 64, group 4: 93 us with rows as M).
 //
-// A block's codes and scales lie together in its page, so four bulk copies
-// bring it (eight with pages of 16), the next block's while one is worked on;
-// with smaller pages the lanes load a key each.  From shared memory they go to
-// MMA operands in registers:
+// The codes and the scales of a head lie together in a page, so a unit comes by
+// four bulk copies a page, asked for by the warps in turn while the unit before
+// it is worked on; with pages under 16 tokens the lanes load a key each.  From
+// shared memory they go to MMA operands in registers:
 //  * S^T: the contraction runs over D in any order, so lane (g, t) takes keys g
 //    and g + 8 of 16 and the t-th quarter of their D codes, D/8 contiguous
 //    bytes; step j uses codes 4j .. 4j+3 of that quarter, and the Q fragments
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 constexpr int kAttnWarps = 4;
 constexpr int kBlockKeys = 32;                  // keys a warp takes at a time
 constexpr int kUnit = kBlockKeys * kAttnWarps;  // keys
-constexpr int kStages = 2;                      // blocks in a warp's ring: one in work, one on its way
+constexpr int kStages = 2;                      // units in shared memory: one in work, one on its way
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
@@ -366,7 +366,7 @@ struct AttendArgs {
     float *lse;            // [tokens][q_heads], may be null
     float *parts;          // workspace of a split launch, else null
     int32_t tokens, seqs, group, max_pages, most_new, window;
-    int32_t tile_rows;     // 8, 16 or 32
+    int32_t tile_rows;     // 8 or 16
     float scale;           // softmax scale
     int32_t *status;
 };
@@ -469,15 +469,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
 template <int D, int NT>
 struct AttnLayout {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kCodes = kBlockKeys * D / 2, kScales = kBlockKeys * D / 16;  // bytes of a block
-    static constexpr int kBlock = 2 * (kCodes + kScales);            // K codes, V codes, K scales, V scales
-    static constexpr int kRing = kAttnWarps * kStages * kBlock;
+    static constexpr int kCodes = kUnit * D / 2, kScales = kUnit * D / 16;  // bytes of a unit
+    static constexpr int kStage = 2 * (kCodes + kScales);            // K codes, V codes, K scales, V scales
+    static constexpr int kRing = kStages * kStage;
     static constexpr int kEighth = D / 8 + 2;                        // floats of an eighth of a row of O
     static constexpr int kRow = 8 * kEighth + 4;                     // of a row: no bank conflicts
     static constexpr int kMerge = kAttnWarps * kRows * (kRow + 2) * 4;  // the warps' O, maxima and sums
     static constexpr int kQ = NT * D * 16;                           // Q fragments
     static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kQ + kRows * 4;
-    static constexpr int kCtas = D == 256 ? 2 : (NT == 4 ? 2 : (NT == 2 ? 4 : 5));  // resident on an SM
+    static constexpr int kCtas = D == 256 ? 2 : (NT == 2 ? 3 : 5);  // resident on an SM
     static constexpr int kPart = kRows * (D + 2);                    // floats of a partial result
     // place of element e in a merged row
     static __device__ int place(int e) { return e / (D / 8) * kEighth + e % (D / 8); }
@@ -490,7 +490,7 @@ struct Piece {
     int k0, k1;  // keys, multiples of kUnit
     // keys that some row of the tile sees, and those that every row sees
     int lo_all, hi_all, lo_in, hi_in;
-    int hi[32];  // the last key that each row sees
+    int hi[16];  // the last key that each row sees
 };
 
 __device__ __forceinline__ int first_seen(const AttendArgs &p, int last) {
@@ -502,7 +502,7 @@ __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
     const int lane = threadIdx.x & 31;
     const int end = min(x.row0 + p.tile_rows, x.q.news * p.group) - 1;
     const auto last_key = [&](int row) { return x.q.len - x.q.news + row / p.group; };
-    x.hi[lane] = last_key(min(x.row0 + lane, end));
+    if (lane < 16) x.hi[lane] = last_key(min(x.row0 + lane, end));
     if (lane == 0) {
         x.hi_in = last_key(x.row0);
         x.hi_all = last_key(end);
@@ -513,100 +513,98 @@ __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
     }
 }
 
-// Runs a piece (set by the caller, before a block barrier).  s_bars: the rings'
-// barriers, whose parities this warp keeps in `phases`.  Afterwards the four
+// Runs a piece (set by the caller, before a block barrier).  s_bars: for each
+// stage the barrier of its copies, then for each the barrier of its readers;
+// unit_no counts the CTA's units, for their parities.  Afterwards the four
 // warps' results lie in `smem` as [warp][kRows][kRow] O, [warp][kRows] maxima and sums.
 template <typename T, int D, int NT>
 __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem, uint64_t *s_bars,
-                                             uint32_t &phases) {
+                                             uint32_t &unit_no) {
     using L = AttnLayout<D, NT>;
     constexpr int kSteps = D / 16;        // MMA steps of S
     constexpr int kTiles = D / 16;        // MMA row tiles of O
     constexpr int kE = D / 8;             // elements of an eighth of a head
     constexpr int kVS = (D + 127) / 128;  // scales of an eighth
     constexpr int kKS = D / 64;           // scales of a quarter
-    constexpr int kTogether = NT > 1 ? 1 : 2;  // halves of 16 keys worked on together
+    constexpr int kTogether = 2;  // halves of 16 keys worked on together
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int head = x.head, k1 = x.k1, lo_all = x.lo_all;
     const int kend = min(x.hi_all, k1 - 1);  // the piece's last key
-    uint8_t *ring = smem + warp * (kStages * L::kBlock);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ - L::kRows * 4);
     float *factors = reinterpret_cast<float *>(smem + L::kBytes - L::kRows * 4);
 
-    // ---- copies of the warp's blocks into its ring
+    // ---- copies of a unit: lane 4 r + a brings array a (K codes, V codes, K
+    // scales, V scales) of the r-th page, or of all keys where a page holds them
     const int page_log2 = p.cache.page_log2, in_page = (1 << page_log2) - 1;
+    const bool bulk = page_log2 >= 4;
     const int32_t *table = p.table + (int64_t)x.seq * p.table_stride;
-    const int64_t head_at = (int64_t)head << page_log2;
+    const uint64_t head_at = (uint64_t)head << page_log2;
     const uint32_t page_tokens = (uint32_t)p.cache.heads << page_log2;
-    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(ring);
-    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(s_bars) + 8u * kStages * warp;
-    const auto page_at = [&](int key) {  // of a key within the piece
-        int page = table[key >> page_log2];
-        if ((uint32_t)page >= (uint32_t)p.cache.pages) {
+    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(smem), bars = (uint32_t)__cvta_generic_to_shared(s_bars);
+    const int run = min(kUnit, 1 << page_log2), run_at = (lane >> 2) * run;
+    const bool copies = bulk && run_at < kUnit;
+    // the page of this lane's run of the unit at `base`; keys outside the piece
+    // stand for the nearest inside it
+    const auto page_of = [&](int unit) -> uint32_t {
+        return copies && unit < k1 ? (uint32_t)table[max(lo_all, min(unit + run_at, kend)) >> page_log2] : 0u;
+    };
+    const auto issue = [&](int unit, uint32_t page, uint32_t no) {  // the no-th unit of this CTA
+        const int st = no % kStages;
+        // its place was read by all four warps in unit no - 2
+        if (no >= kStages) wait_copies(bars + 8u * (kStages + st), (no / kStages + 1) & 1, p.status);
+        const uint32_t bar = bars + 8u * st;
+        if (lane == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(L::kStage) : "memory");
+        if (copies) {
+            if (page >= (uint32_t)p.cache.pages) {
+                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+                page = 0;
+            }
+            const bool codes = !(lane & 2);
+            const uint32_t bytes = codes ? D / 2 : D / 16;  // of a key
+            const uint8_t *src = codes ? (lane & 1 ? p.cache.v_codes : p.cache.k_codes)
+                                       : (lane & 1 ? p.cache.v_scales : p.cache.k_scales);
+            copy_bulk(ring_sa + st * L::kStage + (codes ? (lane & 1) * L::kCodes : 2 * L::kCodes + (lane & 1) * L::kScales) +
+                          run_at * bytes,
+                      src + (head_at + (uint64_t)page * page_tokens + (uint32_t)((unit + run_at) & in_page)) * bytes,
+                      run * bytes, bar);
+        }
+    };
+    // pages under 16: this warp's 32 keys from `base`, one a lane
+    const auto load_block = [&](int base, uint8_t *at) {
+        const int key = base + lane;
+        const bool real = key >= lo_all && key <= kend;
+        uint32_t page = real ? (uint32_t)table[key >> page_log2] : 0u;
+        if (page >= (uint32_t)p.cache.pages) {
             if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
             page = 0;
         }
-        return (uint32_t)page;
-    };
-    const uint64_t page_first = (uint64_t)head_at;  // this head's first token in a page
-    const auto fetch = [&](int base, uint32_t page0, uint32_t page1, int stage) {
-        if (base >= k1) return;
-        const uint32_t bar = bars + 8u * stage, to = ring_sa + stage * L::kBlock;
-        if (page_log2 >= 4) {
-            if (lane == 0) {
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(L::kBlock) : "memory");
-                const auto copy = [&](uint32_t page, int first, uint32_t keys) {
-                    const uint64_t tok = page_first + (uint64_t)page * page_tokens + (uint32_t)((base + first) & in_page);
-                    copy_bulk(to + first * (D / 2), p.cache.k_codes + tok * (D / 2), keys * (D / 2), bar);
-                    copy_bulk(to + L::kCodes + first * (D / 2), p.cache.v_codes + tok * (D / 2), keys * (D / 2), bar);
-                    copy_bulk(to + 2 * L::kCodes + first * (D / 16), p.cache.k_scales + tok * (D / 16), keys * (D / 16), bar);
-                    copy_bulk(to + 2 * L::kCodes + L::kScales + first * (D / 16), p.cache.v_scales + tok * (D / 16),
-                              keys * (D / 16), bar);
-                };
-                if (page_log2 >= 5) {
-                    copy(page0, 0, 32);
-                } else {
-                    copy(page0, 0, 16);
-                    copy(page1, 16, 16);
-                }
-            }
-        } else {  // smaller pages: a lane brings one key itself
-            const int key = base + lane;
-            const bool real = key >= lo_all && key <= kend;
-            const int64_t tok = real ? head_at + (int64_t)page_at(key) * page_tokens + (key & in_page) : 0;
-            uint8_t *at = ring + stage * L::kBlock;
+        const uint64_t tok = head_at + (uint64_t)page * page_tokens + (uint32_t)(key & in_page);
+        const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll 1
-            for (int i = 0; i < D / 32; i++) {
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4 *>(at + lane * (D / 2) + 16 * i) =
-                    real ? *reinterpret_cast<const uint4 *>(p.cache.k_codes + tok * (D / 2) + 16 * i) : zero;
-                *reinterpret_cast<uint4 *>(at + L::kCodes + lane * (D / 2) + 16 * i) =
-                    real ? *reinterpret_cast<const uint4 *>(p.cache.v_codes + tok * (D / 2) + 16 * i) : zero;
-            }
-#pragma unroll 1
-            for (int i = 0; i < D / 64; i++) {
-                uint32_t *ks = reinterpret_cast<uint32_t *>(at + 2 * L::kCodes + lane * (D / 16) + 4 * i);
-                ks[0] = real ? *reinterpret_cast<const uint32_t *>(p.cache.k_scales + tok * (D / 16) + 4 * i) : 0u;
-                ks[L::kScales / 4] = real ? *reinterpret_cast<const uint32_t *>(p.cache.v_scales + tok * (D / 16) + 4 * i) : 0u;
-            }
-            __syncwarp();
-            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+        for (int i = 0; i < D / 32; i++) {
+            uint4 *to = reinterpret_cast<uint4 *>(at + lane * (D / 2) + 16 * i);
+            to[0] = real ? *reinterpret_cast<const uint4 *>(p.cache.k_codes + tok * (D / 2) + 16 * i) : zero;
+            to[L::kCodes / 16] = real ? *reinterpret_cast<const uint4 *>(p.cache.v_codes + tok * (D / 2) + 16 * i) : zero;
         }
-    };
-    // the pages of a block's first and last 16 keys, asked for a block ahead of
-    // their use; a key outside the piece stands for the nearest inside it
-    const auto pages_of = [&](int base, uint32_t &page0, uint32_t &page1) {
-        if (page_log2 < 4 || base >= k1) return;
-        page0 = page_at(max(lo_all, min(base, kend)));
-        if (page_log2 == 4) page1 = page_at(max(lo_all, min(base + 16, kend)));
+#pragma unroll 1
+        for (int i = 0; i < D / 64; i++) {
+            uint32_t *to = reinterpret_cast<uint32_t *>(at + 2 * L::kCodes - warp * kBlockKeys * (D / 2 - D / 16) +
+                                                        lane * (D / 16) + 4 * i);
+            to[0] = real ? *reinterpret_cast<const uint32_t *>(p.cache.k_scales + tok * (D / 16) + 4 * i) : 0u;
+            to[L::kScales / 4] = real ? *reinterpret_cast<const uint32_t *>(p.cache.v_scales + tok * (D / 16) + 4 * i) : 0u;
+        }
     };
     // what was written here by ordinary stores comes before the copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    int base = x.k0 + kBlockKeys * warp;
-    uint32_t page0 = 0, page1 = 0;
-    pages_of(base, page0, page1);
-    fetch(base, page0, page1, 0);
-    pages_of(base + kUnit, page0, page1);
+    // unit `no` is asked for by warp no % 4, whose pages for it were loaded when
+    // it asked for the one before
+    const uint32_t first_no = unit_no;
+    uint32_t page = page_of(x.k0 + (int)((warp - first_no) & 3u) * kUnit);
+    if (bulk && x.k0 < k1 && (first_no & 3u) == (uint32_t)warp) {
+        issue(x.k0, page, first_no);
+        page = page_of(x.k0 + 4 * kUnit);
+    }
 
     // ---- Q: steps 2i and 2i + 1, lane (g, t): elements 8i .. 8i + 7 of quarter t of
     // row g.  A row's factor brings its scores to base 2; it is positive: its sign
@@ -670,17 +668,25 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     // Of eight keys the m-th is m ^ (m >> 1 & 1): the V reads of lanes t = 0..3
     // then fall on rows of both parities.
     const int own_key = g ^ (g >> 1 & 1);
-    int stage = 0;
 #pragma unroll 1
-    for (; base < k1; base += kUnit) {
-        fetch(base + kUnit, page0, page1, stage ^ 1);  // the next block, into the other place
-        pages_of(base + 2 * kUnit, page0, page1);
-        wait_copies(bars + 8u * stage, phases >> stage & 1, p.status);
-        phases ^= 1u << stage;
-        const uint8_t *blk = ring + stage * L::kBlock;
-        stage ^= 1;
+    for (int unit = x.k0; unit < k1; unit += kUnit, unit_no++) {
+        const int base = unit + kBlockKeys * warp, st = unit_no % kStages;
+        uint8_t *const stage = smem + st * L::kStage;
+        // this warp's keys of the unit: codes and, from `scales` on, scales
+        uint8_t *const blk = stage + warp * kBlockKeys * (D / 2);
+        const uint8_t *const scales = stage + 2 * L::kCodes + warp * kBlockKeys * (D / 16);
+        if (bulk) {
+            if (unit + kUnit < k1 && ((unit_no + 1) & 3u) == (uint32_t)warp) {
+                issue(unit + kUnit, page, unit_no + 1);
+                page = page_of(unit + 5 * kUnit);
+            }
+            wait_copies(bars + 8u * st, unit_no / kStages & 1, p.status);
+        } else {
+            load_block(base, blk);
+            __syncwarp();
+        }
         const bool edge = base < inner || base - inner > inner_span;
-#pragma unroll
+#pragma unroll(2 / kTogether)
         for (int y0 = 0; y0 < 2; y0 += kTogether) {
             // ---- scores of the keys base + 16 y ..
             float s[kTogether][NT][4];
@@ -701,7 +707,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                             w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
                         }
                     }
-                    const uint8_t *sp = blk + 2 * L::kCodes + r * (D / 16) + t * kKS;
+                    const uint8_t *sp = scales + r * (D / 16) + t * kKS;
                     if constexpr (kKS == 1) {
                         f[h][0] = e4m3x2_h2(*sp * 0x101u);
                     } else {
@@ -814,7 +820,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                     }
 #pragma unroll
                     for (int i = 0; i < kVS; i++)
-                        sc[k][i] = blk[2 * L::kCodes + L::kScales + r * (D / 16) + g * kE / 16 + i];
+                        sc[k][i] = scales[L::kScales + r * (D / 16) + g * kE / 16 + i];
                 }
                 // Keys outside the piece hold anything: their values count as 0.  A NaN
                 // scale on a key that only some rows see must not reach the others
@@ -885,7 +891,9 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                 }
             }
         }
-        __syncwarp();  // all lanes have read the block before its place is filled again
+        __syncwarp();  // all lanes have read their keys before the place is filled again
+        if (bulk && lane == 0)
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + 8u * (kStages + st)) : "memory");
     }
 
     // ---- the warps' results, side by side
@@ -972,8 +980,9 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, 
 
 // Called by all threads, before a block barrier.
 __device__ __forceinline__ void init_bars(uint64_t *bars) {
-    if (threadIdx.x < kAttnWarps * kStages)
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(bars + threadIdx.x)));
+    if (threadIdx.x < 2 * kStages)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(bars + threadIdx.x)),
+                     "r"(threadIdx.x < kStages ? 1 : kAttnWarps));
     asm volatile("fence.mbarrier_init.release.cluster;");
 }
 
@@ -983,8 +992,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
     __shared__ Piece x;
-    __shared__ __align__(8) uint64_t bars[kAttnWarps * kStages];
-    uint32_t phases = 0;
+    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    uint32_t unit_no = 0;
     init_bars(bars);
     const Sequence q = sequence(p, blockIdx.z);
     if ((int)blockIdx.x * p.tile_rows >= q.news * p.group) return;
@@ -999,7 +1008,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
         set_rows(p, x);
     }
     __syncthreads();
-    attend_piece<T, D, NT>(p, x, smem, bars, phases);
+    attend_piece<T, D, NT>(p, x, smem, bars, unit_no);
     join_warps<T, D, NT>(p, x, smem, nullptr);
 }
 
@@ -1029,8 +1038,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     __shared__ int found_seq, left, take;
     __shared__ bool begins;
     __shared__ Piece x;
-    __shared__ __align__(8) uint64_t bars[kAttnWarps * kStages];
-    uint32_t phases = 0;
+    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    uint32_t unit_no = 0;
     init_bars(bars);
     constexpr int kThreads = kAttnWarps * 32;
     pdl_enter();
@@ -1121,7 +1130,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
         }
         __syncthreads();
         if (take == 0) return;
-        attend_piece<T, D, NT>(p, x, smem, bars, phases);
+        attend_piece<T, D, NT>(p, x, smem, bars, unit_no);
         join_warps<T, D, NT>(p, x, smem,
                          begins && take == x.q.units ? nullptr
                                                      : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D, NT>::kPart : 0));
@@ -1196,17 +1205,11 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
 }
 
-// Rows of a tile.
-int rows_of_tile(int64_t rows, int64_t dim) { return rows <= 8 ? 8 : (rows <= 16 || dim == 256 ? 16 : 32); }
-
 // f(<D, NT>) for a head size and a tile's rows.
 template <typename F>
 auto dispatch_tile(int64_t dim, int tile_rows, F &&f) {
     const auto with = [&](auto d) {
-        if (tile_rows == 8) return f(d, std::integral_constant<int, 1>{});
-        if constexpr (decltype(d)::value != 256)
-            if (tile_rows == 32) return f(d, std::integral_constant<int, 4>{});
-        return f(d, std::integral_constant<int, 2>{});
+        return tile_rows == 8 ? f(d, std::integral_constant<int, 1>{}) : f(d, std::integral_constant<int, 2>{});
     };
     if (dim == 64) return with(std::integral_constant<int, 64>{});
     if (dim == 128) return with(std::integral_constant<int, 128>{});
@@ -1224,7 +1227,7 @@ int make_plan(const Cache &c, int64_t q_heads, int64_t max_pages, int64_t seqs, 
     const int rc = current_sms("kv4_attention", &sms);
     if (rc) return rc;
     plan->rows = (int)(most_new * (q_heads / c.heads));
-    plan->tile_rows = rows_of_tile(plan->rows, c.dim);
+    plan->tile_rows = plan->rows <= 8 ? 8 : 16;
     int64_t keys = max_pages << c.page_log2;
     if (window > 0 && window + most_new < keys) keys = window + most_new;
     const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
