@@ -1052,42 +1052,50 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
         const Sequence s = sequence(p, seq);
         return (int64_t)s.tiles * (s.units + kTileCost) * p.cache.heads;
     };
-    int64_t total = 0;
-    for (int b = tid; b < p.seqs; b += kThreads) total += units_of(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (lane == 0) warp_sum[warp] = total;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < kAttnWarps; w++) total += warp_sum[w];
-    const int64_t per = ceil_div<int64_t>(total, gridDim.x);
-    const int64_t u = per * blockIdx.x;
-    const int64_t u_end = u + per < total ? u + per : total;
-    if (u >= u_end) return;
-    // the sequence in which unit u lies, and that sequence's first unit
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.seqs; b0 += kThreads) {
-        const int64_t n = units_of(b0 + tid);
-        int64_t inc = n;
+    // Units of the 128 sequences from b0 on: this thread's own, those before it,
+    // and all of them.
+    struct Counted {
+        int64_t own, before, all;
+    };
+    const auto count = [&](int b0) {
+        Counted c{units_of(b0 + tid), 0, 0};
+        int64_t inc = c.own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        __syncthreads();
         if (lane == 31) warp_sum[warp] = inc;
         __syncthreads();
-        int64_t from = before + inc - n;
+        c.before = inc - c.own;
+#pragma unroll
         for (int w = 0; w < kAttnWarps; w++) {
-            if (w < warp) from += warp_sum[w];
-            before += warp_sum[w];
+            if (w < warp) c.before += warp_sum[w];
+            c.all += warp_sum[w];
         }
-        if (u >= from && u < from + n) {
-            found_seq = b0 + tid;
-            found_at = from;
+        return c;
+    };
+    const Counted first = count(0);
+    int64_t total = first.all;
+    for (int b0 = kThreads; b0 < p.seqs; b0 += kThreads) {
+        __syncthreads();
+        total += count(b0).all;
+    }
+    const int64_t per = ceil_div<int64_t>(total, gridDim.x);
+    const int64_t u = per * blockIdx.x;
+    const int64_t u_end = u + per < total ? u + per : total;
+    if (u >= u_end) return;
+    // the sequence in which unit u lies, and that sequence's first unit
+    Counted c = first;
+    for (int64_t b0 = 0, from = 0;; b0 += kThreads) {
+        if (u >= from + c.before && u < from + c.before + c.own) {
+            found_seq = (int)b0 + tid;
+            found_at = from + c.before;
         }
         __syncthreads();
-        if (u < before) break;
+        from += c.all;
+        if (u < from) break;
+        c = count((int)b0 + kThreads);
     }
     if (tid == 0) {
         x.seq = found_seq;
@@ -1107,7 +1115,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
                         x.q = sequence(p, ++x.seq);
                         continue;
                     }
-                    const int pair = (int)(at / span), pos = (int)(at - (int64_t)pair * span);
+                    const int pair = at <= INT32_MAX ? (int)((uint32_t)at / (uint32_t)span) : (int)(at / span);
+                    const int pos = (int)(at - (int64_t)pair * span);
                     const int step = min(left, span - pos);
                     at += step;
                     left -= step;
@@ -1141,65 +1150,69 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
 }
 
 // Joins the parts of a tile: part 1 of CTA c, then part 0 of the CTAs after
-// it.  A CTA takes four rows, four warps each that take turns at the parts;
-// the parts' factors come first, so that the loads of O wait for nothing.
+// it.  A CTA takes four rows, four warps each that take turns at the parts,
+// several at a time.
 constexpr int kJoinRows = 4, kJoinWarps = 4;
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel(const AttendArgs p) {
-    constexpr int kMost = 512;  // parts whose factors are kept at a time
-    __shared__ float factor[kJoinRows][kMost], o_of[kJoinRows][kJoinWarps][D];
+    constexpr int kAtATime = 768 / D;  // parts of a warp in flight; twice as many left no room for the next kernel
+    __shared__ float tops[kJoinRows][kJoinWarps], sums[kJoinRows][kJoinWarps], o_of[kJoinRows][kJoinWarps][D];
     pdl_enter();
     const float *at = p.parts + blockIdx.x * split_floats<D, NT>();
     const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
     const int slot = threadIdx.x >> 7, turn = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31;
     const int r = blockIdx.y * kJoinRows + slot;
     if (h.pieces == 0 || (int)blockIdx.y * kJoinRows >= h.rows) return;
-    const auto part = [&](int i) {
-        return at + i * split_floats<D, NT>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D, NT>::kPart);
-    };
     const bool real = r < h.rows;
     float m = -INFINITY, l = 0.f, v[D / 32] = {};
-    for (int i = lane; real && i < h.pieces; i += 32) m = fmaxf(m, part(i)[8 * NT * D + r]);
+    for (int i0 = turn; real && i0 < h.pieces; i0 += kAtATime * kJoinWarps) {
+        float top[kAtATime], sum[kAtATime], o[kAtATime][D / 32];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    for (int i0 = 0; i0 < h.pieces; i0 += kMost) {
-        const int n = min(kMost, h.pieces - i0);
-        __syncthreads();
-        for (int i = turn * 32 + lane; real && i < n; i += kJoinWarps * 32) {
-            const float s = part(i0 + i)[8 * NT * (D + 1) + r], f = part_factor(part(i0 + i)[8 * NT * D + r], s, m);
-            factor[slot][i] = f;
-            l += f * s;
-        }
-        __syncthreads();
-        if (real) {
-#pragma unroll 8
-            for (int i = turn; i < n; i += kJoinWarps) {
-                const float *o = part(i0 + i) + r * D + lane;
-                const float f = factor[slot][i];
+        for (int k = 0; k < kAtATime; k++) {
+            const int i = i0 + k * kJoinWarps;
+            top[k] = -INFINITY, sum[k] = 0.f;
+            if (i < h.pieces) {
+                const float *part = at + i * split_floats<D, NT>() + sizeof(SplitHead) / 4 + (i ? 0 : AttnLayout<D, NT>::kPart);
+                top[k] = part[8 * NT * D + r];
+                sum[k] = part[8 * NT * (D + 1) + r];
 #pragma unroll
-                for (int e = 0; e < D / 32; e++) {
-                    const float x = o[32 * e];
-                    v[e] += f == 0.f ? 0.f : f * x;
-                }
+                for (int e = 0; e < D / 32; e++) o[k][e] = part[r * D + lane + 32 * e];
             }
         }
-    }
+        float n = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        for (int k = 0; k < kAtATime; k++) n = fmaxf(n, top[k]);
+        const float old = part_factor(m, l, n);
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) v[e] *= old;
+#pragma unroll
+        for (int k = 0; k < kAtATime; k++) {
+            const float f = part_factor(top[k], sum[k], n);
+            if (f == 0.f && sum[k] == sum[k]) continue;  // nothing, or too far below to count; a NaN goes on
+            l += f * sum[k];
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) v[e] += f * o[k][e];
+        }
+        m = n;
+    }
+    if (lane == 0) tops[slot][turn] = m, sums[slot][turn] = l;
 #pragma unroll
     for (int e = 0; e < D / 32; e++) o_of[slot][turn][lane + 32 * e] = v[e];
     __syncthreads();
-    if (lane == 0) factor[slot][turn] = l;
-    __syncthreads();
     if (turn || !real) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; w++) m = fmaxf(m, tops[slot][w]);
     l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; w++) l += factor[slot][w];
+    for (int e = 0; e < D / 32; e++) v[e] = 0.f;
 #pragma unroll
-    for (int e = 0; e < D / 32; e++) {
-        v[e] = 0.f;
+    for (int w = 0; w < kJoinWarps; w++) {
+        const float f = part_factor(tops[slot][w], sums[slot][w], m);
+        l += f * sums[slot][w];
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; w++) v[e] += o_of[slot][w][lane + 32 * e];
+        for (int e = 0; e < D / 32; e++) v[e] += f == 0.f ? 0.f : f * o_of[slot][w][lane + 32 * e];
     }
     const int row = h.row0 + r;
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
