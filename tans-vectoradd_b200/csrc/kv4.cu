@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //
 // The codes and the scales of a head lie together in a page, so a unit comes by
 // four bulk copies a page, asked for by the warps in turn while the unit before
-// it is worked on; with pages under 16 tokens the lanes load a key each.  From
+// it is worked on; with pages under 16 tokens every lane copies a key.  From
 // shared memory they go to MMA operands in registers:
 //  * S^T: the contraction runs over D in any order, so lane (g, t) takes keys g
 //    and g + 8 of 16 and the t-th quarter of their D codes, D/8 contiguous
@@ -401,6 +401,17 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs &p, int seq) {
     s.tiles = ceil_div(s.news * p.group, p.tile_rows);
     s.units = max(1, ceil_div(s.hi + 1 - (s.lo & ~(kUnit - 1)), kUnit));
     return s;
+}
+
+// Asynchronous copy of 4, 8 or 16 bytes; zeros in the place of what is not real (then src is not read).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t *src, bool real) {
+    const int n = real ? BYTES : 0;
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
+                     : "memory");
 }
 
 // Bulk copy of `bytes` (a multiple of 16, both ends aligned) into shared memory, counted on `bar`.
@@ -570,40 +581,48 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                       run * bytes, bar);
         }
     };
-    // pages under 16: this warp's 32 keys from `base`, one a lane
-    const auto load_block = [&](int base, uint8_t *at) {
-        const int key = base + lane;
-        const bool real = key >= lo_all && key <= kend;
-        uint32_t page = real ? (uint32_t)table[key >> page_log2] : 0u;
-        if (page >= (uint32_t)p.cache.pages) {
-            if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
-            page = 0;
+    // pages under 16: a lane copies one of its warp's keys, a unit ahead as well;
+    // what is not a key of the piece becomes zeros
+    const auto copy_key = [&](int unit, uint32_t page, uint32_t no) {
+        if (unit < k1) {
+            const int key = unit + kBlockKeys * warp + lane;
+            const bool real = key >= lo_all && key <= kend;
+            if (page >= (uint32_t)p.cache.pages) {
+                if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
+                page = 0;
+            }
+            const uint64_t tok = head_at + (uint64_t)page * page_tokens + (uint32_t)(key & in_page);
+            const uint32_t to = ring_sa + no % kStages * L::kStage + (kBlockKeys * warp + lane) * (D / 2);
+            const uint32_t to_s = ring_sa + no % kStages * L::kStage + 2 * L::kCodes + (kBlockKeys * warp + lane) * (D / 16);
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                copy_async<16>(to + 16 * i, p.cache.k_codes + tok * (D / 2) + 16 * i, real);
+                copy_async<16>(to + L::kCodes + 16 * i, p.cache.v_codes + tok * (D / 2) + 16 * i, real);
+            }
+            copy_async<D / 16>(to_s, p.cache.k_scales + tok * (D / 16), real);
+            copy_async<D / 16>(to_s + L::kScales, p.cache.v_scales + tok * (D / 16), real);
         }
-        const uint64_t tok = head_at + (uint64_t)page * page_tokens + (uint32_t)(key & in_page);
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 1
-        for (int i = 0; i < D / 32; i++) {
-            uint4 *to = reinterpret_cast<uint4 *>(at + lane * (D / 2) + 16 * i);
-            to[0] = real ? *reinterpret_cast<const uint4 *>(p.cache.k_codes + tok * (D / 2) + 16 * i) : zero;
-            to[L::kCodes / 16] = real ? *reinterpret_cast<const uint4 *>(p.cache.v_codes + tok * (D / 2) + 16 * i) : zero;
-        }
-#pragma unroll 1
-        for (int i = 0; i < D / 64; i++) {
-            uint32_t *to = reinterpret_cast<uint32_t *>(at + 2 * L::kCodes - warp * kBlockKeys * (D / 2 - D / 16) +
-                                                        lane * (D / 16) + 4 * i);
-            to[0] = real ? *reinterpret_cast<const uint32_t *>(p.cache.k_scales + tok * (D / 16) + 4 * i) : 0u;
-            to[L::kScales / 4] = real ? *reinterpret_cast<const uint32_t *>(p.cache.v_scales + tok * (D / 16) + 4 * i) : 0u;
-        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const auto key_page = [&](int unit) -> uint32_t {
+        const int key = unit + kBlockKeys * warp + lane;
+        return unit < k1 && key >= lo_all && key <= kend ? (uint32_t)table[key >> page_log2] : 0u;
     };
     // what was written here by ordinary stores comes before the copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     // unit `no` is asked for by warp no % 4, whose pages for it were loaded when
     // it asked for the one before
     const uint32_t first_no = unit_no;
-    uint32_t page = page_of(x.k0 + (int)((warp - first_no) & 3u) * kUnit);
-    if (bulk && x.k0 < k1 && (first_no & 3u) == (uint32_t)warp) {
-        issue(x.k0, page, first_no);
-        page = page_of(x.k0 + 4 * kUnit);
+    uint32_t page;
+    if (bulk) {
+        page = page_of(x.k0 + (int)((warp - first_no) & 3u) * kUnit);
+        if (x.k0 < k1 && (first_no & 3u) == (uint32_t)warp) {
+            issue(x.k0, page, first_no);
+            page = page_of(x.k0 + 4 * kUnit);
+        }
+    } else {
+        copy_key(x.k0, key_page(x.k0), first_no);
+        page = key_page(x.k0 + kUnit);
     }
 
     // ---- Q: steps 2i and 2i + 1, lane (g, t): elements 8i .. 8i + 7 of quarter t of
@@ -671,9 +690,9 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
 #pragma unroll 1
     for (int unit = x.k0; unit < k1; unit += kUnit, unit_no++) {
         const int base = unit + kBlockKeys * warp, st = unit_no % kStages;
-        uint8_t *const stage = smem + st * L::kStage;
+        const uint8_t *const stage = smem + st * L::kStage;
         // this warp's keys of the unit: codes and, from `scales` on, scales
-        uint8_t *const blk = stage + warp * kBlockKeys * (D / 2);
+        const uint8_t *const blk = stage + warp * kBlockKeys * (D / 2);
         const uint8_t *const scales = stage + 2 * L::kCodes + warp * kBlockKeys * (D / 16);
         if (bulk) {
             if (unit + kUnit < k1 && ((unit_no + 1) & 3u) == (uint32_t)warp) {
@@ -682,7 +701,9 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
             }
             wait_copies(bars + 8u * st, unit_no / kStages & 1, p.status);
         } else {
-            load_block(base, blk);
+            copy_key(unit + kUnit, page, unit_no + 1);
+            page = key_page(unit + 2 * kUnit);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncwarp();
         }
         const bool edge = base < inner || base - inner > inner_span;
