@@ -262,13 +262,51 @@ __global__ void __launch_bounds__(256, 4) append_kernel(const AppendArgs p) {
 
 // --------------------------------------------------------------------- read
 
+// Heads h0 .. h1 - 1 of a token's keys or values, this thread's eight elements
+// of each (codes and scales: those of head 0), four heads' loads at a time.
+template <typename T>
+__device__ __forceinline__ void read_heads(const uint8_t *codes, const uint8_t *scales, const float *gain, T *out, int h0,
+                                           int h1, int64_t code_step, int dim, bool real) {
+    constexpr int kAtATime = 4;
+    codes += h0 * code_step;
+    scales += h0 * (code_step / 8);
+    out += (int64_t)h0 * dim;
+    for (int h = h0; h < h1; h += kAtATime) {
+        uint32_t w[kAtATime], e[kAtATime];
+#pragma unroll
+        for (int b = 0; b < kAtATime; b++) {
+            w[b] = e[b] = 0;
+            if (real && h + b < h1) {
+                w[b] = *reinterpret_cast<const uint32_t *>(codes + b * code_step);
+                e[b] = scales[b * (code_step / 8)];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kAtATime; b++) {
+            if (h + b >= h1) break;
+            const float s = e4m3_f32(e[b]) * (gain ? gain[h + b] : 1.f);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t h2 = e2m1x2_f16(w[b] >> (8 * j) & 0xFFu);
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
+                x[2 * j] = f.x * s;
+                x[2 * j + 1] = f.y * s;
+            }
+            store8(out + b * dim, x);
+        }
+        codes += kAtATime * code_step;
+        scales += kAtATime * (code_step / 8);
+        out += kAtATime * dim;
+    }
+}
+
 // k, v [tokens][heads][D] from the cache's slots; a negative slot gives zeros.
 // A thread has eight elements of one token, for `per` of its key and value
-// heads, four heads' loads at a time.
+// heads (16383 tokens of 8 x 128: 15 us, 5.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t *slots, T *k, T *v, int32_t tokens,
                                                    int32_t groups_log2, int32_t per, int32_t *status) {
-    constexpr int kAtATime = 4;
     pdl_enter();
     const int i = blockIdx.x * 256 + threadIdx.x;
     const int token = i >> groups_log2, group = i & ((1 << groups_log2) - 1);
@@ -278,40 +316,17 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
         if (status) atomicOr(status, TANS_B200_DATA_BAD_INDEX);
         slot = -1;
     }
-    const int64_t at0 = slot < 0 ? 0
-                                 : (token_at(c, slot >> c.page_log2, 0, (int)(slot & ((1 << c.page_log2) - 1))) << groups_log2) + group;
-    const int64_t head_step = (int64_t)1 << (c.page_log2 + groups_log2);
-    const int h1 = min(2 * c.heads, ((int)blockIdx.y + 1) * per);
-    for (int h0 = blockIdx.y * per; h0 < h1; h0 += kAtATime) {
-        uint32_t codes[kAtATime], scale[kAtATime];
-#pragma unroll
-        for (int b = 0; b < kAtATime; b++) {
-            const int h = h0 + b;
-            codes[b] = scale[b] = 0;
-            if (h >= h1 || slot < 0) continue;
-            const int64_t at = at0 + (h < c.heads ? h : h - c.heads) * head_step;
-            codes[b] = reinterpret_cast<const uint32_t *>(h < c.heads ? c.k_codes : c.v_codes)[at];
-            scale[b] = (h < c.heads ? c.k_scales : c.v_scales)[at / 2];
-        }
-#pragma unroll
-        for (int b = 0; b < kAtATime; b++) {
-            const int h = h0 + b;
-            if (h >= h1) break;
-            const bool value = h >= c.heads;
-            const int head = value ? h - c.heads : h;
-            const float *gain = value ? c.v_gain : c.k_gain;
-            const float s = e4m3_f32(scale[b]) * (gain ? gain[head] : 1.f);
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t h2 = e2m1x2_f16(codes[b] >> (8 * j) & 0xFFu);
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
-                x[2 * j] = f.x * s;
-                x[2 * j + 1] = f.y * s;
-            }
-            store8((value ? v : k) + ((((int64_t)token * c.heads + head) << groups_log2) + group) * 8, x);
-        }
-    }
+    // in units of eight elements
+    const int64_t at = slot < 0 ? 0
+                                : (token_at(c, slot >> c.page_log2, 0, (int)(slot & ((1 << c.page_log2) - 1))) << groups_log2) + group;
+    const int64_t code_step = (int64_t)4 << (c.page_log2 + groups_log2), to = (((int64_t)token * c.heads) << groups_log2) + group;
+    const int h0 = blockIdx.y * per, h1 = min(2 * c.heads, h0 + per);
+    if (h0 < c.heads)
+        read_heads(c.k_codes + 4 * at, c.k_scales + at / 2, c.k_gain, k + 8 * to, h0, min(h1, c.heads), code_step, c.dim,
+                   slot >= 0);
+    if (h1 > c.heads)
+        read_heads(c.v_codes + 4 * at, c.v_scales + at / 2, c.v_gain, v + 8 * to, max(h0 - c.heads, 0), h1 - c.heads, code_step,
+                   c.dim, slot >= 0);
 }
 
 // ---------------------------------------------------------------- attention
