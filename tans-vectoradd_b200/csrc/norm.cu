@@ -14,6 +14,10 @@
 // One CTA a row, the row in registers between the reduction and the outputs:
 // every input is read once and every output written once, so the kernel is
 // bound by memory for many rows and by launch and reduction latency for few.
+// Measured on one B200, residual and e4m3 output: 16384 x 5120 bf16 95 us =
+// 6.2 TB/s (95 % of the copy rate); 1 x 5120 2.7 us among others in a graph.
+// All loads of a row come before the first use of one: 135 us with the
+// residual's after the sums of x began.
 
 #include "sm100.cuh"
 
@@ -65,25 +69,59 @@ __device__ __forceinline__ float row_factor(const NormArgs &p, float sumsq, floa
     return amax > 1e-30f && amax < 1e30f && top > 1e-30f ? 448.f / amax : inv / scale;
 }
 
-// Rows of whole 8-element vectors, 16-byte aligned everywhere: thread t holds
-// vectors t, t + blockDim, ...
-template <typename T, int VPT, int kMost>
+// Eight elements e0 .. e0 + 7 of a row of `cols`; at its ends, where some lie
+// outside (and count as 0, or stay unwritten), one by one.
+template <typename T>
+__device__ __forceinline__ Eight<T> load_part(const T *row, int e0, int cols) {
+    if (e0 >= 0 && e0 + 8 <= cols) return load_eight(row + e0);
+    Eight<T> r;
+    T *e = reinterpret_cast<T *>(r.u);
+#pragma unroll
+    for (int k = 0; k < 8; k++) e[k] = (unsigned)(e0 + k) < (unsigned)cols ? row[e0 + k] : from_f32<T>(0.f);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_part(T *row, int e0, int cols, const float (&v)[8]) {
+    if (e0 >= 0 && e0 + 8 <= cols) {
+        store8(row + e0, v);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if ((unsigned)(e0 + k) < (unsigned)cols) row[e0 + k] = from_f32<T>(v[k]);
+}
+
+// Rows by 8-element vectors on 16-byte boundaries: thread t holds vectors t, t +
+// blockDim, ...  kShifted: rows begin anywhere, x, residual, h and y alike; the
+// first vector begins at the boundary before the row, and the weight, which lies
+// to another, is read one by one.
+template <typename T, int VPT, int kMost, bool kShifted>
 __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     __shared__ float2 buf[32];
     pdl_enter();
     const int64_t row = blockIdx.x;
-    const int vecs = p.cols / 8;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
+    const int shift = kShifted ? (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % (16 / sizeof(T))) : 0;
+    const int vecs = kShifted ? (p.cols + shift + 7) / 8 : p.cols / 8;
+    const auto load = [&](const T *from, int v) {
+        return kShifted ? load_part(from, 8 * v - shift, p.cols) : load_eight(from + 8 * v);
+    };
+    const auto store = [&](T *to, int v, const float (&a)[8]) {
+        if constexpr (kShifted)
+            store_part(to, 8 * v - shift, p.cols, a);
+        else
+            store8(to + 8 * v, a);
+    };
     // every load of the row before the first use of one
     Eight<T> xv[VPT], rv[VPT], wv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < vecs) {
-            xv[i] = load_eight(x + 8 * v);
-            if (r) rv[i] = load_eight(r + 8 * v);
-            if (p.norm && !p.weight_f32) wv[i] = load_eight(static_cast<const T *>(p.weight) + 8 * v);
+            xv[i] = load(x, v);
+            if (r) rv[i] = load(r, v);
+            if (!kShifted && p.norm && !p.weight_f32) wv[i] = load_eight(static_cast<const T *>(p.weight) + 8 * v);
         }
     }
     float s[VPT][8];
@@ -98,14 +136,24 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
                 rv[i].to(a);
 #pragma unroll
                 for (int k = 0; k < 8; k++) s[i][k] += a[k];
-                store8(static_cast<T *>(p.h) + row * p.h_stride + 8 * v, s[i]);
+                store(static_cast<T *>(p.h) + row * p.h_stride, v, s[i]);
             }
             if (p.norm) {
                 float w[8];
-                if (p.weight_f32)
+                if constexpr (kShifted) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int e = 8 * v - shift + k;
+                        w[k] = (unsigned)e >= (unsigned)p.cols
+                                   ? 0.f
+                                   : (p.weight_f32 ? static_cast<const float *>(p.weight)[e]
+                                                   : to_f32(static_cast<const T *>(p.weight)[e]));
+                    }
+                } else if (p.weight_f32) {
                     load8(static_cast<const float *>(p.weight) + 8 * v, w);
-                else
+                } else {
                     wv[i].to(w);
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
                     sumsq = __fmaf_rn(s[i][k], s[i][k], sumsq);
@@ -132,15 +180,28 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
                 uint2 u;
                 u.x = e4m3x2(s[i][0], s[i][1]) | e4m3x2(s[i][2], s[i][3]) << 16;
                 u.y = e4m3x2(s[i][4], s[i][5]) | e4m3x2(s[i][6], s[i][7]) << 16;
-                *reinterpret_cast<uint2 *>(p.q + row * p.cols + 8 * v) = u;
+                uint8_t *q = p.q + row * p.cols;
+                const int e0 = 8 * v - shift;
+                if (!kShifted) {
+                    *reinterpret_cast<uint2 *>(q + e0) = u;
+                } else if (e0 >= 0 && e0 + 8 <= p.cols) {  // on a boundary of four
+                    reinterpret_cast<uint32_t *>(q + e0)[0] = u.x;
+                    reinterpret_cast<uint32_t *>(q + e0)[1] = u.y;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if ((unsigned)(e0 + k) < (unsigned)p.cols) q[e0 + k] = (uint8_t)((k < 4 ? u.x : u.y) >> (8 * (k & 3)));
+                }
             } else {
-                store8(static_cast<T *>(p.y) + row * p.cols + 8 * v, s[i]);
+                store(static_cast<T *>(p.y) + row * p.cols, v, s[i]);
             }
         }
     }
 }
 
-// Any width, stride and alignment: element by element, s * w kept in shared memory.
+// Wider rows, and rows of tensors that lie to 16-byte boundaries each in its own
+// way: element by element, s * w kept in shared memory (1021 x 4099 f16: 9.7 us
+// out of L2, where vectors take 8.4; bound by its 2-byte accesses).
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
     extern __shared__ float srow[];
@@ -180,30 +241,38 @@ constexpr int kMaxCols = 56 * 1024;  // f32 values of one row that fit a CTA's s
 
 template <typename T>
 int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
-    const auto vec_ok = [&](const void *ptr, int64_t stride) {
-        return !ptr || (is_aligned(ptr, 16) && stride % (16 / (int64_t)sizeof(T)) == 0);
-    };
-    const bool vec = p.cols % 8 == 0 && p.cols <= 1024 * 32 && vec_ok(p.x, p.x_stride) &&
-                     vec_ok(p.residual, p.r_stride) && vec_ok(p.h, p.h_stride) && vec_ok(p.y, p.cols) &&
-                     is_aligned(p.weight, 16) && is_aligned(p.q, 8);
+    constexpr int64_t kPer = 16 / (int64_t)sizeof(T);  // elements between boundaries
     const dim3 grid((unsigned)rows);
-    if (!vec) {
+    // One of x, residual, h and y that exists: do its rows begin where x's do, in
+    // every row, relative to 16-byte boundaries?
+    const auto as_x = [&](const void *ptr, int64_t stride) {
+        return !ptr || ((reinterpret_cast<uintptr_t>(ptr) - reinterpret_cast<uintptr_t>(p.x)) % 16 == 0 &&
+                        (stride - p.x_stride) % kPer == 0);
+    };
+    const bool alike = as_x(p.residual, p.r_stride) && as_x(p.h, p.h_stride) && as_x(p.y, p.cols);
+    const bool vec = alike && p.cols % 8 == 0 && p.cols <= 32 * 1024 && is_aligned(p.x, 16) && p.x_stride % kPer == 0 &&
+                     is_aligned(p.weight, 16) && is_aligned(p.q, 8);
+    // Otherwise by vectors all the same (1021 x 4099 f16, odd rows: 8.4 us, element by
+    // element 9.7); the bytes of q then lie to boundaries of four as x's elements do.
+    const bool shifted = alike && p.cols <= 32 * 1024 - 8 && reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 &&
+                         (!p.q || (is_aligned(p.q, 4) && is_aligned(p.x, 16) && (p.x_stride - p.cols) % kPer == 0));
+    if (!vec && !shifted) {
         const int threads = p.cols >= 1024 ? 512 : (p.cols >= 256 ? 128 : 32);
         const int smem = p.cols * 4;
         const int rc = allow_smem<norm_any_kernel<T>>("norm_any_kernel", kMaxCols * 4);
         if (rc) return rc;
         return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
     }
-    const int vecs = p.cols / 8;
+    const int vecs = vec ? p.cols / 8 : (p.cols + 14) / 8;
     // four vectors a thread: a row's loads are in flight at once, with many rows resident
     const int threads = ceil_div(ceil_div(vecs, 4), 32) * 32;
     const auto launch = [&](auto kernel) {
         return launch_ex(kernel, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
     };
-    if (vecs <= threads) return launch(norm_vec_kernel<T, 1, 32>);
-    if (vecs <= 2 * threads) return launch(norm_vec_kernel<T, 2, 32>);
-    if (threads <= 256) return launch(norm_vec_kernel<T, 4, 256>);
-    return launch(norm_vec_kernel<T, 4, 1024>);
+    if (vecs <= threads) return vec ? launch(norm_vec_kernel<T, 1, 32, false>) : launch(norm_vec_kernel<T, 1, 32, true>);
+    if (vecs <= 2 * threads) return vec ? launch(norm_vec_kernel<T, 2, 32, false>) : launch(norm_vec_kernel<T, 2, 32, true>);
+    if (threads <= 256) return vec ? launch(norm_vec_kernel<T, 4, 256, false>) : launch(norm_vec_kernel<T, 4, 256, true>);
+    return vec ? launch(norm_vec_kernel<T, 4, 1024, false>) : launch(norm_vec_kernel<T, 4, 1024, true>);
 }
 
 int check_rows(const char *what, int64_t rows, int64_t cols) {

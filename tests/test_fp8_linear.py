@@ -91,6 +91,26 @@ def test_norm_strided_rows_and_in_place(cuda, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cols", [1, 7, 9, 250, 1023, 4099, 32759, 32761])
+def test_norm_rows_at_any_address(cuda, dtype, cols):
+    """x, residual and the sum's rows begin the same or different distances past 16-byte boundaries, between NaN
+    that must neither be read nor written over."""
+    w = (1 + rand((cols,), 5, cuda, mul=0.3)).to(dtype)
+    for seed, (at_x, at_r, at_h, gap) in enumerate([(0, 0, 0, 9), (1, 1, 1, 16), (1, 2, 1, 16), (3, 3, 5, 17), (8, 0, 8, 8)]):
+        width = (cols + 15) // 8 * 8 + gap
+        held = [torch.full((5, width), float("nan"), device=cuda, dtype=dtype) for _ in range(3)]
+        x, r, h = (t[:, a:a + cols] for t, a in zip(held, (at_x, at_r, at_h)))
+        x.copy_(rand((5, cols), seed, cuda, dtype))
+        r.copy_(rand((5, cols), seed + 50, cuda, dtype, 2.0))
+        for quantize in (False, True):
+            check_norm(x, w, r, quantize=quantize, residual_out=h)
+            check_norm(x, w.float(), None, quantize=quantize)
+        for t in held:
+            assert int(torch.isnan(t).sum()) == 5 * (width - cols)
+
+
+@pytest.mark.gpu
 def test_norm_zero_nan_inf_rows_and_empty(cuda):
     x = rand((5, 512), 0, cuda, torch.bfloat16)
     x[1] = 0
