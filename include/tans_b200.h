@@ -455,9 +455,11 @@ int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slots, void *k
  * pages table[b * table_stride + i], i < max_pages.  The i-th of n new tokens
  * sees keys up to lens[b] - n + i, with window > 0 only the last `window` of
  * them.  scale multiplies the scores.  lse (f32 [tokens][q_heads], may be
- * null): log of the sum of exponentials.  A token that sees no key gets zeros
- * and lse -inf.  Malformed starts, lens or pages set TANS_B200_DATA_BAD_INDEX
- * and read nothing out of bounds.  workspace: caller-owned device memory,
+ * null): log of the sum of exponentials.  A token that sees no key, and a row
+ * before the first sequence's or after the last's, gets zeros and lse -inf.
+ * Malformed starts, lens or pages set TANS_B200_DATA_BAD_INDEX
+ * and read nothing out of bounds; the rows of a sequence whose starts are
+ * malformed are not written.  workspace: caller-owned device memory,
  * 16-byte aligned, of tans_b200_kv4_attention_workspace_bytes() bytes (may be
  * 0); calls that overlap must not share it. */
 int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cache, int64_t q_heads,

@@ -13,6 +13,12 @@
 // Quantisation of 16 values x (already divided by the gain):
 //   s = e4m3(max|x| / 6), at most 448;  code = e2m1(x / s), 0 where s is 0;
 // both round to nearest even.  A NaN makes the block's scale NaN.
+//
+// Measured on one B200 (8 KV heads of 128, bf16, calls among others in a graph):
+// append of 16383 tokens with 32 query heads 72 us = 5.0 TB/s (bound by memory
+// latency), their read 15 us = 5.7 TB/s; a step of 32 tokens 4.5 us for both.
+// Attention of 64 sequences up to 8192 tokens, group 4: 72 us = 4.2 TB/s; of one
+// with 131071 tokens 46 us with pages of 64 = 3.3 TB/s, 52 us with pages of 16.
 
 #include "sm100.cuh"
 
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 // Both products are transposed, S^T = K Q^T and O^T = V^T P^T: the codes are the
 // A operand of m16n8k16 MMAs and the rows the N dimension, so few rows cost
 // an N of 8 and half the MMAs, sums and exponentials that an M of 16 would
-// (batch of 64, group 4: 93 us with rows as M).
+// (64 sequences up to 8192 tokens, group 4: 93 us with rows as M, 76 so).
 //
 // The codes and the scales of a head lie together in a page, so a unit comes by
 // four bulk copies a page, asked for by the warps in turn while the unit before
@@ -359,9 +365,17 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //    fragment; merging the nibbles of two keys gives bytes whose conversion is
 //    the f16 pair (key, other key) of one element, two elements a MMA.
 // code * scale is exact in f16; P enters in f16 relative to a maximum that may
-// lag by up to 2^8; sums, maxima and O stay in f32.  bf16 queries become f16
-// after a power of two per row that brings their largest element to 2^14: an
+// lag by up to 2^8; sums, maxima and O stay in f32 (sums by an MMA over the
+// rounded P were no faster and cost the lse its last bits).  bf16 queries become
+// f16 after a power of two per row that brings their largest element to 2^14: an
 // element loses bits only below 2^-28 of that.
+//
+// Bound: turning codes into operands.  Per 16 keys of D = 128 a warp issues about
+// 300 instructions, 64 conversions and 64 multiplications by the scale among
+// them; the issue slots are 62 %, the ALU pipe 50 %, memory 64 % busy, and 20
+// warps an SM (95 registers, 40 KB of shared memory a CTA) hide the rest.  With
+// few long sequences the two launches, the start and the join of the parts
+// take about 15 us beside the keys' time.
 
 constexpr int kAttnWarps = 4;
 constexpr int kBlockKeys = 32;                  // keys a warp takes at a time
@@ -1022,6 +1036,21 @@ __device__ __forceinline__ void init_bars(uint64_t *bars) {
     asm volatile("fence.mbarrier_init.release.cluster;");
 }
 
+// The rows of q that lie before the first sequence's and after the last's see
+// nothing: zeros and -inf, by all CTAs of a launch.
+template <typename T, int D>
+__device__ __forceinline__ void clear_spare_rows(const AttendArgs &p, int64_t cta, int64_t ctas) {
+    if (!p.starts) return;
+    const int first = min(max(p.starts[0], 0), p.tokens), last = min(max(p.starts[p.seqs], first), p.tokens);
+    const int q_heads = p.cache.heads * p.group;
+    for (int64_t i = cta; i < p.tokens - (last - first); i += ctas) {
+        const int64_t row = (i < first ? i : i - first + last) * q_heads;
+        uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * D);
+        for (int j = threadIdx.x; j < q_heads * (D / 8); j += blockDim.x) out[j] = uint4{};
+        for (int j = threadIdx.x; p.lse && j < q_heads; j += blockDim.x) p.lse[row + j] = -INFINITY;
+    }
+}
+
 // One CTA a (tile, head, sequence), over all its keys.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) attend_kernel(const AttendArgs p) {
@@ -1031,6 +1060,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     __shared__ __align__(8) uint64_t bars[2 * kStages];
     uint32_t unit_no = 0;
     init_bars(bars);
+    clear_spare_rows<T, D>(p, blockIdx.x + (int64_t)gridDim.x * (blockIdx.y + (int64_t)gridDim.y * blockIdx.z),
+                           (int64_t)gridDim.x * gridDim.y * gridDim.z);
+    if (p.seqs == 0) return;
     const Sequence q = sequence(p, blockIdx.z);
     if ((int)blockIdx.x * p.tile_rows >= q.news * p.group) return;
     if (threadIdx.x < 32) {
@@ -1196,6 +1228,7 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
     pdl_enter();
     const float *at = p.parts + blockIdx.x * split_floats<D, NT>();
     const SplitHead h = *reinterpret_cast<const SplitHead *>(at);
+    clear_spare_rows<T, D>(p, blockIdx.x + (int64_t)gridDim.x * blockIdx.y, (int64_t)gridDim.x * gridDim.y);
     const int slot = threadIdx.x >> 7, turn = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31;
     const int r = blockIdx.y * kJoinRows + slot;
     if (h.pieces == 0 || (int)blockIdx.y * kJoinRows >= h.rows) return;
@@ -1298,7 +1331,7 @@ int launch_attend(const AttendArgs &p, const Plan &plan, cudaStream_t st) {
     if (!plan.ctas) {
         const int rc = allow_smem<attend_kernel<T, D, NT>>("attend_kernel", L::kBytes);
         return rc ? rc
-                  : launch_ex(attend_kernel<T, D, NT>, dim3(ceil_div(plan.rows, L::kRows), p.cache.heads, p.seqs), block,
+                  : launch_ex(attend_kernel<T, D, NT>, dim3(ceil_div(plan.rows, L::kRows), p.cache.heads, p.seqs ? p.seqs : 1), block,
                               L::kBytes, 1, st, "attend_kernel", p);
     }
     int rc = allow_smem<attend_split_kernel<T, D, NT>>("attend_split_kernel", L::kBytes);
@@ -1467,14 +1500,14 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
                                        void *workspace, int64_t workspace_bytes, int dtype, int32_t *status,
                                        void *stream) {
     clear_error();
-    if (tokens == 0 || seqs == 0) return TANS_B200_OK;
+    if (tokens == 0) return TANS_B200_OK;
     AttendArgs p{};
     Plan plan;
     int rc = check_attention(cache, &p.cache, q_heads, max_pages, seqs, tokens, most_new, window);
     if (rc) return rc;
     if (!starts && tokens != seqs)
         return fail(TANS_B200_ERR_INVALID, "kv4_attention: one new token a sequence without starts");
-    if (!q || !out || !lens || (!table && max_pages) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
+    if (!q || !out || (seqs && (!lens || (!table && max_pages))) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_attention: q, out (16-byte aligned, q's stride a multiple of 8), lens and table are needed");
     rc = make_plan(p.cache, q_heads, max_pages, seqs, most_new, window, &plan);

@@ -188,8 +188,8 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     [seqs + 1] int32: the rows of q that are each sequence's new tokens, at
     most most_new of them; without it every sequence has one.  Causal: the i-th
     of n new tokens sees keys up to lens - n + i, only the last `window` of them
-    if window > 0.  scale defaults to dim ** -0.5.  A token that sees nothing
-    gets zeros.  With return_lse also the f32 [tokens, q_heads] logarithm of the
+    if window > 0.  scale defaults to dim ** -0.5.  A token that sees nothing,
+    and a row of q outside starts, gets zeros.  With return_lse also the f32 [tokens, q_heads] logarithm of the
     sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
     least `attention_workspace_bytes`, else allocated."""
     dt, dev = q.dtype, cache.device

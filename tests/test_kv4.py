@@ -340,6 +340,36 @@ def test_attention_ignores_what_is_masked(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page", [4, 32])
+@pytest.mark.parametrize("columns", [20, 300])  # too few pages at most to split the keys, and enough
+@pytest.mark.parametrize("before,after", [(0, 0), (0, 3), (2, 1)])
+def test_attention_takes_views_and_spare_rows(cuda, page, columns, before, after):
+    """q between other columns of one tensor, a table within a wider one, rows of q that no sequence has."""
+    cache, q, table, ln, starts, keys, vals = build([70, 33, 9], [2, 1, 4], 2, 3, 128, page, torch.bfloat16, 3, cuda)
+    want, lse, bo, bl = reference(q, keys, vals, ln.tolist(), [2, 1, 4], 3, 128 ** -0.5, 0)
+    tokens = before + 7 + after
+    wide = torch.full((tokens, 6 * 128 + 264), float("nan"), dtype=torch.bfloat16, device=cuda)
+    view = wide[:, 264:].unflatten(1, (6, 128))
+    view[before:before + 7] = q.to(cuda)
+    tables = torch.full((3, columns + 5), 1 << 29, dtype=torch.int32, device=cuda)
+    tables[:, 3:3 + table.shape[1]] = table.to(cuda)
+    del wide
+    torch.full((tokens, 6, 128), float("nan"), dtype=torch.bfloat16, device=cuda)  # what the output's memory may hold
+    _C.data_status()
+    got, got_lse = kv4.attention(cache, view, tables[:, 3:-2], ln.to(cuda), starts=starts.to(cuda) + before, most_new=4,
+                                 return_lse=True)
+    assert _C.data_status() == 0
+    got, got_lse = got.cpu(), got_lse.cpu()
+    own = slice(before, before + 7)
+    assert bool(((got[own].double() - want).abs() <= bo).all()) and bool(((got_lse[own].double() - lse).abs() <= bl).all())
+    spare = torch.ones(tokens, dtype=torch.bool)
+    spare[own] = False
+    assert not got[spare].any() and torch.isneginf(got_lse[spare]).all()
+    none, none_lse = kv4.attention(cache, view, tables[:0], ln[:0].to(cuda), starts=starts[:1].to(cuda), return_lse=True)
+    assert not none.any() and torch.isneginf(none_lse).all()
+
+
+@pytest.mark.gpu
 def test_attention_flags_bad_metadata(cuda):
     cache, q, table, ln, starts, *_ = build([40, 40], [1, 1], 1, 2, 64, 16, torch.bfloat16, 1, cuda)
     run = lambda t=table, n=ln, **kw: kv4.attention(cache, q.to(cuda), t.to(cuda), n.to(cuda), **kw)  # noqa: E731
