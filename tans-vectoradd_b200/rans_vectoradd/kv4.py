@@ -62,6 +62,8 @@ class KV4Cache:
         self._c = KV4(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), ptr(self.k_gain), ptr(self.v_gain),
                       pages, heads, size, 2 * half)
         self._ref = ctypes.addressof(self._c)
+        # what every call asks for, as plain attributes (a ctypes field takes longer to read)
+        self._dev, self._kv_heads, self._page, self._dim = dev, heads, size, 2 * half
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_size: int = 64, head_dim: int = 128,
@@ -92,21 +94,22 @@ class KV4Cache:
         return self.heads * self.head_dim * 9 // 8
 
 
-def _heads(name: str, t: torch.Tensor, cache: KV4Cache, dtype: torch.dtype) -> int:
-    """Checks [tokens, heads, dim] with dense heads; the stride between tokens."""
-    D = cache._c.dim
-    if t.dim() != 3 or t.shape[2] != D or t.dtype != dtype or t.device != cache.k_codes.device:
-        raise RuntimeError(f"{name} must be [tokens, heads, {D}] {dtype} on the cache's device")
+def _heads(name: str, t: torch.Tensor, dim: int, dtype: torch.dtype, dev: torch.device) -> tuple[int, int, int]:
+    """Checks [tokens, heads, dim] with dense heads: (tokens, heads, stride between tokens)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or t.dtype != dtype or t.device != dev:
+        raise RuntimeError(f"{name} must be [tokens, heads, {dim}] {dtype} on the cache's device")
+    n, heads, _ = shape
     if t.is_contiguous():
-        return t.shape[1] * D
+        return n, heads, heads * dim
     st = t.stride()
-    if st[2] != 1 or (st[1] != D and t.shape[1] != 1):
-        raise RuntimeError(f"{name}'s heads must be dense (strides {D} and 1)")
-    return st[0] if t.shape[0] > 1 else t.shape[1] * D
+    if st[2] != 1 or (st[1] != dim and heads != 1):
+        raise RuntimeError(f"{name}'s heads must be dense (strides {dim} and 1)")
+    return n, heads, st[0] if n > 1 else heads * dim
 
 
 def _index(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: torch.device) -> int:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != dev:
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
         raise RuntimeError(f"{name} must be a contiguous {dtype} tensor of {n} on the cache's device")
     return t.data_ptr()
 
@@ -120,34 +123,37 @@ def append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
     keys rotated by positions [tokens] int64, rows of cos and sin f32
     [max_position, half] (pairs (i, i + half), or (2i, 2i+1) if interleaved;
     2 * half <= dim).  Returns q [tokens, q_heads, dim] rotated alike, if given."""
-    dt, dev = k.dtype, cache.device
+    dt, dev, dim = k.dtype, cache._dev, cache._dim
     if dt not in _HALF:
         raise RuntimeError("k must be bfloat16 or float16")
-    ks, vs = _heads("k", k, cache, dt), _heads("v", v, cache, dt)
-    T = k.shape[0]
-    _req(k.shape[1] == cache.heads and v.shape == k.shape, "k and v must have the cache's heads")
+    T, heads, ks = _heads("k", k, dim, dt, dev)
+    vt, vheads, vs = _heads("v", v, dim, dt, dev)
+    if heads != cache._kv_heads or vheads != heads or vt != T:
+        raise RuntimeError("k and v must have the cache's heads")
     half = top = qs = qh = 0
-    pos_p = cos_p = sin_p = None
+    pos_p = cos_p = sin_p = q_p = out = out_p = None
     if positions is not None:
-        _req(cos is not None and sin is not None, "positions need cos and sin")
-        _req(cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
-             and cos.is_contiguous() and sin.is_contiguous() and cos.device == sin.device == dev,
-             "cos and sin must be contiguous f32 [max_position, half] on the cache's device")
-        top, half = cos.shape
+        if cos is None or sin is None:
+            raise RuntimeError("positions need cos and sin")
+        shape, f32 = cos.shape, torch.float32
+        if (len(shape) != 2 or sin.shape != shape or cos.dtype != f32 or sin.dtype != f32 or not cos.is_contiguous()
+                or not sin.is_contiguous() or cos.device != dev or sin.device != dev):
+            raise RuntimeError("cos and sin must be contiguous f32 [max_position, half] on the cache's device")
+        top, half = shape
         pos_p, cos_p, sin_p = _index("positions", positions, T, torch.int64, dev), cos.data_ptr(), sin.data_ptr()
-    else:
-        _req(cos is None and sin is None, "cos and sin need positions")
-    out = None
-    if q is not None:
-        qs, qh = _heads("q", q, cache, dt), q.shape[1]
-        _req(q.shape[0] == T, "q must have k's tokens")
+    elif cos is not None or sin is not None:
+        raise RuntimeError("cos and sin need positions")
+    slots_p = _index("slots", slots, T, torch.int64, dev)
     with on_device(dev):
         if q is not None:
-            out = torch.empty(*q.shape, dtype=dt, device=dev)
+            qt, qh, qs = _heads("q", q, dim, dt, dev)
+            if qt != T:
+                raise RuntimeError("q must have k's tokens")
+            q_p, out = q.data_ptr(), torch.empty(T, qh, dim, dtype=dt, device=dev)
+            out_p = out.data_ptr()
         check(LIB.tans_b200_kv4_append(
-            cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, _index("slots", slots, T, torch.int64, dev),
-            ptr(q), qs, qh, ptr(out), pos_p, cos_p,
-            sin_p, top, half, int(interleaved), T, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
+            cache._ref, k.data_ptr(), ks, v.data_ptr(), vs, slots_p, q_p, qs, qh, out_p, pos_p, cos_p,
+            sin_p, top, half, interleaved, T, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
     return out
 
@@ -157,9 +163,9 @@ def read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat
     """The keys and values [tokens, heads, dim] that the cache holds in slots
     [tokens] int64 (zeros for a negative slot)."""
     _req(dtype in _FLOAT, "dtype must be bfloat16, float16 or float32")
-    dev, T = cache.device, slots.shape[0]
+    dev, T = cache._dev, slots.shape[0]
     with on_device(dev):
-        k = torch.empty(T, cache._c.heads, cache._c.dim, dtype=dtype, device=dev)
+        k = torch.empty(T, cache._kv_heads, cache._dim, dtype=dtype, device=dev)
         v = torch.empty_like(k)
         check(LIB.tans_b200_kv4_read(cache._ref, _index("slots", slots, T, torch.int64, dev), k.data_ptr(),
                                      v.data_ptr(), T, _FLOAT[dtype], _status(dev).data_ptr(), raw_stream(dev)))
@@ -192,27 +198,26 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     and a row of q outside starts, gets zeros.  With return_lse also the f32 [tokens, q_heads] logarithm of the
     sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
     least `attention_workspace_bytes`, else allocated."""
-    dt, dev = q.dtype, cache.device
+    dt, dev, D = q.dtype, cache._dev, cache._dim
     if dt not in _HALF:
         raise RuntimeError("q must be bfloat16 or float16")
-    qs = _heads("q", q, cache, dt)
-    T, H, D = q.shape
-    B = lens.shape[0] if lens.dim() == 1 else -1
-    if (table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B or table.device != dev
-            or not (table.is_contiguous() or table.stride(1) == 1 or table.shape[1] <= 1)):
+    T, H, qs = _heads("q", q, D, dt, dev)
+    shape, st = table.shape, table.stride()
+    if (len(shape) != 2 or table.dtype != torch.int32 or table.device != dev
+            or not (st[1] == 1 or shape[1] <= 1 or table.is_contiguous())):
         raise RuntimeError("table must be int32 [seqs, max_pages], rows dense")
+    B, P = shape
     lens_p = _index("lens", lens, B, torch.int32, dev)
     starts_p = None if starts is None else _index("starts", starts, B + 1, torch.int32, dev)
-    P = table.shape[1]
     with on_device(dev):
         out = torch.empty(T, H, D, dtype=dt, device=dev)
         lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
-        need = attention_workspace_bytes(cache._c.heads, cache._c.page_size, D, H, P, B, T, most_new, window, dev)
+        need = attention_workspace_bytes(cache._kv_heads, cache._page, D, H, P, B, T, most_new, window, dev)
         if need and workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
         check(LIB.tans_b200_kv4_attention(
-            cache._ref, q.data_ptr(), qs, H, table.data_ptr(), table.stride(0), P, lens_p, starts_p, B, T, most_new,
+            cache._ref, q.data_ptr(), qs, H, table.data_ptr(), st[0], P, lens_p, starts_p, B, T, most_new,
             D ** -0.5 if scale is None else scale, window, out.data_ptr(), ptr(lse),
             ws, ws_bytes, _HALF[dt], _status(dev).data_ptr(), raw_stream(dev)))
     _post_check(dev)
