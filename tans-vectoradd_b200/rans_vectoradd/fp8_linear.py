@@ -22,39 +22,46 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu_tanh": 3}
 
 
-def _rows(name: str, t: torch.Tensor) -> int:
-    """Checks [rows, cols] with a dense last dimension; the stride between rows."""
-    if t.dim() != 2 or t.dtype not in _TYPES or not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor")
+def _stride(name: str, t: torch.Tensor, cols: int) -> int:
+    """The stride between the rows of a two-dimensional t whose last dimension must be dense."""
     if t.is_contiguous():
-        return t.shape[1]
-    if t.stride(1) != 1 and t.shape[1] != 1:
+        return cols
+    st = t.stride()
+    if st[1] != 1 and cols != 1:
         raise RuntimeError(f"{name} must have dense rows")
-    return t.stride(0)
+    return st[0]
 
 
-def _like_x(name: str, t: torch.Tensor, x: torch.Tensor) -> int:
-    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+def _rows(name: str, t: torch.Tensor) -> tuple[torch.Size, int]:
+    """Checks [rows, cols] with a dense last dimension: its shape, the stride between rows."""
+    shape = t.shape
+    if len(shape) != 2 or t.dtype not in _TYPES or not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA [rows, cols] bfloat16, float16 or float32 tensor")
+    return shape, _stride(name, t, shape[1])
+
+
+def _like_x(name: str, t: torch.Tensor, shape: torch.Size, dtype: torch.dtype, dev: torch.device) -> int:
+    if t.shape != shape or t.dtype != dtype or t.device != dev:
         raise RuntimeError(f"{name} must have x's shape, type and device")
-    return _rows(name, t)
+    return _stride(name, t, shape[1])
 
 
 def _norm(x, weight, residual, eps, residual_out, quantize):
-    xs = _rows("x", x)
-    R, C = x.shape
+    shape, xs = _rows("x", x)
+    R, C = shape
     dev, dt, wt = x.device, x.dtype, weight.dtype
-    if (weight.dim() != 1 or weight.shape[0] != C or not weight.is_contiguous() or weight.device != dev
+    if (weight.shape != (C,) or not weight.is_contiguous() or weight.device != dev
             or (wt != dt and wt != torch.float32)):
         raise RuntimeError("weight must be a contiguous [cols] tensor of x's type or float32")
     rs = hs = 0
     h, r_ptr, h_ptr = x, None, None
     with on_device(dev):
         if residual is not None:
-            rs, r_ptr = _like_x("residual", residual, x), residual.data_ptr()
+            rs, r_ptr = _like_x("residual", residual, shape, dt, dev), residual.data_ptr()
             if residual_out is None:
                 h, hs = torch.empty(R, C, dtype=dt, device=dev), C
             else:
-                h, hs = residual_out, _like_x("residual_out", residual_out, x)
+                h, hs = residual_out, _like_x("residual_out", residual_out, shape, dt, dev)
             h_ptr = h.data_ptr()
         elif residual_out is not None:
             raise RuntimeError("residual_out needs residual")
@@ -91,8 +98,7 @@ def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
 
 def quantize_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(q, scale): x [rows, cols] as e4m3 (uint8) and one f32 scale a row."""
-    xs = _rows("x", x)
-    R, C = x.shape
+    (R, C), xs = _rows("x", x)
     dev = x.device
     with on_device(dev):
         q = torch.empty(R, C, dtype=torch.uint8, device=dev)
