@@ -16,7 +16,7 @@
 //
 // Measured on one B200 (8 KV heads of 128, bf16, calls among others in a graph):
 // append of 16383 tokens with 32 query heads 72 us = 5.0 TB/s (bound by memory
-// latency), their read 15 us = 5.7 TB/s; a step of 32 tokens 4.5 us for both.
+// latency), their read 15 us = 5.7 TB/s; a step of 32 tokens 4.5-5 us for both.
 // Attention of 64 sequences up to 8192 tokens, group 4: 72 us = 4.2 TB/s; of one
 // with 131071 tokens 46 us with pages of 64 = 3.3 TB/s, 52 us with pages of 16.
 

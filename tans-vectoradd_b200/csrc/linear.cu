@@ -16,6 +16,12 @@
 // (cta_group::2) own 256 rows x 256 tokens, stay resident over the tiles and
 // write one tile out of tensor memory while they multiply the next: many
 // tokens, bound by the tensor cores.
+//
+// Measured on one B200 (calls among others in a graph): [17408 x 5120], one
+// token 17.3 us = 5.2 TB/s of w; [5120 x 17408], 48 tokens with a residual
+// 21.8 us; [17408 x 5120], 8192 tokens with bias, GELU and a factor 547-582 us =
+// 2.5-2.7 PFLOP/s (a library e4m3 product without any epilogue: 493 us), 640-660
+// us in a loop of seconds, where the power limit sets the clock.
 
 #include "sm100.cuh"
 
@@ -175,6 +181,11 @@ __device__ __forceinline__ void write_eight(const LinearArgs &p, float (&v)[8], 
 }
 
 // ------------------------------------------------------------ split form
+//
+// Reads w at 79 % of the copy rate at one token; what is left is the pipeline's
+// first and last microsecond, when memory idles.  Asking for w in L2 ahead of the
+// kernel before it, more stages and walking the columns from different places
+// on were no faster.
 //
 // Copy warp, MMA warp, and four warps that read tensor memory.  The CTAs of a
 // cluster take equal stretches of the chunks; each puts its f32 sums into its
@@ -372,7 +383,9 @@ __global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __
 // stage in both.  The accumulator has two places in tensor memory; eight warps
 // in each CTA write its 128 rows of one tile while the next is multiplied.
 // Tiles are taken in bands of eight token tiles, the row tiles in turn within
-// a band, so that the tiles in work at a time share their operands in L2.
+// a band, so that the tiles in work at a time share their operands in L2 (8192
+// tokens: 562 us with bands of 4, 547 with 8, 540 with 16; 2048 tokens 170, 144
+// and 147).  Without its epilogue the kernel takes 482 us for the 8192 tokens.
 constexpr int kPairThreads = 320;
 constexpr int kBand = 8;
 constexpr int kWarpFloats = 16 * 32 + 128;  // an epilogue warp's shared memory: 16 tokens x 32 rows, 128 scales
