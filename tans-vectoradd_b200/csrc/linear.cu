@@ -545,15 +545,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             }
             asm volatile("tcgen05.fence::after_thread_sync;");
             const uint32_t acc = tmem + (uint32_t)((it & 1) * p.bn) + ((uint32_t)(32 * quarter) << 16);
-            for (int32_t col = begin; col < end; col += 16) {
-                const int64_t at = (int64_t)(t0 + col + lane / 4) * p.rows + r8;
-                Operands<T> ops[2] = {};
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (real8 > 0 && col + 8 * h + lane / 4 < end) load_operands<T>(p, at + 8 * h * p.rows, ops[h]);
+            const auto values = [&](int32_t col, float (&v)[16]) {  // this lane's row, tokens col .. col + 15
                 uint32_t raw[16];
                 tmem_load(acc + (uint32_t)col, raw);
-                float v[16];
 #pragma unroll
                 for (int k = 0; k < 16; k += 4) {
                     const float4 x = *reinterpret_cast<const float4 *>(xs + col - begin + k);
@@ -563,6 +557,35 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                     v[k + 3] = __fmaf_rn(__uint_as_float(raw[k + 3]) * ws, x.w, bias);
                 }
                 activate(v, p.act);
+            };
+            if (!p.vec)
+                for (int32_t col = begin; col < end; col += 16) {
+                    const int64_t at = (int64_t)(t0 + col) * p.rows + r;
+                    T mul[16] = {}, residual[16] = {};
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        if (real && col + k < end) {
+                            if (p.mul) mul[k] = static_cast<const T *>(p.mul)[at + k * p.rows];
+                            if (p.residual) residual[k] = static_cast<const T *>(p.residual)[at + k * p.rows];
+                        }
+                    float v[16];
+                    values(col, v);
+#pragma unroll
+                    for (int k = 0; k < 16; k++)
+                        if (real && col + k < end) {
+                            if (p.mul) v[k] *= to_f32(mul[k]);
+                            if (p.residual) v[k] += to_f32(residual[k]);
+                            static_cast<T *>(p.y)[at + k * p.rows] = from_f32<T>(v[k]);
+                        }
+                }
+            else for (int32_t col = begin; col < end; col += 16) {
+                const int64_t at = (int64_t)(t0 + col + lane / 4) * p.rows + r8;
+                Operands<T> ops[2] = {};
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (real8 > 0 && col + 8 * h + lane / 4 < end) load_operands<T>(p, at + 8 * h * p.rows, ops[h]);
+                float v[16];
+                values(col, v);
                 __syncwarp();
 #pragma unroll
                 for (int k = 0; k < 16; k++) turned[k * 32 + lane] = v[k];
