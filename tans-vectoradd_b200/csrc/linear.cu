@@ -145,11 +145,11 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// The last step of eight rows r .. r + 7 (`real` of them exist) of token t:
-// v = act(..) becomes v * mul + residual, rounded once.
+// The last step of eight rows r .. r + 7 of token t, where p.vec holds: v = act(..)
+// becomes v * mul + residual, rounded once.
 template <typename T>
 struct Operands {
-    uint4 mul, residual;  // eight values each, loaded ahead where p.vec allows
+    uint4 mul, residual;  // eight values each, loaded ahead
 };
 template <typename T>
 __device__ __forceinline__ void load_operands(const LinearArgs &p, int64_t at, Operands<T> &o) {
@@ -157,28 +157,43 @@ __device__ __forceinline__ void load_operands(const LinearArgs &p, int64_t at, O
     if (p.vec && p.residual) o.residual = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + at);
 }
 template <typename T>
-__device__ __forceinline__ void write_eight(const LinearArgs &p, float (&v)[8], int64_t at, int32_t real, const Operands<T> &o) {
-    if (p.vec) {  // rows are a multiple of 8: all eight exist
-        const T *mu = reinterpret_cast<const T *>(&o.mul), *re = reinterpret_cast<const T *>(&o.residual);
-        if (p.mul) {
+__device__ __forceinline__ void write_eight(const LinearArgs &p, float (&v)[8], int64_t at, const Operands<T> &o) {
+    const T *mu = reinterpret_cast<const T *>(&o.mul), *re = reinterpret_cast<const T *>(&o.residual);
+    if (p.mul) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] *= to_f32(mu[k]);
-        }
-        if (p.residual) {
+        for (int k = 0; k < 8; k++) v[k] *= to_f32(mu[k]);
+    }
+    if (p.residual) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] += to_f32(re[k]);
-        }
-        store8(static_cast<T *>(p.y) + at, v);
-    } else {
+        for (int k = 0; k < 8; k++) v[k] += to_f32(re[k]);
+    }
+    store8(static_cast<T *>(p.y) + at, v);
+}
+
+// The same for one row of N tokens, where eight rows of a token have no common
+// alignment: neighbouring lanes take neighbouring rows.
+template <typename T, int N>
+struct RowOperands {
+    T mul[N], residual[N];
+    __device__ __forceinline__ void load(const LinearArgs &p, int64_t at, int32_t tokens) {
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (k < real) {
-                if (p.mul) v[k] *= to_f32(static_cast<const T *>(p.mul)[at + k]);
-                if (p.residual) v[k] += to_f32(static_cast<const T *>(p.residual)[at + k]);
-                static_cast<T *>(p.y)[at + k] = from_f32<T>(v[k]);
+        for (int k = 0; k < N; k++)
+            if (k < tokens) {
+                if (p.mul) mul[k] = static_cast<const T *>(p.mul)[at + k * p.rows];
+                if (p.residual) residual[k] = static_cast<const T *>(p.residual)[at + k * p.rows];
             }
     }
-}
+    __device__ __forceinline__ void write(const LinearArgs &p, const float (&v)[N], int64_t at, int32_t tokens) const {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (k < tokens) {
+                float e = v[k];
+                if (p.mul) e *= to_f32(mul[k]);
+                if (p.residual) e += to_f32(residual[k]);
+                static_cast<T *>(p.y)[at + k * p.rows] = from_f32<T>(e);
+            }
+    }
+};
 
 // ------------------------------------------------------------ split form
 //
@@ -237,13 +252,15 @@ __global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __
     constexpr int32_t kTokensAtATime = 8;
     const bool writer = warp >= 2;
     const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
-    const int32_t row8 = (threadIdx.x & 15) * 8;
-    const int64_t r = r0 + row8;
-    const int32_t real = p.rows - r < 8 ? (int32_t)(p.rows - r) : 8;
-    const int32_t first = tokens * (int32_t)rank / p.splits + ((int32_t)(threadIdx.x - 64) >> 4);
+    // (where p.vec does not hold: row r of every token)
+    const int32_t row8 = (threadIdx.x & 15) * 8, row1 = (int32_t)threadIdx.x - 64;
+    const int64_t r = r0 + (p.vec ? row8 : row1);
+    const int32_t real = p.vec ? (p.rows - r < 8 ? (int32_t)(p.rows - r) : 8) : (int32_t)(r < p.rows);
+    const int32_t first = tokens * (int32_t)rank / p.splits + (p.vec ? (int32_t)(threadIdx.x - 64) >> 4 : 0);
     const int32_t last = tokens * (int32_t)(rank + 1) / p.splits;
     float ws[8], bias[8], xs_next = 0.f;
     Operands<T> ops{};
+    RowOperands<T, kTokensAtATime> row_ops{};
     if (writer) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
@@ -252,6 +269,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __
         }
         if (first < last && real > 0) {
             load_operands<T>(p, (int64_t)(t0 + first) * p.rows + r, ops);
+            if (!p.vec) row_ops.load(p, (int64_t)(t0 + first) * p.rows + r, last - first);
             xs_next = p.x_scale[t0 + first];
         }
     }
@@ -325,7 +343,31 @@ __global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __
         cluster_sync();
     else
         __syncthreads();
-    if (writer && !*failed && real > 0) {
+    if (writer && !*failed && real > 0 && !p.vec) {
+        for (int32_t col = first; col < last; col += kTokensAtATime) {
+            const RowOperands<T, kTokensAtATime> now = row_ops;
+            const int64_t at = (int64_t)(t0 + col) * p.rows + r;
+            row_ops.load(p, at + kTokensAtATime * p.rows, last - col - kTokensAtATime);
+            float v[kTokensAtATime] = {}, xs[kTokensAtATime];
+#pragma unroll
+            for (int k = 0; k < kTokensAtATime; k++) xs[k] = col + k < last ? p.x_scale[t0 + col + k] : 0.f;
+#pragma unroll 2
+            for (int s = 0; s < p.splits; s++) {
+                const uint32_t from = cluster_addr(a_sa, s) + (uint32_t)(col * 128 + (row1 ^ (row1 >> 3 & 4))) * 4u;
+                float part[kTokensAtATime] = {};
+#pragma unroll
+                for (int k = 0; k < kTokensAtATime; k++)
+                    if (col + k < last)
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[k]) : "r"(from + 512u * k) : "memory");
+#pragma unroll
+                for (int k = 0; k < kTokensAtATime; k++) v[k] += part[k];
+            }
+#pragma unroll
+            for (int k = 0; k < kTokensAtATime; k++) v[k] = __fmaf_rn(v[k] * ws[0], xs[k], bias[0]);
+            activate(v, p.act);
+            now.write(p, v, at, last - col);
+        }
+    } else if (writer && !*failed && real > 0) {
         for (int32_t col = first; col < last; col += kTokensAtATime) {
             const Operands<T> now = ops;
             const float xs = xs_next;
@@ -362,7 +404,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) linear_split_kernel(const __
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = __fmaf_rn(v[k] * ws[k], xs, bias[k]);
             activate(v, p.act);
-            write_eight<T>(p, v, at, real, now);
+            write_eight<T>(p, v, at, now);
         }
     }
     if (p.splits > 1) {
@@ -535,6 +577,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             const int32_t real8 = p.rows - r8 < 8 ? (int32_t)(p.rows - r8) : 8;
             const int32_t tokens = p.m - t0 < p.bn ? (int32_t)(p.m - t0) : p.bn;
             const int32_t begin = half * p.bn / 2, end = min(tokens, begin + p.bn / 2);
+            // the factor and the residual are asked for 16 tokens ahead, the first before the sums are there
+            int64_t at = p.vec ? (int64_t)(t0 + begin + lane / 4) * p.rows + r8 : (int64_t)(t0 + begin) * p.rows + r;
+            Operands<T> next[2] = {};
+            const auto fetch = [&](int32_t col, int64_t from) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (real8 > 0 && col + 8 * h + lane / 4 < end) load_operands<T>(p, from + 8 * h * p.rows, next[h]);
+            };
+            RowOperands<T, 16> row_next{};
+            if (p.vec)
+                fetch(begin, at);
+            else if (real)
+                row_next.load(p, at, end - begin);
             __syncwarp();
             for (int32_t i = lane; i < p.bn / 2; i += 32) xs[i] = begin + i < end ? p.x_scale[t0 + begin + i] : 0.f;
             __syncwarp();
@@ -558,43 +613,30 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 }
                 activate(v, p.act);
             };
-            if (!p.vec)
-                for (int32_t col = begin; col < end; col += 16) {
-                    const int64_t at = (int64_t)(t0 + col) * p.rows + r;
-                    T mul[16] = {}, residual[16] = {};
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        if (real && col + k < end) {
-                            if (p.mul) mul[k] = static_cast<const T *>(p.mul)[at + k * p.rows];
-                            if (p.residual) residual[k] = static_cast<const T *>(p.residual)[at + k * p.rows];
-                        }
+            if (!p.vec) {
+                for (int32_t col = begin; col < end; col += 16, at += 16 * p.rows) {
+                    const RowOperands<T, 16> now = row_next;
+                    if (real) row_next.load(p, at + 16 * p.rows, end - col - 16);
                     float v[16];
                     values(col, v);
-#pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        if (real && col + k < end) {
-                            if (p.mul) v[k] *= to_f32(mul[k]);
-                            if (p.residual) v[k] += to_f32(residual[k]);
-                            static_cast<T *>(p.y)[at + k * p.rows] = from_f32<T>(v[k]);
-                        }
+                    if (real) now.write(p, v, at, end - col);
                 }
-            else for (int32_t col = begin; col < end; col += 16) {
-                const int64_t at = (int64_t)(t0 + col + lane / 4) * p.rows + r8;
-                Operands<T> ops[2] = {};
+            } else {
+                for (int32_t col = begin; col < end; col += 16, at += 16 * p.rows) {
+                    const Operands<T> now[2] = {next[0], next[1]};
+                    fetch(col + 16, at + 16 * p.rows);
+                    float v[16];
+                    values(col, v);
+                    __syncwarp();
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (real8 > 0 && col + 8 * h + lane / 4 < end) load_operands<T>(p, at + 8 * h * p.rows, ops[h]);
-                float v[16];
-                values(col, v);
-                __syncwarp();
+                    for (int k = 0; k < 16; k++) turned[k * 32 + lane] = v[k];
+                    __syncwarp();
 #pragma unroll
-                for (int k = 0; k < 16; k++) turned[k * 32 + lane] = v[k];
-                __syncwarp();
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float e[8];
-                    load8(turned + (8 * h + lane / 4) * 32 + lane % 4 * 8, e);
-                    if (real8 > 0 && col + 8 * h + lane / 4 < end) write_eight<T>(p, e, at + 8 * h * p.rows, real8, ops[h]);
+                    for (int h = 0; h < 2; h++) {
+                        float e[8];
+                        load8(turned + (8 * h + lane / 4) * 32 + lane % 4 * 8, e);
+                        if (real8 > 0 && col + 8 * h + lane / 4 < end) write_eight<T>(p, e, at + 8 * h * p.rows, now[h]);
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;");
