@@ -208,6 +208,27 @@ def test_linear_epilogues(cuda, dtype, act, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 7, 32), (5, 333, 2064), (37, 130, 4096), (150, 335, 512), (131, 9601, 64), (260, 9600, 64),
+                                   (513, 5003, 144)])
+@pytest.mark.parametrize("into", ["mul", "residual", "none"])
+def test_linear_at_any_address(cuda, m, n, k, into):
+    """Rows of any count, operands and output two bytes past an alignment of 16, the output in an operand's place;
+    nothing beyond its ends is written."""
+    x8, xs = quantized(m, k, m, cuda)
+    w8, ws = quantized(n, k, n, cuda, 0.1)
+    held = {name: torch.full((m * n + 20,), 77.0, dtype=torch.bfloat16, device=cuda) for name in ("mul", "residual", "none")}
+    at = {name: t[1:1 + m * n].view(m, n) for name, t in held.items()}
+    at["mul"].copy_(rand((m, n), 1, cuda))
+    at["residual"].copy_(rand((m, n), 2, cuda))
+    b, mul, residual = rand((n,), 3, cuda, torch.bfloat16), at["mul"].clone(), at["residual"].clone()
+    want = check_linear(x8, xs, w8, ws, b, "silu", mul, residual)
+    got = fp8_linear.linear(x8, xs, w8, ws, bias=b, act="silu", mul=at["mul"], residual=at["residual"], out=at[into])
+    assert got is at[into] and torch.equal(got, want)
+    for t in held.values():
+        assert t[0] == 77 and bool((t[1 + m * n:] == 77).all())
+
+
+@pytest.mark.gpu
 def test_linear_is_deterministic_and_takes_an_empty_batch(cuda):
     x8, xs = quantized(48, 17408, 3, cuda)
     w8, ws = quantized(640, 17408, 4, cuda)
