@@ -15,7 +15,8 @@
 // every input is read once and every output written once, so the kernel is
 // bound by memory for many rows and by launch and reduction latency for few.
 // Measured on one B200, residual and e4m3 output: 16384 x 5120 bf16 95 us =
-// 6.2 TB/s (95 % of the copy rate); 1 x 5120 2.7 us among others in a graph.
+// 6.2 TB/s (95 % of the copy rate), 16384 x 5121 104 us; 1 x 5120 2.7 us among
+// others in a graph.
 // All loads of a row come before the first use of one: 135 us with the
 // residual's after the sums of x began.
 
@@ -34,6 +35,7 @@ struct NormArgs {
     float eps;
     bool weight_f32;
     bool norm;
+    bool weight_vec = false;  // the weight has x's type and begins on a 16-byte boundary
 };
 
 // Sum of a and maximum (NaN kept) of b over the block; every thread gets both.
@@ -69,32 +71,40 @@ __device__ __forceinline__ float row_factor(const NormArgs &p, float sumsq, floa
     return amax > 1e-30f && amax < 1e30f && top > 1e-30f ? 448.f / amax : inv / scale;
 }
 
-// Eight elements e0 .. e0 + 7 of a row of `cols`; at its ends, where some lie
-// outside (and count as 0, or stay unwritten), one by one.
+// Elements o .. o + 7 of the sixteen in a and b, 0 < o < 8, the same o in all lanes.
 template <typename T>
-__device__ __forceinline__ Eight<T> load_part(const T *row, int e0, int cols) {
-    if (e0 >= 0 && e0 + 8 <= cols) return load_eight(row + e0);
-    Eight<T> r;
-    T *e = reinterpret_cast<T *>(r.u);
+__device__ __forceinline__ Eight<T> window(const Eight<T> &a, const Eight<T> &b, int o) {
+    constexpr int kWords = 2 * (int)sizeof(T);
+    uint32_t w[2 * kWords];
 #pragma unroll
-    for (int k = 0; k < 8; k++) e[k] = (unsigned)(e0 + k) < (unsigned)cols ? row[e0 + k] : from_f32<T>(0.f);
-    return r;
-}
-template <typename T>
-__device__ __forceinline__ void store_part(T *row, int e0, int cols, const float (&v)[8]) {
-    if (e0 >= 0 && e0 + 8 <= cols) {
-        store8(row + e0, v);
-        return;
+    for (int i = 0; i < kWords; i++) {
+        w[i] = reinterpret_cast<const uint32_t *>(a.u)[i];
+        w[kWords + i] = reinterpret_cast<const uint32_t *>(b.u)[i];
     }
+    if (o & 4) {
 #pragma unroll
-    for (int k = 0; k < 8; k++)
-        if ((unsigned)(e0 + k) < (unsigned)cols) row[e0 + k] = from_f32<T>(v[k]);
+        for (int i = 0; i < 3 * kWords / 2; i++) w[i] = w[i + kWords / 2];
+    }
+    if (o & 2) {
+#pragma unroll
+        for (int i = 0; i < 5 * kWords / 4; i++) w[i] = w[i + kWords / 4];
+    }
+    if (o & 1) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) w[i] = sizeof(T) == 4 ? w[i + 1] : __funnelshift_r(w[i], w[i + 1], 16);
+    }
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < kWords; i++) reinterpret_cast<uint32_t *>(r.u)[i] = w[i];
+    return r;
 }
 
 // Rows by 8-element vectors on 16-byte boundaries: thread t holds vectors t, t +
 // blockDim, ...  kShifted: rows begin anywhere, x, residual, h and y alike; the
-// first vector begins at the boundary before the row, and the weight, which lies
-// to another, is read one by one.
+// vectors are those between the row's first and last boundary, the elements at
+// its ends are one each of the block's first 16 threads, and the weight, which lies
+// otherwise, is cut out of two of its own vectors (one of another type or off
+// its boundary: read one by one).
 template <typename T, int VPT, int kMost, bool kShifted>
 __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     __shared__ float2 buf[32];
@@ -102,26 +112,28 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     const int64_t row = blockIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
     const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
-    const int shift = kShifted ? (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % (16 / sizeof(T))) : 0;
-    const int vecs = kShifted ? (p.cols + shift + 7) / 8 : p.cols / 8;
-    const auto load = [&](const T *from, int v) {
-        return kShifted ? load_part(from, 8 * v - shift, p.cols) : load_eight(from + 8 * v);
-    };
-    const auto store = [&](T *to, int v, const float (&a)[8]) {
-        if constexpr (kShifted)
-            store_part(to, 8 * v - shift, p.cols, a);
-        else
-            store8(to + 8 * v, a);
-    };
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const int head = kShifted ? min((kPer - (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % kPer)) % kPer, p.cols) : 0;
+    const int vecs = (p.cols - head) / 8;
+    // this thread's element of the ends, or none
+    const int end = (int)threadIdx.x < 8 ? (int)threadIdx.x : head + 8 * vecs + (int)threadIdx.x - 8;
+    const bool has_end = kShifted && threadIdx.x < 16 && end < (threadIdx.x < 8 ? head : p.cols);
+    const T *wt = static_cast<const T *>(p.weight);
+    float at_end = 0.f, w_end = 1.f;
+    if (has_end) {
+        at_end = to_f32(x[end]);
+        if (r) at_end += to_f32(r[end]);
+        if (p.norm) w_end = p.weight_f32 ? static_cast<const float *>(p.weight)[end] : to_f32(wt[end]);
+    }
     // every load of the row before the first use of one
     Eight<T> xv[VPT], rv[VPT], wv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < vecs) {
-            xv[i] = load(x, v);
-            if (r) rv[i] = load(r, v);
-            if (!kShifted && p.norm && !p.weight_f32) wv[i] = load_eight(static_cast<const T *>(p.weight) + 8 * v);
+            xv[i] = load_eight(x + head + 8 * v);
+            if (r) rv[i] = load_eight(r + head + 8 * v);
+            if (!kShifted && p.norm && !p.weight_f32) wv[i] = load_eight(wt + 8 * v);
         }
     }
     float s[VPT][8];
@@ -136,18 +148,21 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
                 rv[i].to(a);
 #pragma unroll
                 for (int k = 0; k < 8; k++) s[i][k] += a[k];
-                store(static_cast<T *>(p.h) + row * p.h_stride, v, s[i]);
+                store8(static_cast<T *>(p.h) + row * p.h_stride + head + 8 * v, s[i]);
             }
             if (p.norm) {
                 float w[8];
                 if constexpr (kShifted) {
+                    if (p.weight_vec && (head == 0 || 8 * v + 16 <= p.cols)) {
+                        Eight<T> e = load_eight(wt + 8 * v);
+                        if (head) e = window(e, load_eight(wt + 8 * v + 8), head);
+                        e.to(w);
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int e = 8 * v - shift + k;
-                        w[k] = (unsigned)e >= (unsigned)p.cols
-                                   ? 0.f
-                                   : (p.weight_f32 ? static_cast<const float *>(p.weight)[e]
-                                                   : to_f32(static_cast<const T *>(p.weight)[e]));
+                        for (int k = 0; k < 8; k++) {
+                            const int e = head + 8 * v + k;
+                            w[k] = p.weight_f32 ? static_cast<const float *>(p.weight)[e] : to_f32(wt[e]);
+                        }
                     }
                 } else if (p.weight_f32) {
                     load8(static_cast<const float *>(p.weight) + 8 * v, w);
@@ -166,10 +181,22 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
             }
         }
     }
+    if (has_end) {
+        if (r) static_cast<T *>(p.h)[row * p.h_stride + end] = from_f32<T>(at_end);
+        if (p.norm) sumsq = __fmaf_rn(at_end, at_end, sumsq);
+        at_end *= w_end;
+        if (p.q) amax = max_nan(amax, fabsf(at_end));
+    }
     block_reduce(sumsq, amax, buf);
     float scale;
     const float f = row_factor(p, sumsq, amax, scale);
     if (p.q && threadIdx.x == 0) p.scale[row] = scale;
+    if (has_end) {
+        if (p.q)
+            p.q[row * p.cols + end] = (uint8_t)e4m3x2(at_end * f, 0.f);
+        else
+            static_cast<T *>(p.y)[row * p.cols + end] = from_f32<T>(at_end * f);
+    }
 #pragma unroll
     for (int i = 0; i < VPT; i++) {
         const int v = threadIdx.x + i * blockDim.x;
@@ -180,20 +207,15 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
                 uint2 u;
                 u.x = e4m3x2(s[i][0], s[i][1]) | e4m3x2(s[i][2], s[i][3]) << 16;
                 u.y = e4m3x2(s[i][4], s[i][5]) | e4m3x2(s[i][6], s[i][7]) << 16;
-                uint8_t *q = p.q + row * p.cols;
-                const int e0 = 8 * v - shift;
+                uint8_t *q = p.q + row * p.cols + head + 8 * v;
                 if (!kShifted) {
-                    *reinterpret_cast<uint2 *>(q + e0) = u;
-                } else if (e0 >= 0 && e0 + 8 <= p.cols) {  // on a boundary of four
-                    reinterpret_cast<uint32_t *>(q + e0)[0] = u.x;
-                    reinterpret_cast<uint32_t *>(q + e0)[1] = u.y;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        if ((unsigned)(e0 + k) < (unsigned)p.cols) q[e0 + k] = (uint8_t)((k < 4 ? u.x : u.y) >> (8 * (k & 3)));
+                    *reinterpret_cast<uint2 *>(q) = u;
+                } else {  // on a boundary of four
+                    reinterpret_cast<uint32_t *>(q)[0] = u.x;
+                    reinterpret_cast<uint32_t *>(q)[1] = u.y;
                 }
             } else {
-                store(static_cast<T *>(p.y) + row * p.cols, v, s[i]);
+                store8(static_cast<T *>(p.y) + row * p.cols + head + 8 * v, s[i]);
             }
         }
     }
@@ -201,7 +223,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
 
 // Wider rows, and rows of tensors that lie to 16-byte boundaries each in its own
 // way: element by element, s * w kept in shared memory (1021 x 4099 f16: 9.7 us
-// out of L2, where vectors take 8.4; bound by its 2-byte accesses).
+// out of L2, where vectors take 5.5; bound by its 2-byte accesses).
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
     extern __shared__ float srow[];
@@ -240,7 +262,8 @@ __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
 constexpr int kMaxCols = 56 * 1024;  // f32 values of one row that fit a CTA's shared memory
 
 template <typename T>
-int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
+int launch_norm(NormArgs p, int64_t rows, cudaStream_t st) {
+    p.weight_vec = is_aligned(p.weight, 16) && (!p.weight_f32 || sizeof(T) == 4);
     constexpr int64_t kPer = 16 / (int64_t)sizeof(T);  // elements between boundaries
     const dim3 grid((unsigned)rows);
     // One of x, residual, h and y that exists: do its rows begin where x's do, in
@@ -252,9 +275,9 @@ int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
     const bool alike = as_x(p.residual, p.r_stride) && as_x(p.h, p.h_stride) && as_x(p.y, p.cols);
     const bool vec = alike && p.cols % 8 == 0 && p.cols <= 32 * 1024 && is_aligned(p.x, 16) && p.x_stride % kPer == 0 &&
                      is_aligned(p.weight, 16) && is_aligned(p.q, 8);
-    // Otherwise by vectors all the same (1021 x 4099 f16, odd rows: 8.4 us, element by
+    // Otherwise by vectors all the same (1021 x 4099 f16, odd rows: 5.5 us, element by
     // element 9.7); the bytes of q then lie to boundaries of four as x's elements do.
-    const bool shifted = alike && p.cols <= 32 * 1024 - 8 && reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 &&
+    const bool shifted = alike && p.cols < 32 * 1024 + 8 && reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 &&
                          (!p.q || (is_aligned(p.q, 4) && is_aligned(p.x, 16) && (p.x_stride - p.cols) % kPer == 0));
     if (!vec && !shifted) {
         const int threads = p.cols >= 1024 ? 512 : (p.cols >= 256 ? 128 : 32);
@@ -263,7 +286,7 @@ int launch_norm(const NormArgs &p, int64_t rows, cudaStream_t st) {
         if (rc) return rc;
         return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
     }
-    const int vecs = vec ? p.cols / 8 : (p.cols + 14) / 8;
+    const int vecs = p.cols < 8 ? 1 : p.cols / 8;
     // four vectors a thread: a row's loads are in flight at once, with many rows resident
     const int threads = ceil_div(ceil_div(vecs, 4), 32) * 32;
     const auto launch = [&](auto kernel) {
