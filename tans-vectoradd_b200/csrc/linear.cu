@@ -33,6 +33,12 @@ namespace {
 constexpr int kMaxStages = 8;
 constexpr uint32_t kWaitLimit = 1u << 16;  // polls per wait
 constexpr uint32_t kPollNs = 10000;        // suspend-time hint per poll: bound ~0.66 s
+// Polls of the pair form's epilogue for a tile's sums.  A build with 0 makes every
+// such wait run out at once, which shows that the status says so.
+#ifndef TANS_B200_EPILOGUE_POLLS
+#define TANS_B200_EPILOGUE_POLLS kWaitLimit
+#endif
+constexpr uint32_t kEpiloguePolls = TANS_B200_EPILOGUE_POLLS;
 constexpr int kMaxSmem = 225 * 1024;       // dynamic; the barriers' few bytes are static
 constexpr uint32_t kTileA = 128 * 128;     // bytes of 128 rows x 128 columns
 
@@ -59,9 +65,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 // Wait for the phase of `bar` with the given parity; false when the wait runs
 // out or (checked every 16 polls) *failed became non-zero.  kCluster: arrivals
 // of the cluster's other CTA are acquired too.
-template <bool kCluster = false>
+template <bool kCluster = false, uint32_t kPolls = kWaitLimit>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const volatile int32_t *failed) {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+    for (uint32_t i = 0; i < kPolls; i++) {
         uint32_t done;
         if constexpr (kCluster)
             asm volatile(
@@ -448,6 +454,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
     __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_s;
     __shared__ int32_t failed_s;
+    __shared__ int64_t copied_s;  // stages that this CTA's copy thread has filled
     volatile int32_t *failed = &failed_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
@@ -525,9 +532,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 if (++s == p.stages) s = 0, ph ^= 1u;
             }
         }
-        if (*failed && rank == 0)  // copies in flight land before the pair may end
-            for (int64_t c = copied > p.stages ? copied - p.stages : 0; c < copied; c++)
-                mbar_wait(full0 + 8u * (uint32_t)(c % p.stages), (uint32_t)(c / p.stages & 1), nullptr);
+        copied_s = copied;
     } else if (warp == 1 && lane == 0 && rank == 0) {  // ---------- MMA, for both CTAs
         const uint32_t idesc = (1u << 4) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
         const auto commit = [&](uint32_t bar) {
@@ -564,7 +569,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
                 commit(empty0 + 8u * s);
                 if (++s == p.stages) s = 0, ph ^= 1u;
             }
-            if (ok) commit(accf0 + 8u * (it & 1));
+            if (!ok) give_up();
+            commit(accf0 + 8u * (it & 1));  // what was multiplied is waited for even then
         }
         if (!ok) give_up();
         if (it > 0 && !mbar_wait(accf0 + 8u * ((it - 1) & 1), ((it - 1) >> 1) & 1, nullptr)) give_up();
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
             __syncwarp();
             for (int32_t i = lane; i < p.bn / 2; i += 32) xs[i] = begin + i < end ? p.x_scale[t0 + begin + i] : 0.f;
             __syncwarp();
-            uint32_t ok = lane ? 1u : (uint32_t)mbar_wait(accf0 + 8u * (it & 1), (it >> 1) & 1, failed);
+            uint32_t ok = lane ? 1u : (uint32_t)mbar_wait<false, kEpiloguePolls>(accf0 + 8u * (it & 1), (it >> 1) & 1, failed);
             if (!__all_sync(0xffffffffu, ok)) {
                 if (lane == 0) give_up();
                 break;
@@ -658,9 +664,36 @@ __global__ void __launch_bounds__(kPairThreads, 1) linear_pair_kernel(const __gr
         }
     }
     __syncwarp();
-    if (*failed && threadIdx.x == 0 && p.status) atomicOr(p.status, TANS_B200_DATA_TIMEOUT);
     asm volatile("tcgen05.fence::before_thread_sync;");
-    cluster_sync();  // neither CTA leaves while the other may reach its memory
+    // Every role of both CTAs has ended, and both see a wait that ran out in any of
+    // them; neither CTA leaves while the other may reach its memory.
+    cluster_sync();
+    if (*failed) {
+        if (threadIdx.x == 0) {
+            if (p.status) atomicOr(p.status, TANS_B200_DATA_TIMEOUT);
+            if (rank == 0) {  // copies in flight land before the pair may end
+                const int64_t mine = copied_s;
+                int64_t other;
+                asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(other) : "r"(cluster_addr(shared_addr(&copied_s), 1))
+                             : "memory");
+                const int64_t most = mine > other ? mine : other;
+                for (int64_t c = most > p.stages ? most - p.stages : 0; c < most; c++) {
+                    const uint32_t bar = full0 + 8u * (uint32_t)(c % p.stages);
+                    // a stage that one CTA alone has filled: expect its bytes only
+                    if (c >= mine)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kTileA + b_bytes)
+                                     : "memory");
+                    else if (c >= other)
+                        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar),
+                                     "r"(kTileA + b_bytes)
+                                     : "memory");
+                    mbar_wait<true>(bar, (uint32_t)(c / p.stages & 1), nullptr);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(ncols));
