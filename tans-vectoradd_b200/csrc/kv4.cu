@@ -22,6 +22,8 @@
 
 #include "sm100.cuh"
 
+#include <stddef.h>
+
 namespace tans_b200 {
 namespace {
 
@@ -450,20 +452,50 @@ __device__ __forceinline__ void copy_bulk(uint32_t dst, const uint8_t *src, uint
                  : "memory");
 }
 
-// Waits for the phase of `bar` with the given parity.  Bounded: copies that do
-// not land within about a second set TANS_B200_DATA_TIMEOUT.
-__device__ __forceinline__ void wait_copies(uint32_t bar, uint32_t parity, int32_t *status) {
-    for (uint32_t i = 0; i < 1u << 16; i++) {
+constexpr uint32_t kWaitLimit = 1u << 16;  // polls of a wait, 10 us each at most
+// Polls of the waits for a unit's copies and for its readers.  A build with 0
+// makes them run out at once, which shows that the status says so.
+#ifndef TANS_B200_COPY_POLLS
+#define TANS_B200_COPY_POLLS kWaitLimit
+#endif
+
+// The barriers of a CTA's copies, in shared memory: for each stage the one of its
+// copies, then for each the one of its readers.
+struct Copies {
+    uint64_t bars[2 * kStages];
+    uint32_t issued;  // units asked for
+    uint32_t failed;  // a wait ran out: no more copies, no more units
+};
+
+// Waits for the phase with the given parity of the barrier `at` of the Copies at
+// `copies`.  Bounded: false, `failed` and TANS_B200_DATA_TIMEOUT when it has not
+// come within 0.66 s, or (looked at every 16 polls) another wait of the CTA has run
+// out.  kLast: for what is in flight after that; with it a CTA's waits end
+// within three such limits.
+template <uint32_t kPolls = TANS_B200_COPY_POLLS, bool kLast = false>
+__device__ __forceinline__ bool wait_copies(uint32_t copies, int at, uint32_t parity, int32_t *status) {
+    for (uint32_t i = 0; i < kPolls; i++) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, 10000;\n\t"
             "selp.b32 %0, 1, 0, P1;\n\t}"
             : "=r"(done)
-            : "r"(bar), "r"(parity)
+            : "r"(copies + 8u * at), "r"(parity)
             : "memory");
-        if (done) return;
+        if (done) return true;
+        if (!kLast && (i & 15u) == 15u) {
+            uint32_t failed;
+            asm volatile("ld.volatile.shared.b32 %0, [%1];"
+                         : "=r"(failed)
+                         : "r"(copies + (uint32_t)offsetof(Copies, failed))
+                         : "memory");
+            if (failed) return false;
+        }
     }
+    if (!kLast)
+        asm volatile("st.volatile.shared.b32 [%0], 1;" ::"r"(copies + (uint32_t)offsetof(Copies, failed)) : "memory");
     if (status) atomicOr(status, TANS_B200_DATA_TIMEOUT);
+    return false;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
@@ -553,12 +585,12 @@ __device__ __forceinline__ void set_rows(const AttendArgs &p, Piece &x) {
     }
 }
 
-// Runs a piece (set by the caller, before a block barrier).  s_bars: for each
-// stage the barrier of its copies, then for each the barrier of its readers;
-// unit_no counts the CTA's units, for their parities.  Afterwards the four
-// warps' results lie in `smem` as [warp][kRows][kRow] O, [warp][kRows] maxima and sums.
+// Runs a piece (set by the caller, before a block barrier).  unit_no counts the
+// CTA's units, for their parities.  Afterwards the four warps' results lie in
+// `smem` as [warp][kRows][kRow] O, [warp][kRows] maxima and sums.  False if a wait
+// ran out: there are no results, and no copies in flight.
 template <typename T, int D, int NT>
-__device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem, uint64_t *s_bars,
+__device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x, uint8_t *smem, Copies &s_copies,
                                              uint32_t &unit_no) {
     using L = AttnLayout<D, NT>;
     constexpr int kSteps = D / 16;        // MMA steps of S
@@ -568,7 +600,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     constexpr int kKS = D / 64;           // scales of a quarter
     constexpr int kTogether = 2;  // halves of 16 keys worked on together
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int head = x.head, k1 = x.k1, lo_all = x.lo_all;
+    const int head = x.head, lo_all = x.lo_all;
+    int k1 = x.k1;
     const int kend = min(x.hi_all, k1 - 1);  // the piece's last key
     uint4 *qs = reinterpret_cast<uint4 *>(smem + L::kBytes - L::kQ - L::kRows * 4);
     float *factors = reinterpret_cast<float *>(smem + L::kBytes - L::kRows * 4);
@@ -580,7 +613,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     const int32_t *table = p.table + (int64_t)x.seq * p.table_stride;
     const uint64_t head_at = (uint64_t)head << page_log2;
     const uint32_t page_tokens = (uint32_t)p.cache.heads << page_log2;
-    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(smem), bars = (uint32_t)__cvta_generic_to_shared(s_bars);
+    const uint32_t ring_sa = (uint32_t)__cvta_generic_to_shared(smem), copies_sa = (uint32_t)__cvta_generic_to_shared(&s_copies);
     const int run = min(kUnit, 1 << page_log2), run_at = (lane >> 2) * run;
     const bool copies = bulk && run_at < kUnit;
     // the page of this lane's run of the unit at `base`; keys outside the piece
@@ -591,10 +624,14 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
     const auto issue = [&](int unit, uint32_t page, uint32_t no) {  // the no-th unit of this CTA
         const int st = no % kStages;
         // its place was read by all four warps in unit no - 2
-        if (no >= kStages) wait_copies(bars + 8u * (kStages + st), (no / kStages + 1) & 1, p.status);
-        const uint32_t bar = bars + 8u * st;
-        if (lane == 0)
+        if (no >= kStages &&
+            !__all_sync(0xffffffffu, wait_copies(copies_sa, kStages + st, (no / kStages + 1) & 1, p.status)))
+            return;
+        const uint32_t bar = copies_sa + 8u * st;
+        if (lane == 0) {
+            s_copies.issued = no + 1;
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(L::kStage) : "memory");
+        }
         if (copies) {
             if (page >= (uint32_t)p.cache.pages) {
                 if (p.status) atomicOr(p.status, TANS_B200_DATA_BAD_INDEX);
@@ -728,7 +765,8 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                 issue(unit + kUnit, page, unit_no + 1);
                 page = page_of(unit + 5 * kUnit);
             }
-            wait_copies(bars + 8u * st, unit_no / kStages & 1, p.status);
+            // (after a wait that ran out the unit's work is done on what lies there, and is the last)
+            if (!__all_sync(0xffffffffu, wait_copies(copies_sa, st, unit_no / kStages & 1, p.status))) k1 = unit;
         } else {
             copy_key(unit + kUnit, page, unit_no + 1);
             page = key_page(unit + 2 * kUnit);
@@ -943,11 +981,18 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
         }
         __syncwarp();  // all lanes have read their keys before the place is filled again
         if (bulk && lane == 0)
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + 8u * (kStages + st)) : "memory");
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(copies_sa + 8u * (kStages + st)) : "memory");
     }
 
     // ---- the warps' results, side by side
     __syncthreads();
+    if (s_copies.failed) {
+        if (threadIdx.x == 0)
+            for (uint32_t no = s_copies.issued - min(s_copies.issued, (uint32_t)kStages); no < s_copies.issued; no++)
+                wait_copies<kWaitLimit, true>(copies_sa, no % kStages, no / kStages & 1, p.status);
+        __syncthreads();
+        return false;
+    }
     float *merge = reinterpret_cast<float *>(smem);
     float *tops = merge + kAttnWarps * L::kRows * L::kRow, *sums = tops + kAttnWarps * L::kRows;
 #pragma unroll
@@ -967,6 +1012,7 @@ __device__ __forceinline__ void attend_piece(const AttendArgs &p, const Piece &x
                     make_float2(o[j][n][i], o[j][n][2 + i]);
         }
     __syncthreads();
+    return true;
 }
 
 // The factor that brings a part with maximum `top` and sum `sum` to the common
@@ -1029,10 +1075,11 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, 
 }
 
 // Called by all threads, before a block barrier.
-__device__ __forceinline__ void init_bars(uint64_t *bars) {
+__device__ __forceinline__ void init_copies(Copies &c) {
     if (threadIdx.x < 2 * kStages)
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(bars + threadIdx.x)),
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(c.bars + threadIdx.x)),
                      "r"(threadIdx.x < kStages ? 1 : kAttnWarps));
+    if (threadIdx.x == 0) c.issued = 0, c.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;");
 }
 
@@ -1057,9 +1104,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     extern __shared__ __align__(16) uint8_t smem[];
     pdl_enter();
     __shared__ Piece x;
-    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    __shared__ Copies copies;
     uint32_t unit_no = 0;
-    init_bars(bars);
+    init_copies(copies);
     clear_spare_rows<T, D>(p, blockIdx.x + (int64_t)gridDim.x * (blockIdx.y + (int64_t)gridDim.y * blockIdx.z),
                            (int64_t)gridDim.x * gridDim.y * gridDim.z);
     if (p.seqs == 0) return;
@@ -1076,8 +1123,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
         set_rows(p, x);
     }
     __syncthreads();
-    attend_piece<T, D, NT>(p, x, smem, bars, unit_no);
-    join_warps<T, D, NT>(p, x, smem, nullptr);
+    if (attend_piece<T, D, NT>(p, x, smem, copies, unit_no)) join_warps<T, D, NT>(p, x, smem, nullptr);
 }
 
 // Split form: the units of all tiles in a row (sequence, head, tile, unit),
@@ -1106,9 +1152,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     __shared__ int found_seq, left, take;
     __shared__ bool begins;
     __shared__ Piece x;
-    __shared__ __align__(8) uint64_t bars[2 * kStages];
+    __shared__ Copies copies;
     uint32_t unit_no = 0;
-    init_bars(bars);
+    init_copies(copies);
     constexpr int kThreads = kAttnWarps * 32;
     pdl_enter();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1207,7 +1253,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
         }
         __syncthreads();
         if (take == 0) return;
-        attend_piece<T, D, NT>(p, x, smem, bars, unit_no);
+        if (!attend_piece<T, D, NT>(p, x, smem, copies, unit_no)) return;
         join_warps<T, D, NT>(p, x, smem,
                          begins && take == x.q.units ? nullptr
                                                      : mine + sizeof(SplitHead) / 4 + (begins ? AttnLayout<D, NT>::kPart : 0));

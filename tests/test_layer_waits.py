@@ -10,12 +10,13 @@ import ctypes
 import os
 import shutil
 import subprocess
+import types
 
 import pytest
 import torch
 
 import build
-from rans_vectoradd import _C, fp8_linear
+from rans_vectoradd import _C, fp8_linear, kv4
 from rans_vectoradd._lib import DATA_TIMEOUT, LIB
 
 
@@ -60,3 +61,37 @@ def test_linear_reports_a_wait_of_its_epilogue_that_ran_out(cuda, tmp_path_facto
     # and the device goes on
     _C.data_status()
     assert torch.equal(fp8_linear.linear(x8, xs, w8, ws), want) and _C.data_status() == 0
+
+
+@pytest.fixture(scope="module")
+def no_copy_polls(tmp_path_factory):
+    lib = variant(tmp_path_factory, "kv4.cu", "TANS_B200_COPY_POLLS=0")
+    lib.tans_b200_kv4_attention.argtypes = LIB.tans_b200_kv4_attention.argtypes
+    return types.SimpleNamespace(tans_b200_kv4_attention=lib.tans_b200_kv4_attention,
+                                 tans_b200_kv4_attention_workspace_bytes=LIB.tans_b200_kv4_attention_workspace_bytes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [4, 16])  # tiles of 8 rows and of 16
+@pytest.mark.parametrize("lens", [[400, 1, 130], [9000, 3000]])  # the keys of a tile in one CTA, and cut
+def test_attention_reports_a_wait_for_copies_that_ran_out(cuda, monkeypatch, no_copy_polls, dim, group, lens):
+    page, counts = 64, [-(-n // 64) for n in lens]
+    cache = kv4.KV4Cache.allocate(sum(counts), 2, page, dim, cuda)
+    for t in (cache.k_codes, cache.v_codes):
+        t.random_(0, 256)
+    for t in (cache.k_scales, cache.v_scales):
+        t.fill_(0x30)
+    table = torch.zeros(len(lens), max(counts), dtype=torch.int32, device=cuda)
+    for b, c in enumerate(counts):
+        table[b, :c] = torch.arange(c) + sum(counts[:b])
+    n = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    q = torch.randn(len(lens), 2 * group, dim, device=cuda).to(torch.bfloat16)
+    _C.data_status()
+    want = kv4.attention(cache, q, table, n)
+    assert _C.data_status() == 0
+    with monkeypatch.context() as m:
+        m.setattr(kv4, "LIB", no_copy_polls)
+        kv4.attention(cache, q, table, n)
+        assert _C.data_status() == DATA_TIMEOUT
+    assert torch.equal(kv4.attention(cache, q, table, n), want) and _C.data_status() == 0
