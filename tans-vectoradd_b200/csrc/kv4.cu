@@ -474,6 +474,7 @@ struct Copies {
 // within three such limits.
 template <uint32_t kPolls = TANS_B200_COPY_POLLS, bool kLast = false>
 __device__ __forceinline__ bool wait_copies(uint32_t copies, int at, uint32_t parity, int32_t *status) {
+#pragma unroll 1
     for (uint32_t i = 0; i < kPolls; i++) {
         uint32_t done;
         asm volatile(
