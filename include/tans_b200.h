@@ -459,7 +459,8 @@ int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slots, void *k
  * before the first sequence's or after the last's, gets zeros and lse -inf.
  * Malformed starts, lens or pages set TANS_B200_DATA_BAD_INDEX
  * and read nothing out of bounds; the rows of a sequence whose starts are
- * malformed are not written.  workspace: caller-owned device memory,
+ * malformed (out of range, or more than most_new) get zeros and -inf too (where
+ * starts descend and sequences share rows, any of what they would hold).  workspace: caller-owned device memory,
  * 16-byte aligned, of tans_b200_kv4_attention_workspace_bytes() bytes (may be
  * 0); calls that overlap must not share it. */
 int tans_b200_kv4_attention_workspace_bytes(const tans_b200_kv4 *cache, int64_t q_heads,

@@ -406,18 +406,17 @@ struct AttendArgs {
 struct Sequence {
     int first, news, len, lo, hi;
     int tiles, units;  // units of one tile; at least one, which writes the zeros of rows that see nothing
+    bool refused;      // its rows of q are out of range or too many; it has none then
 };
 
 __device__ __forceinline__ Sequence sequence(const AttendArgs &p, int seq) {
-    Sequence s{seq, 1, 0, 0, 0, 0, 0};
+    Sequence s{seq, 1, 0, 0, 0, 0, 0, false};
     bool bad = false;
     if (p.starts) {
         s.first = p.starts[seq];
-        s.news = p.starts[seq + 1] - s.first;
-        if (s.first < 0 || s.news < 0 || s.news > p.most_new || s.first > p.tokens - s.news) {
-            bad = true;
-            s.news = 0;
-        }
+        const int next = p.starts[seq + 1];
+        bad = s.refused = s.first < 0 || next < s.first || next - s.first > p.most_new || next > p.tokens;
+        s.news = bad ? 0 : next - s.first;
     }
     s.len = p.lens[seq];
     const int64_t room = (int64_t)p.max_pages << p.cache.page_log2;
@@ -1084,19 +1083,29 @@ __device__ __forceinline__ void init_copies(Copies &c) {
     asm volatile("fence.mbarrier_init.release.cluster;");
 }
 
-// The rows of q that lie before the first sequence's and after the last's see
-// nothing: zeros and -inf, by all CTAs of a launch.
+// Zeros and -inf in a row of q that sees nothing.
+template <typename T, int D>
+__device__ __forceinline__ void clear_row(const AttendArgs &p, int64_t i) {
+    const int q_heads = p.cache.heads * p.group;
+    const int64_t row = i * q_heads;
+    uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * D);
+    for (int j = threadIdx.x; j < q_heads * (D / 8); j += blockDim.x) out[j] = uint4{};
+    for (int j = threadIdx.x; p.lse && j < q_heads; j += blockDim.x) p.lse[row + j] = -INFINITY;
+}
+
+// The rows of q that lie before the first sequence's and after the last's, by all CTAs of a launch.
 template <typename T, int D>
 __device__ __forceinline__ void clear_spare_rows(const AttendArgs &p, int64_t cta, int64_t ctas) {
     if (!p.starts) return;
     const int first = min(max(p.starts[0], 0), p.tokens), last = min(max(p.starts[p.seqs], first), p.tokens);
-    const int q_heads = p.cache.heads * p.group;
-    for (int64_t i = cta; i < p.tokens - (last - first); i += ctas) {
-        const int64_t row = (i < first ? i : i - first + last) * q_heads;
-        uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(p.out) + row * D);
-        for (int j = threadIdx.x; j < q_heads * (D / 8); j += blockDim.x) out[j] = uint4{};
-        for (int j = threadIdx.x; p.lse && j < q_heads; j += blockDim.x) p.lse[row + j] = -INFINITY;
-    }
+    for (int64_t i = cta; i < p.tokens - (last - first); i += ctas) clear_row<T, D>(p, i < first ? i : i - first + last);
+}
+
+// The rows of a sequence that sequence() refuses, as far as they exist, by one CTA.
+template <typename T, int D>
+__device__ __forceinline__ void clear_refused_rows(const AttendArgs &p, int seq) {
+    const int last = min(p.starts[seq + 1], p.tokens);
+    for (int i = max(p.starts[seq], 0); i < last; i++) clear_row<T, D>(p, i);
 }
 
 // One CTA a (tile, head, sequence), over all its keys.
@@ -1112,7 +1121,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
                            (int64_t)gridDim.x * gridDim.y * gridDim.z);
     if (p.seqs == 0) return;
     const Sequence q = sequence(p, blockIdx.z);
-    if ((int)blockIdx.x * p.tile_rows >= q.news * p.group) return;
+    if ((int)blockIdx.x * p.tile_rows >= q.news * p.group) {
+        if (q.refused && blockIdx.x == 0 && blockIdx.y == 0) clear_refused_rows<T, D>(p, blockIdx.z);
+        return;
+    }
     if (threadIdx.x < 32) {
         if (threadIdx.x == 0) {
             x.q = q;
@@ -1138,7 +1150,8 @@ constexpr int kTileCost = 2;
 struct SplitHead {
     int32_t pieces;  // 0: none
     int32_t seq, head, row0, rows, first;
-    int32_t pad[2];
+    int32_t refused;  // the rows of some sequence of the call are refused
+    int32_t pad;
 };
 
 template <int D, int NT>
@@ -1161,10 +1174,11 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     float *mine = p.parts + blockIdx.x * split_floats<D, NT>();
     SplitHead *info = reinterpret_cast<SplitHead *>(mine);
-    if (tid == 0) info->pieces = 0;
+    bool refusals = false;  // this thread's, then the call's
     const auto units_of = [&](int seq) -> int64_t {
         if (seq >= p.seqs) return 0;
         const Sequence s = sequence(p, seq);
+        refusals |= s.refused;
         return (int64_t)s.tiles * (s.units + kTileCost) * p.cache.heads;
     };
     // Units of the 128 sequences from b0 on: this thread's own, those before it,
@@ -1181,7 +1195,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
             if (lane >= o) inc += v;
         }
         if (lane == 31) warp_sum[warp] = inc;
-        __syncthreads();
+        refusals = __syncthreads_or(refusals);
         c.before = inc - c.own;
 #pragma unroll
         for (int w = 0; w < kAttnWarps; w++) {
@@ -1199,6 +1213,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
     const int64_t per = ceil_div<int64_t>(total, gridDim.x);
     const int64_t u = per * blockIdx.x;
     const int64_t u_end = u + per < total ? u + per : total;
+    if (tid == 0) *info = SplitHead{0, 0, 0, 0, 0, 0, refusals, 0};
     if (u >= u_end) return;
     // the sequence in which unit u lies, and that sequence's first unit
     Counted c = first;
@@ -1245,7 +1260,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, AttnLayout<D, NT>::kCtas) att
                     x.k1 = x.k0 + take * kUnit;
                     if (begins && u1 < x.q.units)
                         *info = SplitHead{1 + (int)ceil_div<int64_t>(x.q.units - u1, per), x.seq, x.head, x.row0,
-                                          min(p.tile_rows, x.q.news * p.group - x.row0), x.q.first, {0, 0}};
+                                          min(p.tile_rows, x.q.news * p.group - x.row0), x.q.first, refusals, 0};
                     break;
                 }
             }
@@ -1278,6 +1293,9 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
     clear_spare_rows<T, D>(p, blockIdx.x + (int64_t)gridDim.x * blockIdx.y, (int64_t)gridDim.x * gridDim.y);
     const int slot = threadIdx.x >> 7, turn = threadIdx.x >> 5 & 3, lane = threadIdx.x & 31;
     const int r = blockIdx.y * kJoinRows + slot;
+    if (h.refused && blockIdx.y == 0)
+        for (int seq = blockIdx.x; seq < p.seqs; seq += gridDim.x)
+            if (sequence(p, seq).refused) clear_refused_rows<T, D>(p, seq);
     if (h.pieces == 0 || (int)blockIdx.y * kJoinRows >= h.rows) return;
     const bool real = r < h.rows;
     float m = -INFINITY, l = 0.f, v[D / 32] = {};

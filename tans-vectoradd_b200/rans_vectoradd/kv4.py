@@ -195,8 +195,10 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     most most_new of them; without it every sequence has one.  Causal: the i-th
     of n new tokens sees keys up to lens - n + i, only the last `window` of them
     if window > 0.  scale defaults to dim ** -0.5.  A token that sees nothing,
-    and a row of q outside starts, gets zeros.  With return_lse also the f32 [tokens, q_heads] logarithm of the
-    sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
+    and a row of q outside starts, gets zeros; so do the rows of a sequence that
+    starts gives more than most_new tokens or rows that q has not, which
+    data_status() tells.  With return_lse also the f32 [tokens, q_heads] logarithm
+    of the sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
     least `attention_workspace_bytes`, else allocated."""
     dt, dev, D = q.dtype, cache._dev, cache._dim
     if dt not in _HALF:
