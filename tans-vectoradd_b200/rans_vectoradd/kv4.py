@@ -29,10 +29,12 @@ _HALF = {torch.bfloat16: 0, torch.float16: 1}
 _FLOAT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-@dataclass
+@dataclass(init=False)
 class KV4Cache:
     """k/v codes u8 [pages, heads, page_size, dim/2] and e4m3 scales u8
-    [pages, heads, page_size, dim/16]; optional f32 gains [heads]."""
+    [pages, heads, page_size, dim/16]; optional f32 gains [heads].  A field may be
+    set to another tensor that fits the rest (gains found after the cache was
+    made), which the next call then uses; other shapes need another cache."""
     k_codes: torch.Tensor
     k_scales: torch.Tensor
     v_codes: torch.Tensor
@@ -40,8 +42,11 @@ class KV4Cache:
     k_gain: torch.Tensor | None = None
     v_gain: torch.Tensor | None = None
 
-    def __post_init__(self):
-        kc, ks, vc, vs = self.k_codes, self.k_scales, self.v_codes, self.v_scales
+    def __init__(self, k_codes, k_scales, v_codes, v_scales, k_gain=None, v_gain=None):
+        self._bind(k_codes, k_scales, v_codes, v_scales, k_gain, v_gain)
+
+    def _bind(self, kc, ks, vc, vs, kg, vg):
+        """Checks the fields and takes them, with what the calls pass of them, all or none."""
         shape, u8 = kc.shape, torch.uint8
         if len(shape) != 4 or shape[3] not in (32, 64, 128):
             raise RuntimeError("codes must be [pages, heads, page_size, dim/2] with dim 64, 128 or 256")
@@ -55,15 +60,26 @@ class KV4Cache:
                 or not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous())):
             raise RuntimeError("cache arrays must be contiguous CUDA uint8, codes [.., dim/2] and scales [.., dim/16], "
                                "on one device")
-        for t in (self.k_gain, self.v_gain):
+        for t in (kg, vg):
             if t is not None:
                 _req(t.dtype == torch.float32 and t.shape == (heads,) and t.is_contiguous() and t.device == dev,
                      "gains must be contiguous f32 [heads]")
-        self._c = KV4(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), ptr(self.k_gain), ptr(self.v_gain),
-                      pages, heads, size, 2 * half)
-        self._ref = ctypes.addressof(self._c)
-        # what every call asks for, as plain attributes (a ctypes field takes longer to read)
-        self._dev, self._kv_heads, self._page, self._dim = dev, heads, size, 2 * half
+        c = KV4(kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), ptr(kg), ptr(vg), pages, heads, size, 2 * half)
+        # (_dev and so on: what every call asks for; a ctypes field takes longer to read)
+        self.__dict__.update(k_codes=kc, k_scales=ks, v_codes=vc, v_scales=vs, k_gain=kg, v_gain=vg,
+                             _c=c, _ref=ctypes.addressof(c), _dev=dev, _kv_heads=heads, _page=size, _dim=2 * half)
+
+    def __setattr__(self, name: str, value) -> None:
+        fields = self.__dataclass_fields__
+        if name in fields:
+            self._bind(*(value if f == name else getattr(self, f) for f in fields))
+        else:
+            object.__setattr__(self, name, value)
+
+    def __delattr__(self, name: str) -> None:
+        if name in self.__dataclass_fields__:
+            raise AttributeError(f"{name} cannot be deleted; gains may be set to None")
+        object.__delattr__(self, name)
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page_size: int = 64, head_dim: int = 128,
