@@ -214,8 +214,8 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
     and a row of q outside starts, gets zeros; so do the rows of a sequence that
     starts gives more than most_new tokens or rows that q has not, which
     data_status() tells.  With return_lse also the f32 [tokens, q_heads] logarithm
-    of the sum of exponentials (-inf where nothing is seen).  `workspace`: uint8 of at
-    least `attention_workspace_bytes`, else allocated."""
+    of the sum of exponentials (-inf where nothing is seen).  `workspace`: contiguous
+    uint8 of at least `attention_workspace_bytes`, else allocated."""
     dt, dev, D = q.dtype, cache._dev, cache._dim
     if dt not in _HALF:
         raise RuntimeError("q must be bfloat16 or float16")
@@ -231,7 +231,10 @@ def attention(cache: KV4Cache, q: torch.Tensor, table: torch.Tensor, lens: torch
         out = torch.empty(T, H, D, dtype=dt, device=dev)
         lse = torch.empty(T, H, dtype=torch.float32, device=dev) if return_lse else None
         need = attention_workspace_bytes(cache._kv_heads, cache._page, D, H, P, B, T, most_new, window, dev)
-        if need and workspace is None:
+        if workspace is not None:
+            _req(workspace.dtype == torch.uint8 and workspace.is_contiguous() and workspace.device == dev,
+                 "workspace must be a contiguous uint8 tensor on the cache's device")
+        elif need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
         check(LIB.tans_b200_kv4_attention(
