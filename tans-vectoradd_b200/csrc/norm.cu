@@ -34,7 +34,6 @@ struct NormArgs {
     int32_t cols;
     float eps;
     bool weight_f32;
-    bool norm;
     bool weight_vec = false;  // the weight has x's type and begins on a 16-byte boundary
 };
 
@@ -60,15 +59,25 @@ __device__ __forceinline__ void block_reduce(float &a, float &b, float2 *buf) {
 }
 
 // From a row's sum of squares and max|s * w|: what brings s * w to y, or to
-// y / scale when quantising, and the scale.  There the root cancels, y / scale
-// = s * w * 448 / max|s * w|, one rounding less; sizes far out of range (and
+// y / scale when quantising a norm, and the scale.  There the root cancels, y /
+// scale = s * w * 448 / max|s * w|, one rounding less; sizes far out of range (and
 // NaN) take the long way.
+template <bool kNorm>
 __device__ __forceinline__ float row_factor(const NormArgs &p, float sumsq, float amax, float &scale) {
-    const float inv = p.norm ? rsqrtf(sumsq / (float)p.cols + p.eps) : 1.f;
+    const float inv = kNorm ? rsqrtf(sumsq / (float)p.cols + p.eps) : 1.f;
     if (!p.q) return inv;
     const float top = amax * inv;
     scale = top == 0.f ? 1.f : max_nan(top / 448.f, 1.17549435e-38f);
     return amax > 1e-30f && amax < 1e30f && top > 1e-30f ? 448.f / amax : inv / scale;
+}
+
+// s * w as y, or as y / scale when quantising, from row_factor's f and scale.
+// Without a norm y is x, whose few bits make ties of two e4m3 values common: its
+// quotient by the scale is rounded once (by a factor 448 / max|x| 317 of 2 million
+// bf16 values came out on the other side of a tie).
+template <bool kNorm>
+__device__ __forceinline__ float scaled(float sw, float f, float scale) {
+    return kNorm ? sw * f : sw / scale;
 }
 
 // Elements o .. o + 7 of the sixteen in a and b, 0 < o < 8, the same o in all lanes.
@@ -105,13 +114,13 @@ __device__ __forceinline__ Eight<T> window(const Eight<T> &a, const Eight<T> &b,
 // its ends are one each of the block's first 16 threads, and the weight, which lies
 // otherwise, is cut out of two of its own vectors (one of another type or off
 // its boundary: read one by one).
-template <typename T, int VPT, int kMost, bool kShifted>
+template <typename T, int VPT, int kMost, bool kShifted, bool kNorm>
 __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     __shared__ float2 buf[32];
     pdl_enter();
     const int64_t row = blockIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
-    const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
+    const T *r = kNorm && p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
     constexpr int kPer = 16 / (int)sizeof(T);
     const int head = kShifted ? min((kPer - (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % kPer)) % kPer, p.cols) : 0;
     const int vecs = (p.cols - head) / 8;
@@ -123,7 +132,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     if (has_end) {
         at_end = to_f32(x[end]);
         if (r) at_end += to_f32(r[end]);
-        if (p.norm) w_end = p.weight_f32 ? static_cast<const float *>(p.weight)[end] : to_f32(wt[end]);
+        if (kNorm) w_end = p.weight_f32 ? static_cast<const float *>(p.weight)[end] : to_f32(wt[end]);
     }
     // every load of the row before the first use of one
     Eight<T> xv[VPT], rv[VPT], wv[VPT];
@@ -133,7 +142,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
         if (v < vecs) {
             xv[i] = load_eight(x + head + 8 * v);
             if (r) rv[i] = load_eight(r + head + 8 * v);
-            if (!kShifted && p.norm && !p.weight_f32) wv[i] = load_eight(wt + 8 * v);
+            if (!kShifted && kNorm && !p.weight_f32) wv[i] = load_eight(wt + 8 * v);
         }
     }
     float s[VPT][8];
@@ -150,7 +159,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
                 for (int k = 0; k < 8; k++) s[i][k] += a[k];
                 store8(static_cast<T *>(p.h) + row * p.h_stride + head + 8 * v, s[i]);
             }
-            if (p.norm) {
+            if (kNorm) {
                 float w[8];
                 if constexpr (kShifted) {
                     if (p.weight_vec && (head == 0 || 8 * v + 16 <= p.cols)) {
@@ -183,17 +192,17 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
     }
     if (has_end) {
         if (r) static_cast<T *>(p.h)[row * p.h_stride + end] = from_f32<T>(at_end);
-        if (p.norm) sumsq = __fmaf_rn(at_end, at_end, sumsq);
+        if (kNorm) sumsq = __fmaf_rn(at_end, at_end, sumsq);
         at_end *= w_end;
         if (p.q) amax = max_nan(amax, fabsf(at_end));
     }
     block_reduce(sumsq, amax, buf);
     float scale;
-    const float f = row_factor(p, sumsq, amax, scale);
+    const float f = row_factor<kNorm>(p, sumsq, amax, scale);
     if (p.q && threadIdx.x == 0) p.scale[row] = scale;
     if (has_end) {
         if (p.q)
-            p.q[row * p.cols + end] = (uint8_t)e4m3x2(at_end * f, 0.f);
+            p.q[row * p.cols + end] = (uint8_t)e4m3x2(scaled<kNorm>(at_end, f, scale), 0.f);
         else
             static_cast<T *>(p.y)[row * p.cols + end] = from_f32<T>(at_end * f);
     }
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
         const int v = threadIdx.x + i * blockDim.x;
         if (v < vecs) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) s[i][k] *= f;
+            for (int k = 0; k < 8; k++) s[i][k] = scaled<kNorm>(s[i][k], f, scale);
             if (p.q) {
                 uint2 u;
                 u.x = e4m3x2(s[i][0], s[i][1]) | e4m3x2(s[i][2], s[i][3]) << 16;
@@ -224,14 +233,14 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
 // Wider rows, and rows of tensors that lie to 16-byte boundaries each in its own
 // way: element by element, s * w kept in shared memory (1021 x 4099 f16: 9.7 us
 // out of L2, where vectors take 5.5; bound by its 2-byte accesses).
-template <typename T>
+template <typename T, bool kNorm>
 __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
     extern __shared__ float srow[];
     __shared__ float2 buf[32];
     pdl_enter();
     const int64_t row = blockIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.x_stride;
-    const T *r = p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
+    const T *r = kNorm && p.residual ? static_cast<const T *>(p.residual) + row * p.r_stride : nullptr;
     T *h = r ? static_cast<T *>(p.h) + row * p.h_stride : nullptr;
     float sumsq = 0.f, amax = 0.f;
     for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
@@ -241,17 +250,17 @@ __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
             h[c] = from_f32<T>(s);
         }
         sumsq += s * s;
-        if (p.norm)
+        if (kNorm)
             s *= p.weight_f32 ? static_cast<const float *>(p.weight)[c] : to_f32(static_cast<const T *>(p.weight)[c]);
         amax = max_nan(amax, fabsf(s));
         srow[c] = s;
     }
     block_reduce(sumsq, amax, buf);
     float scale;
-    const float f = row_factor(p, sumsq, amax, scale);
+    const float f = row_factor<kNorm>(p, sumsq, amax, scale);
     if (p.q && threadIdx.x == 0) p.scale[row] = scale;
     for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
-        const float y = srow[c] * f;
+        const float y = scaled<kNorm>(srow[c], f, scale);
         if (p.q)
             p.q[row * p.cols + c] = (uint8_t)e4m3x2(y, 0.f);
         else
@@ -261,7 +270,7 @@ __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
 
 constexpr int kMaxCols = 56 * 1024;  // f32 values of one row that fit a CTA's shared memory
 
-template <typename T>
+template <typename T, bool kNorm>
 int launch_norm(NormArgs p, int64_t rows, cudaStream_t st) {
     p.weight_vec = is_aligned(p.weight, 16) && (!p.weight_f32 || sizeof(T) == 4);
     constexpr int64_t kPer = 16 / (int64_t)sizeof(T);  // elements between boundaries
@@ -282,9 +291,9 @@ int launch_norm(NormArgs p, int64_t rows, cudaStream_t st) {
     if (!vec && !shifted) {
         const int threads = p.cols >= 1024 ? 512 : (p.cols >= 256 ? 128 : 32);
         const int smem = p.cols * 4;
-        const int rc = allow_smem<norm_any_kernel<T>>("norm_any_kernel", kMaxCols * 4);
+        const int rc = allow_smem<norm_any_kernel<T, kNorm>>("norm_any_kernel", kMaxCols * 4);
         if (rc) return rc;
-        return launch_ex(norm_any_kernel<T>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
+        return launch_ex(norm_any_kernel<T, kNorm>, grid, dim3(threads), smem, 1, st, "norm_any_kernel", p);
     }
     const int vecs = p.cols < 8 ? 1 : p.cols / 8;
     // four vectors a thread: a row's loads are in flight at once, with many rows resident
@@ -292,10 +301,14 @@ int launch_norm(NormArgs p, int64_t rows, cudaStream_t st) {
     const auto launch = [&](auto kernel) {
         return launch_ex(kernel, grid, dim3(threads), 0, 1, st, "norm_vec_kernel", p);
     };
-    if (vecs <= threads) return vec ? launch(norm_vec_kernel<T, 1, 32, false>) : launch(norm_vec_kernel<T, 1, 32, true>);
-    if (vecs <= 2 * threads) return vec ? launch(norm_vec_kernel<T, 2, 32, false>) : launch(norm_vec_kernel<T, 2, 32, true>);
-    if (threads <= 256) return vec ? launch(norm_vec_kernel<T, 4, 256, false>) : launch(norm_vec_kernel<T, 4, 256, true>);
-    return vec ? launch(norm_vec_kernel<T, 4, 1024, false>) : launch(norm_vec_kernel<T, 4, 1024, true>);
+    const auto form = [&](auto shifted) {
+        constexpr bool S = decltype(shifted)::value;
+        if (vecs <= threads) return launch(norm_vec_kernel<T, 1, 32, S, kNorm>);
+        if (vecs <= 2 * threads) return launch(norm_vec_kernel<T, 2, 32, S, kNorm>);
+        if (threads <= 256) return launch(norm_vec_kernel<T, 4, 256, S, kNorm>);
+        return launch(norm_vec_kernel<T, 4, 1024, S, kNorm>);
+    };
+    return vec ? form(std::false_type{}) : form(std::true_type{});
 }
 
 int check_rows(const char *what, int64_t rows, int64_t cols) {
@@ -324,9 +337,9 @@ extern "C" int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const voi
         return fail(TANS_B200_ERR_INVALID, "add_rms_norm: the weight must have x's type or be f32");
     if (!(eps >= 0.f)) return fail(TANS_B200_ERR_INVALID, "add_rms_norm: eps must not be negative");
     NormArgs p{x, residual, weight, x_stride, r_stride, h_stride, residual ? h : nullptr, y, q, scale,
-               (int32_t)cols, eps, weight_dtype == TANS_B200_F32, true};
+               (int32_t)cols, eps, weight_dtype == TANS_B200_F32};
     return dispatch_float(dtype, "add_rms_norm", [&](auto t) {
-        return launch_norm<decltype(t)>(p, rows, (cudaStream_t)stream);
+        return launch_norm<decltype(t), true>(p, rows, (cudaStream_t)stream);
     });
 }
 
@@ -337,8 +350,8 @@ extern "C" int tans_b200_quantize_tokens(const void *x, int64_t x_stride, uint8_
     if (rc) return rc;
     if (rows == 0) return TANS_B200_OK;
     if (!x || !q || !scale) return fail(TANS_B200_ERR_INVALID, "quantize_tokens: null pointer");
-    NormArgs p{x, nullptr, nullptr, x_stride, 0, 0, nullptr, nullptr, q, scale, (int32_t)cols, 0.f, false, false};
+    NormArgs p{x, nullptr, nullptr, x_stride, 0, 0, nullptr, nullptr, q, scale, (int32_t)cols, 0.f, false};
     return dispatch_float(dtype, "quantize_tokens", [&](auto t) {
-        return launch_norm<decltype(t)>(p, rows, (cudaStream_t)stream);
+        return launch_norm<decltype(t), false>(p, rows, (cudaStream_t)stream);
     });
 }
