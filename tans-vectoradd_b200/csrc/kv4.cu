@@ -366,9 +366,10 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //  * O^T: lane (g, t) takes the g-th eighth of D of the four keys of its P^T
 //    fragment; merging the nibbles of two keys gives bytes whose conversion is
 //    the f16 pair (key, other key) of one element, two elements a MMA.
-// code * scale is exact in f16; P enters in f16 relative to a maximum that may
-// lag by up to 2^8; sums, maxima and O stay in f32 (sums by an MMA over the
-// rounded P were no faster and cost the lse its last bits).  bf16 queries become
+// code * scale is exact in f16; P enters in f16 relative to 2^-7 of a maximum that
+// may lag by up to 2^8: at most 2^15, and a weight errs by at most 2^-32 of the row's
+// largest where it is below f16's normal range.  Sums, maxima and O stay in f32
+// (sums by an MMA over the rounded P were no faster and cost the lse its last bits).  bf16 queries become
 // f16 after a power of two per row that brings their largest element to 2^14: an
 // element loses bits only below 2^-28 of that.
 //
@@ -384,6 +385,8 @@ constexpr int kBlockKeys = 32;                  // keys a warp takes at a time
 constexpr int kUnit = kBlockKeys * kAttnWarps;  // keys
 constexpr int kStages = 2;                      // units in shared memory: one in work, one on its way
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLag = 8.f;       // log2 of what a score may pass the maximum in use by
+constexpr float kHeadroom = 7.f;  // log2 of the weight of a score that equals it; kLag + kHeadroom is below f16's 16
 
 struct AttendArgs {
     Cache cache;
@@ -744,7 +747,8 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
     for (int j = 0; j < kTiles; j++)
 #pragma unroll
         for (int n = 0; n < NT; n++) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
-    // scores up to `limit` need no new maximum; `less` is subtracted; the sums are this lane's keys'
+    // scores up to `limit` need no new maximum; `less`, kHeadroom below the last one, is
+    // subtracted; the sums are this lane's keys'
     float limit[NT][2], less[NT][2], sum[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
@@ -859,11 +863,11 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const float top = limit[n][i] == -INFINITY ? -INFINITY : less[n][i];
-                        float v = fmaxf(m[n][i], top);
+                        float v = fmaxf(m[n][i], top + kHeadroom);
 #pragma unroll
                         for (int lanes = 4; lanes < 32; lanes *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
-                        limit[n][i] = v + 8.f;
-                        less[n][i] = v == -INFINITY ? 0.f : v;
+                        limit[n][i] = v + kLag;
+                        less[n][i] = v == -INFINITY ? 0.f : v - kHeadroom;
                         const float f = exp2f(top - less[n][i]);  // nothing to scale yet while top is -inf
                         sum[n][i] *= f;
 #pragma unroll
@@ -1015,14 +1019,14 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
     return true;
 }
 
-// The factor that brings a part with maximum `top` and sum `sum` to the common
-// maximum m (0 where it is -inf); a part that saw nothing has factor 0, one
+// The factor that brings a part whose weights are relative to `top`, with sum `sum`,
+// to the common m (0 where it is -inf); a part that saw nothing has factor 0, one
 // whose scores are all NaN keeps its NaN.
 __device__ __forceinline__ float part_factor(float top, float sum, float m) {
     return top == -INFINITY && sum == 0.f ? 0.f : exp2f(top - (m == -INFINITY ? 0.f : m));
 }
 
-// One row of the output from its sum l and O v, both relative to the maximum m; a lane has every 32nd element.
+// One row of the output from its sum l and O v, both relative to m; a lane has every 32nd element.
 template <typename T, int D>
 __device__ __forceinline__ void write_row(const AttendArgs &p, int head, int heads, int64_t token, int in_group, float m,
                                           float l, const float (&v)[D / 32]) {
