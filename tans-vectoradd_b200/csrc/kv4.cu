@@ -866,8 +866,9 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
                         float v = fmaxf(m[n][i], top + kHeadroom);
 #pragma unroll
                         for (int lanes = 4; lanes < 32; lanes *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
-                        limit[n][i] = v + kLag;
                         less[n][i] = v == -INFINITY ? 0.f : v - kHeadroom;
+                        // (past 2^26 the two sums round, together to as much as f16's end)
+                        limit[n][i] = v + kLag - less[n][i] > kLag + kHeadroom ? v : v + kLag;
                         const float f = exp2f(top - less[n][i]);  // nothing to scale yet while top is -inf
                         sum[n][i] *= f;
 #pragma unroll
