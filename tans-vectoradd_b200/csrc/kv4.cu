@@ -1381,7 +1381,7 @@ int make_plan(const Cache &c, int64_t q_heads, int64_t max_pages, int64_t seqs, 
     plan->rows = (int)(most_new * (q_heads / c.heads));
     plan->tile_rows = plan->rows <= 8 ? 8 : 16;
     int64_t keys = max_pages << c.page_log2;
-    if (window > 0 && window + most_new < keys) keys = window + most_new;
+    if (window > 0 && window < keys - most_new) keys = window + most_new;
     const int64_t units = ceil_div<int64_t>(keys, kUnit) + 1;
     const int64_t all = seqs * c.heads * ceil_div(plan->rows, plan->tile_rows) * units;
     dispatch_tile(c.dim, plan->tile_rows, [&](auto d, auto nt) {
