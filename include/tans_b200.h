@@ -371,7 +371,8 @@ int tans_b200_decode_noalloc(const uint8_t *compressed, int64_t compressed_bytes
 /* ------------------------------------------------ decoder-layer operators
  *
  * What a decoder layer with e4m3 weights needs between and around its matrix
- * products (no counterpart in the reference).  Element types of activations:
+ * products (no counterpart in the reference).  Arrays are aligned to their
+ * elements where no more is asked.  Element types of activations:
  */
 #define TANS_B200_BF16 0
 #define TANS_B200_F16 1

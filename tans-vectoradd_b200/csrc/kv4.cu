@@ -1424,6 +1424,7 @@ int check_cache(const char *what, const tans_b200_kv4 *c, Cache *out) {
     if (!is_aligned(c->k_codes, 16) || !is_aligned(c->v_codes, 16) || !is_aligned(c->k_scales, 16) ||
         !is_aligned(c->v_scales, 16))
         return fail(TANS_B200_ERR_INVALID, "%s: cache arrays must be 16-byte aligned", what);
+    if (!may_hold(4, c->k_gain, c->v_gain)) return fail(TANS_B200_ERR_INVALID, "%s: gains must be 4-byte aligned", what);
     *out = Cache{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->k_gain, c->v_gain, c->pages,
                  (int32_t)c->heads, __builtin_ctz((unsigned)c->page_size), (int32_t)c->dim};
     return TANS_B200_OK;
@@ -1454,6 +1455,8 @@ extern "C" int tans_b200_kv4_append(const tans_b200_kv4 *cache, const void *k, i
     if (!is_aligned(k, 16) || !is_aligned(v, 16) || !is_aligned(q, 16) || !is_aligned(q_out, 16) || !is_aligned(cos, 16) || !is_aligned(sin, 16) || k_stride % 8 ||
         v_stride % 8 || (q && q_stride % 8))
         return fail(TANS_B200_ERR_INVALID, "kv4_append: q, k, v, cos and sin must be 16-byte aligned, the strides multiples of 8");
+    if (!may_hold(8, slots, positions) || !may_hold(4, status))
+        return fail(TANS_B200_ERR_INVALID, "kv4_append: an array is not aligned to its elements");
     p.q = q;
     p.k = k;
     p.v = v;
@@ -1511,6 +1514,8 @@ extern "C" int tans_b200_kv4_read(const tans_b200_kv4 *cache, const int64_t *slo
     if (tokens == 0) return TANS_B200_OK;
     if (!slots || !k || !v || !is_aligned(k, 16) || !is_aligned(v, 16))
         return fail(TANS_B200_ERR_INVALID, "kv4_read: slots, and k and v 16-byte aligned, are needed");
+    if (!may_hold(8, slots) || !may_hold(4, status))
+        return fail(TANS_B200_ERR_INVALID, "kv4_read: an array is not aligned to its elements");
     int sms;
     rc = current_sms("kv4_read", &sms);
     if (rc) return rc;
@@ -1580,6 +1585,8 @@ extern "C" int tans_b200_kv4_attention(const tans_b200_kv4 *cache, const void *q
     if (!q || !out || (seqs && (!lens || (!table && max_pages))) || !is_aligned(q, 16) || q_stride % 8 || !is_aligned(out, 16))
         return fail(TANS_B200_ERR_INVALID,
                     "kv4_attention: q, out (16-byte aligned, q's stride a multiple of 8), lens and table are needed");
+    if (!may_hold(4, table, lens, starts, lse, status))
+        return fail(TANS_B200_ERR_INVALID, "kv4_attention: an array is not aligned to its elements");
     rc = make_plan(p.cache, q_heads, max_pages, seqs, most_new, window, &plan);
     if (rc) return rc;
     if (workspace_bytes < plan.floats * 4 || (plan.ctas && (!workspace || !is_aligned(workspace, 16))))

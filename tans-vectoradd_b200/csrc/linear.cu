@@ -763,6 +763,8 @@ extern "C" int tans_b200_linear(const uint8_t *x, const float *x_scale, const ui
     if (m == 0) return TANS_B200_OK;
     if (!x || !x_scale || !w || !w_scale || !y || !is_aligned(x, 16) || !is_aligned(w, 16))
         return fail(TANS_B200_ERR_INVALID, "linear: x and w (16-byte aligned), their scales and y are needed");
+    if (!may_hold(4, x_scale, w_scale, status) || !may_hold(element_bytes(dtype), bias, mul, residual, y))
+        return fail(TANS_B200_ERR_INVALID, "linear: an array is not aligned to its elements");
     LinearArgs p{};
     p.x_scale = x_scale;
     p.w_scale = w_scale;

@@ -335,6 +335,8 @@ extern "C" int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const voi
                     "add_rms_norm: x, weight, h with a residual, and either y or q and scale are needed");
     if (weight_dtype != dtype && weight_dtype != TANS_B200_F32)
         return fail(TANS_B200_ERR_INVALID, "add_rms_norm: the weight must have x's type or be f32");
+    if (!may_hold(element_bytes(dtype), x, residual, h, y) || !may_hold(element_bytes(weight_dtype), weight) || !may_hold(4, scale))
+        return fail(TANS_B200_ERR_INVALID, "add_rms_norm: an array is not aligned to its elements");
     if (!(eps >= 0.f)) return fail(TANS_B200_ERR_INVALID, "add_rms_norm: eps must not be negative");
     NormArgs p{x, residual, weight, x_stride, r_stride, h_stride, residual ? h : nullptr, y, q, scale,
                (int32_t)cols, eps, weight_dtype == TANS_B200_F32};
@@ -350,6 +352,8 @@ extern "C" int tans_b200_quantize_tokens(const void *x, int64_t x_stride, uint8_
     if (rc) return rc;
     if (rows == 0) return TANS_B200_OK;
     if (!x || !q || !scale) return fail(TANS_B200_ERR_INVALID, "quantize_tokens: null pointer");
+    if (!may_hold(element_bytes(dtype), x) || !may_hold(4, scale))
+        return fail(TANS_B200_ERR_INVALID, "quantize_tokens: an array is not aligned to its elements");
     NormArgs p{x, nullptr, nullptr, x_stride, 0, 0, nullptr, nullptr, q, scale, (int32_t)cols, 0.f, false};
     return dispatch_float(dtype, "quantize_tokens", [&](auto t) {
         return launch_norm<decltype(t), false>(p, rows, (cudaStream_t)stream);

@@ -91,6 +91,12 @@ int allow_smem(const char *what, int bytes) {
 }
 
 inline bool is_aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+// whether elements of `size` bytes may lie at each of p (null: yes)
+template <typename... P>
+bool may_hold(uintptr_t size, const P *...p) {
+    return (is_aligned(p, size) && ...);
+}
+inline uintptr_t element_bytes(int dtype) { return dtype == TANS_B200_F32 ? 4 : 2; }
 
 template <typename I>
 __host__ __device__ constexpr I ceil_div(I a, I b) {
