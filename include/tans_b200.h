@@ -385,8 +385,8 @@ int tans_b200_decode_noalloc(const uint8_t *compressed, int64_t compressed_bytes
  *   scale[r] = max|y| / 448 (1 for a row of zeros), q = e4m3(y / scale).
  * x, residual, h: [rows][cols] with strides between rows in elements (the
  * last dimension dense); y, q: dense; weight: [cols] of x's type or f32.  h is
- * written only with a residual and may be x or residual itself.  A NaN makes
- * its row NaN.  cols: 1..57344.  dtype: any of the three. */
+ * written only with a residual and may be x or residual itself; its rows do not
+ * overlap.  A NaN makes its row NaN.  cols: 1..57344.  dtype: any of the three. */
 int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
                            int64_t r_stride, const void *weight, int weight_dtype, float eps,
                            void *h, int64_t h_stride, void *y, uint8_t *q, float *scale,

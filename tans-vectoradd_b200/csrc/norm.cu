@@ -337,6 +337,8 @@ extern "C" int tans_b200_add_rms_norm(const void *x, int64_t x_stride, const voi
         return fail(TANS_B200_ERR_INVALID, "add_rms_norm: the weight must have x's type or be f32");
     if (!may_hold(element_bytes(dtype), x, residual, h, y) || !may_hold(element_bytes(weight_dtype), weight) || !may_hold(4, scale))
         return fail(TANS_B200_ERR_INVALID, "add_rms_norm: an array is not aligned to its elements");
+    if (residual && rows > 1 && h_stride > -cols && h_stride < cols)
+        return fail(TANS_B200_ERR_INVALID, "add_rms_norm: the rows of h overlap");
     if (!(eps >= 0.f)) return fail(TANS_B200_ERR_INVALID, "add_rms_norm: eps must not be negative");
     NormArgs p{x, residual, weight, x_stride, r_stride, h_stride, residual ? h : nullptr, y, q, scale,
                (int32_t)cols, eps, weight_dtype == TANS_B200_F32};

@@ -1,9 +1,13 @@
-"""Arrays off their elements' alignment are refused by the decoder-layer entry points
-before any launch."""
+"""Arrays off their elements' alignment, and sums whose rows overlap, are refused by the
+decoder-layer entry points before any launch."""
 from __future__ import annotations
 
 import ctypes
 
+import pytest
+import torch
+
+from rans_vectoradd import fp8_linear
 from rans_vectoradd._lib import KV4, LIB
 
 P = 256  # an aligned address that is never followed
@@ -19,6 +23,8 @@ def test_norm_alignment():
     for kw in ({"x": P + 1}, {"r": P + 1}, {"w": P + 1}, {"h": P + 1}, {"s": P + 2}, {"y": P + 1, "q": None, "s": None},
                {"x": P + 2, "dt": 2, "wt": 2}, {"w": P + 2, "wt": 2}):
         refused(norm(**kw), "aligned")
+    for hs in (0, 1, 7, -7):
+        refused(norm(hs=hs), "overlap")
     refused(LIB.tans_b200_quantize_tokens(P + 1, 8, P, P, 1, 8, 0, None), "aligned")
     refused(LIB.tans_b200_quantize_tokens(P, 8, P, P + 2, 1, 8, 0, None), "aligned")
 
@@ -54,3 +60,20 @@ def test_kv4_alignment():
     refused(read(slots=P + 4), "aligned")
     for kw in ({"table": P + 2}, {"lens": P + 2}, {"starts": P + 1}, {"lse": P + 2}):
         refused(attend(**kw), "aligned")
+
+
+@pytest.mark.gpu
+def test_a_sum_in_the_place_of_a_broadcast_input_is_refused(cuda):
+    x, w = torch.randn(4, 64, device=cuda), torch.ones(64, device=cuda)
+    r = torch.randn(1, 64, device=cuda).expand(4, 64)
+    keep = r.clone()
+    with pytest.raises(RuntimeError, match="overlap"):
+        fp8_linear.add_rms_norm(x, w, r, residual_out=r)
+    with pytest.raises(RuntimeError, match="overlap"):
+        fp8_linear.add_rms_norm_e4m3(x, w, r, residual_out=torch.empty(64 + 3 * 8, device=cuda).as_strided((4, 64), (8, 1)))
+    assert torch.equal(r, keep)
+    y, h = fp8_linear.add_rms_norm(x, w, r)
+    assert torch.equal(h, x + r) and torch.isfinite(y).all()
+    one = r[:1]
+    fp8_linear.add_rms_norm(x[:1], w, one, residual_out=one)
+    assert torch.equal(one, x[:1] + keep[:1])
