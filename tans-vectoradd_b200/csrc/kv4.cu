@@ -601,7 +601,6 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
     constexpr int kE = D / 8;             // elements of an eighth of a head
     constexpr int kVS = (D + 127) / 128;  // scales of an eighth
     constexpr int kKS = D / 64;           // scales of a quarter
-    constexpr int kTogether = 2;  // halves of 16 keys worked on together
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int head = x.head, lo_all = x.lo_all;
     int k1 = x.k1;
@@ -778,208 +777,205 @@ __device__ __forceinline__ bool attend_piece(const AttendArgs &p, const Piece &x
             __syncwarp();
         }
         const bool edge = base < inner || base - inner > inner_span;
-#pragma unroll(2 / kTogether)
-        for (int y0 = 0; y0 < 2; y0 += kTogether) {
-            // ---- scores of the keys base + 16 y ..
-            float s[kTogether][NT][4];
+        // ---- scores of the keys base + 16 y .., both sixteens worked on together
+        float s[2][NT][4];
 #pragma unroll
-            for (int y = 0; y < kTogether; y++) {
-                uint32_t w[2][D / 32], f[2][kKS];
+        for (int y = 0; y < 2; y++) {
+            uint32_t w[2][D / 32], f[2][kKS];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int r = 16 * y + 8 * h + own_key;
+                const uint8_t *kp = blk + r * (D / 2) + t * (D / 8);
+                if constexpr (D == 64) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(kp);
+                    w[h][0] = v.x, w[h][1] = v.y;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 128; i++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(kp + 16 * i);
+                        w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
+                    }
+                }
+                const uint8_t *sp = scales + r * (D / 16) + t * kKS;
+                if constexpr (kKS == 1) {
+                    f[h][0] = e4m3x2_h2(*sp * 0x101u);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kKS; i += 2) {
+                        const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
+                        f[h][i] = __byte_perm(two, two, 0x1010);
+                        f[h][i + 1] = __byte_perm(two, two, 0x3232);
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[y][n][0] = s[y][n][1] = s[y][n][2] = s[y][n][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps / 2; i++) {
+                uint32_t a[2][4];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int r = 16 * (y0 + y) + 8 * h + own_key;
-                    const uint8_t *kp = blk + r * (D / 2) + t * (D / 8);
-                    if constexpr (D == 64) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(kp);
-                        w[h][0] = v.x, w[h][1] = v.y;
-                    } else {
+                    e2m1x8_h2(w[h][i], a[h]);
 #pragma unroll
-                        for (int i = 0; i < D / 128; i++) {
-                            const uint4 v = *reinterpret_cast<const uint4 *>(kp + 16 * i);
-                            w[h][4 * i] = v.x, w[h][4 * i + 1] = v.y, w[h][4 * i + 2] = v.z, w[h][4 * i + 3] = v.w;
-                        }
-                    }
-                    const uint8_t *sp = scales + r * (D / 16) + t * kKS;
-                    if constexpr (kKS == 1) {
-                        f[h][0] = e4m3x2_h2(*sp * 0x101u);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kKS; i += 2) {
-                            const uint32_t two = e4m3x2_h2(*reinterpret_cast<const uint16_t *>(sp + i));
-                            f[h][i] = __byte_perm(two, two, 0x1010);
-                            f[h][i + 1] = __byte_perm(two, two, 0x3232);
-                        }
-                    }
+                    for (int k = 0; k < 4; k++) a[h][k] = mul_h2(a[h][k], f[h][i / 2]);
                 }
 #pragma unroll
-                for (int n = 0; n < NT; n++) s[y][n][0] = s[y][n][1] = s[y][n][2] = s[y][n][3] = 0.f;
-#pragma unroll
-                for (int i = 0; i < kSteps / 2; i++) {
-                    uint32_t a[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        e2m1x8_h2(w[h][i], a[h]);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) a[h][k] = mul_h2(a[h][k], f[h][i / 2]);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const uint4 q = qs[(n * (kSteps / 2) + i) * 32 + lane];
-                        mma_f16(s[y][n], make_uint4(a[0][0], a[1][0], a[0][1], a[1][1]), q.x, q.y);
-                        mma_f16(s[y][n], make_uint4(a[0][2], a[1][2], a[0][3], a[1][3]), q.z, q.w);
-                    }
+                for (int n = 0; n < NT; n++) {
+                    const uint4 q = qs[(n * (kSteps / 2) + i) * 32 + lane];
+                    mma_f16(s[y][n], make_uint4(a[0][0], a[1][0], a[0][1], a[1][1]), q.x, q.y);
+                    mma_f16(s[y][n], make_uint4(a[0][2], a[1][2], a[0][3], a[1][3]), q.z, q.w);
                 }
             }
-            // ---- the running maximum and the weights
-            if (edge) {
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int last = x.hi[8 * n + 2 * t + i], lo = first_seen(p, last), hi = min(last, kend);
-#pragma unroll
-                        for (int y = 0; y < kTogether; y++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const int key = base + 16 * (y0 + y) + 8 * h + own_key;
-                                if (key < lo || key > hi) s[y][n][2 * h + i] = -INFINITY;
-                            }
-                    }
-            }
-            float m[NT][2];
-            bool grew = false;
+        }
+        // ---- the running maximum and the weights
+        if (edge) {
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    m[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
-                    if (kTogether == 2) m[n][i] = fmaxf(m[n][i], fmaxf(s[kTogether - 1][n][i], s[kTogether - 1][n][2 + i]));
-                    m[n][i] *= i ? to_log2[n].y : to_log2[n].x;
-                    grew |= m[n][i] > limit[n][i];
-                }
-            if (__any_sync(0xffffffffu, grew)) {
+                    const int last = x.hi[8 * n + 2 * t + i], lo = first_seen(p, last), hi = min(last, kend);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float top = limit[n][i] == -INFINITY ? -INFINITY : less[n][i];
-                        float v = fmaxf(m[n][i], top + kHeadroom);
-#pragma unroll
-                        for (int lanes = 4; lanes < 32; lanes *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
-                        less[n][i] = v == -INFINITY ? 0.f : v - kHeadroom;
-                        // (past 2^26 the two sums round, together to as much as f16's end)
-                        limit[n][i] = v + kLag - less[n][i] > kLag + kHeadroom ? v : v + kLag;
-                        const float f = exp2f(top - less[n][i]);  // nothing to scale yet while top is -inf
-                        sum[n][i] *= f;
-#pragma unroll
-                        for (int j = 0; j < kTiles; j++) {
-                            o[j][n][i] *= f;
-                            o[j][n][2 + i] *= f;
-                        }
-                    }
-            }
-            uint32_t pt[kTogether][NT][2];  // P^T fragments
-#pragma unroll
-            for (int y = 0; y < kTogether; y++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        s[y][n][c] = exp2_fast(__fmaf_rn(s[y][n][c], c & 1 ? to_log2[n].y : to_log2[n].x, -less[n][c & 1]));
-                        sum[n][c & 1] += s[y][n][c];
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
-                            : "=r"(pt[y][n][h])
-                            : "r"(h2_of(s[y][n][2 * h], s[y][n][2 * h + 1])));
-                }
-            // ---- values of the lane's four keys of each 16
-#pragma unroll
-            for (int y = 0; y < kTogether; y++) {
-                uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int r = 16 * (y0 + y) + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-                    const uint8_t *vp = blk + L::kCodes + r * (D / 2);
-                    if constexpr (D == 64) {
-                        w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
-                    } else if constexpr (D == 128) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(vp + 8 * g);
-                        w[k][0] = v.x, w[k][1] = v.y;
-                    } else {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
-                        w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
-                    }
-#pragma unroll
-                    for (int i = 0; i < kVS; i++)
-                        sc[k][i] = scales[L::kScales + r * (D / 16) + g * kE / 16 + i];
-                }
-                // Keys outside the piece hold anything: their values count as 0.  A NaN
-                // scale on a key that only some rows see must not reach the others
-                // as 0 * NaN: its values count as 0 here and are added below.
-                uint32_t nan_keys = 0;
-                if (edge) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int key = base + 16 * (y0 + y) + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
-                        const bool real = key >= lo_all && key <= kend;
-#pragma unroll
-                        for (int i = 0; i < kVS; i++) {
-                            const bool nan = (sc[k][i] & 0x7Fu) == 0x7Fu;
-                            if (nan && real) nan_keys |= 1u << (k * kVS + i);
-                            if (nan || !real) sc[k][i] = 0;
-                        }
-                    }
-                }
-                constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
-#pragma unroll
-                for (int i = 0; i < kVS; i++) {
-                    const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
-#pragma unroll
-                    for (int j = 0; j < kPer; j += 8) {
-                        const int word = (i * 16 + j) / 8;
-                        uint32_t even[2][4], odd[2][4];
-#pragma unroll
-                        for (int b = 0; b < 2; b++) {
-                            const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
-                            e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
-                            e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const uint4 a = make_uint4(mul_h2(even[0][e], f[0]), mul_h2(odd[0][e], f[0]),
-                                                       mul_h2(even[1][e], f[1]), mul_h2(odd[1][e], f[1]));
-#pragma unroll
-                            for (int n = 0; n < NT; n++) mma_f16(o[(i * 16 + j) / 2 + e][n], a, pt[y][n][0], pt[y][n][1]);
-                        }
-                    }
-                }
-                if (edge && __any_sync(0xffffffffu, nan_keys)) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const int last = x.hi[8 * n + g], lo = first_seen(p, last), hi = min(last, kend);
-                        uint32_t seen[2];
+                    for (int y = 0; y < 2; y++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const int a = base + 16 * (y0 + y) + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
-                            seen[h] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
+                            const int key = base + 16 * y + 8 * h + own_key;
+                            if (key < lo || key > hi) s[y][n][2 * h + i] = -INFINITY;
                         }
+                }
+        }
+        float m[NT][2];
+        bool grew = false;
 #pragma unroll
-                        for (int i = 0; i < kVS; i++) {
-                            uint32_t flag[2];
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int k = 0; k < 2; k++)
-                                flag[k] = h2_of(nan_keys >> (2 * k * kVS + i) & 1 ? 1.f : 0.f,
-                                                nan_keys >> ((2 * k + 1) * kVS + i) & 1 ? 1.f : 0.f);
-                            float v[4] = {};
-                            mma_f16(v, make_uint4(flag[0], flag[0], flag[1], flag[1]), seen[0], seen[1]);
+            for (int i = 0; i < 2; i++) {
+                m[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
+                m[n][i] = fmaxf(m[n][i], fmaxf(s[1][n][i], s[1][n][2 + i]));
+                m[n][i] *= i ? to_log2[n].y : to_log2[n].x;
+                grew |= m[n][i] > limit[n][i];
+            }
+        if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                            for (int j = 0; j < kPer / 2; j++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                                for (int c = 0; c < 4; c++)
-                                    if (v[c] > 0.f) o[i * 8 + j][n][c] = NAN;
-                        }
+                for (int i = 0; i < 2; i++) {
+                    const float top = limit[n][i] == -INFINITY ? -INFINITY : less[n][i];
+                    float v = fmaxf(m[n][i], top + kHeadroom);
+#pragma unroll
+                    for (int lanes = 4; lanes < 32; lanes *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, lanes));
+                    less[n][i] = v == -INFINITY ? 0.f : v - kHeadroom;
+                    // (past 2^26 the two sums round, together to as much as f16's end)
+                    limit[n][i] = v + kLag - less[n][i] > kLag + kHeadroom ? v : v + kLag;
+                    const float f = exp2f(top - less[n][i]);  // nothing to scale yet while top is -inf
+                    sum[n][i] *= f;
+#pragma unroll
+                    for (int j = 0; j < kTiles; j++) {
+                        o[j][n][i] *= f;
+                        o[j][n][2 + i] *= f;
+                    }
+                }
+        }
+        uint32_t pt[2][NT][2];  // P^T fragments
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    s[y][n][c] = exp2_fast(__fmaf_rn(s[y][n][c], c & 1 ? to_log2[n].y : to_log2[n].x, -less[n][c & 1]));
+                    sum[n][c & 1] += s[y][n][c];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;"
+                        : "=r"(pt[y][n][h])
+                        : "r"(h2_of(s[y][n][2 * h], s[y][n][2 * h + 1])));
+            }
+        // ---- values of the lane's four keys of each 16
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+            uint32_t w[4][(D / 16 + 3) / 4], sc[4][kVS];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int r = 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                const uint8_t *vp = blk + L::kCodes + r * (D / 2);
+                if constexpr (D == 64) {
+                    w[k][0] = *reinterpret_cast<const uint32_t *>(vp + 4 * g);
+                } else if constexpr (D == 128) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(vp + 8 * g);
+                    w[k][0] = v.x, w[k][1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(vp + 16 * g);
+                    w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+                }
+#pragma unroll
+                for (int i = 0; i < kVS; i++)
+                    sc[k][i] = scales[L::kScales + r * (D / 16) + g * kE / 16 + i];
+            }
+            // Keys outside the piece hold anything: their values count as 0.  A NaN
+            // scale on a key that only some rows see must not reach the others
+            // as 0 * NaN: its values count as 0 here and are added below.
+            uint32_t nan_keys = 0;
+            if (edge) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int key = base + 16 * y + 8 * (k >> 1) + ((2 * t + (k & 1)) ^ (t & 1));
+                    const bool real = key >= lo_all && key <= kend;
+#pragma unroll
+                    for (int i = 0; i < kVS; i++) {
+                        const bool nan = (sc[k][i] & 0x7Fu) == 0x7Fu;
+                        if (nan && real) nan_keys |= 1u << (k * kVS + i);
+                        if (nan || !real) sc[k][i] = 0;
+                    }
+                }
+            }
+            constexpr int kPer = kE < 16 ? kE : 16;  // elements under one scale here
+#pragma unroll
+            for (int i = 0; i < kVS; i++) {
+                const uint32_t f[2] = {e4m3x2_h2(sc[0][i] | sc[1][i] << 8), e4m3x2_h2(sc[2][i] | sc[3][i] << 8)};
+#pragma unroll
+                for (int j = 0; j < kPer; j += 8) {
+                    const int word = (i * 16 + j) / 8;
+                    uint32_t even[2][4], odd[2][4];
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const uint32_t u = w[2 * b][word], v = w[2 * b + 1][word];
+                        e2m1x8_h2((u & 0x0F0F0F0Fu) | (v << 4 & 0xF0F0F0F0u), even[b]);
+                        e2m1x8_h2((u >> 4 & 0x0F0F0F0Fu) | (v & 0xF0F0F0F0u), odd[b]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint4 a = make_uint4(mul_h2(even[0][e], f[0]), mul_h2(odd[0][e], f[0]),
+                                                   mul_h2(even[1][e], f[1]), mul_h2(odd[1][e], f[1]));
+#pragma unroll
+                        for (int n = 0; n < NT; n++) mma_f16(o[(i * 16 + j) / 2 + e][n], a, pt[y][n][0], pt[y][n][1]);
+                    }
+                }
+            }
+            if (edge && __any_sync(0xffffffffu, nan_keys)) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const int last = x.hi[8 * n + g], lo = first_seen(p, last), hi = min(last, kend);
+                    uint32_t seen[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int a = base + 16 * y + 8 * h + ((2 * t) ^ (t & 1)), b = a ^ 1;
+                        seen[h] = h2_of(a >= lo && a <= hi ? 1.f : 0.f, b >= lo && b <= hi ? 1.f : 0.f);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kVS; i++) {
+                        uint32_t flag[2];
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+                            flag[k] = h2_of(nan_keys >> (2 * k * kVS + i) & 1 ? 1.f : 0.f,
+                                            nan_keys >> ((2 * k + 1) * kVS + i) & 1 ? 1.f : 0.f);
+                        float v[4] = {};
+                        mma_f16(v, make_uint4(flag[0], flag[0], flag[1], flag[1]), seen[0], seen[1]);
+#pragma unroll
+                        for (int j = 0; j < kPer / 2; j++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++)
+                                if (v[c] > 0.f) o[i * 8 + j][n][c] = NAN;
                     }
                 }
             }
