@@ -1058,8 +1058,8 @@ __device__ __forceinline__ void join_warps(const AttendArgs &p, const Piece &x, 
         for (int i = 0; i < D / 32; i++) {
             v[i] = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; w++)
-                if (f[w] != 0.f) v[i] += f[w] * merge[(w * L::kRows + r) * L::kRow + L::place(lane + 32 * i)];
+            for (int w = 0; w < kAttnWarps; w++)  // (a factor that is 0 still passes on a NaN among the values)
+                v[i] += f[w] * merge[(w * L::kRows + r) * L::kRow + L::place(lane + 32 * i)];
         }
         if (part) {
 #pragma unroll
@@ -1324,7 +1324,7 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
 #pragma unroll
         for (int k = 0; k < kAtATime; k++) {
             const float f = part_factor(top[k], sum[k], n);
-            if (f == 0.f && sum[k] == sum[k]) continue;  // nothing, or too far below to count; a NaN goes on
+            if (top[k] == -INFINITY && sum[k] == 0.f) continue;  // nothing; what is too far below to count may be a NaN
             l += f * sum[k];
 #pragma unroll
             for (int e = 0; e < D / 32; e++) v[e] += f * o[k][e];
@@ -1347,7 +1347,7 @@ __global__ void __launch_bounds__(kJoinRows *kJoinWarps * 32) attend_join_kernel
         const float f = part_factor(tops[slot][w], sums[slot][w], m);
         l += f * sums[slot][w];
 #pragma unroll
-        for (int e = 0; e < D / 32; e++) v[e] += f == 0.f ? 0.f : f * o_of[slot][w][lane + 32 * e];
+        for (int e = 0; e < D / 32; e++) v[e] += f * o_of[slot][w][lane + 32 * e];
     }
     const int row = h.row0 + r;
     write_row<T, D>(p, h.head, p.cache.heads, h.first + row / p.group, row % p.group, m, l, v);
