@@ -15,10 +15,11 @@
 // both round to nearest even.  A NaN makes the block's scale NaN.
 //
 // Measured on one B200 (8 KV heads of 128, bf16, calls among others in a graph):
-// append of 16383 tokens with 32 query heads 72 us = 5.0 TB/s (bound by memory
-// latency), their read 15 us = 5.7 TB/s; a step of 32 tokens 4.5-5 us for both.
-// Attention of 64 sequences up to 8192 tokens, group 4: 72 us = 4.2 TB/s; of one
-// with 131071 tokens 46 us with pages of 64 = 3.3 TB/s, 52 us with pages of 16.
+// append of 16383 tokens with 32 query heads 71 us = 5.0 TB/s with neighbours
+// rotated, 83 with halves (bound by memory latency), their read 15 us = 5.7 TB/s; a
+// step of 32 tokens 4.5 us for both.  Attention of 64 sequences up to 8192 tokens,
+// group 4: 74 us = 4.1 TB/s; of one with 131071 tokens 46 us with pages of 64 = 3.3
+// TB/s, 52 us with pages of 16.
 
 #include "sm100.cuh"
 
@@ -78,8 +79,8 @@ struct AppendArgs {
 enum Rotation { kNoTurn, kHalves, kNeighbours, kMixed };
 
 // Heads whose loads are in flight together: two with a load for the partners
-// (halves of 128 elements, 16383 tokens: 106 us against 118 with four), else
-// four (neighbours: 93 us, 103 with two).
+// (halves, 16383 tokens of 32 + 8 + 8 heads of 128: append 83 us, 94 with four),
+// else four (neighbours: 71 us, 80 with two).
 template <Rotation R>
 constexpr int kBatch = R == kHalves || R == kMixed ? 2 : 4;
 
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(256) read_kernel(const Cache c, const int64_t 
 //
 // Bound: turning codes into operands.  Per 16 keys of D = 128 a warp issues about
 // 300 instructions, 64 conversions and 64 multiplications by the scale among
-// them; the issue slots are 62 %, the ALU pipe 50 %, memory 64 % busy, and 20
+// them; the issue slots are 62 %, the ALU pipe 50 %, memory 63 % busy, and 20
 // warps an SM (95 registers, 40 KB of shared memory a CTA) hide the rest.  With
 // few long sequences the two launches, the start and the join of the parts
 // take about 15 us beside the keys' time.

@@ -19,9 +19,9 @@
 //
 // Measured on one B200 (calls among others in a graph): [17408 x 5120], one
 // token 17.3 us = 5.2 TB/s of w; [5120 x 17408], 48 tokens with a residual
-// 21.8 us; [17408 x 5120], 8192 tokens with bias, GELU and a factor 547-582 us =
-// 2.5-2.7 PFLOP/s (a library e4m3 product without any epilogue: 493 us), 640-660
-// us in a loop of seconds, where the power limit sets the clock.
+// 21.5 us; [17408 x 5120], 8192 tokens with bias, GELU and a factor 544-582 us =
+// 2.5-2.7 PFLOP/s (a library e4m3 product without any epilogue: 493 us), 634-667
+// us in a loop of calls, where the power limit sets the clock.
 
 #include "sm100.cuh"
 

@@ -15,8 +15,9 @@
 // every input is read once and every output written once, so the kernel is
 // bound by memory for many rows and by launch and reduction latency for few.
 // Measured on one B200, residual and e4m3 output: 16384 x 5120 bf16 95 us =
-// 6.2 TB/s (95 % of the copy rate), 16384 x 5121 104 us; 1 x 5120 2.7 us among
-// others in a graph.
+// 6.2 TB/s (95 % of the copy rate), 16384 x 5121 102 us; 1 x 5120 2.7 us among
+// others in a graph.  e4m3 alone, without a norm: 16384 x 5120 57 us, 1 x 5120 2.7-3.0
+// us (2.2 with a factor in the divisions' place).
 // All loads of a row come before the first use of one: 135 us with the
 // residual's after the sums of x began.
 
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(kMost) norm_vec_kernel(const NormArgs p) {
 
 // Wider rows, and rows of tensors that lie to 16-byte boundaries each in its own
 // way: element by element, s * w kept in shared memory (1021 x 4099 f16: 9.7 us
-// out of L2, where vectors take 5.5; bound by its 2-byte accesses).
+// out of L2, where vectors take 5.3; bound by its 2-byte accesses).
 template <typename T, bool kNorm>
 __global__ void __launch_bounds__(1024) norm_any_kernel(const NormArgs p) {
     extern __shared__ float srow[];
@@ -284,7 +285,7 @@ int launch_norm(NormArgs p, int64_t rows, cudaStream_t st) {
     const bool alike = as_x(p.residual, p.r_stride) && as_x(p.h, p.h_stride) && as_x(p.y, p.cols);
     const bool vec = alike && p.cols % 8 == 0 && p.cols <= 32 * 1024 && is_aligned(p.x, 16) && p.x_stride % kPer == 0 &&
                      is_aligned(p.weight, 16) && is_aligned(p.q, 8);
-    // Otherwise by vectors all the same (1021 x 4099 f16, odd rows: 5.5 us, element by
+    // Otherwise by vectors all the same (1021 x 4099 f16, odd rows: 5.3 us, element by
     // element 9.7); the bytes of q then lie to boundaries of four as x's elements do.
     const bool shifted = alike && p.cols < 32 * 1024 + 8 && reinterpret_cast<uintptr_t>(p.x) % sizeof(T) == 0 &&
                          (!p.q || (is_aligned(p.q, 4) && is_aligned(p.x, 16) && (p.x_stride - p.cols) % kPer == 0));

@@ -128,12 +128,12 @@ def check(rc: int, lib: ctypes.CDLL | None = None) -> None:
         raise RuntimeError(msg or f"libtans_b200 error {rc}")
 
 
-_HERE = contextlib.nullcontext()
+_CURRENT = contextlib.nullcontext()
 
 
 def on_device(dev: torch.device):
     """A device guard for `dev`; nothing to enter where `dev` is already current."""
-    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+    return _CURRENT if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def raw_stream(dev: torch.device) -> int:
